@@ -438,6 +438,28 @@ int reskv_kmeans_incremental(const void* x, int batch, int kv_heads, int tokens,
                              const void* old_centroids, int old_clusters, void* new_centroids, int new_clusters,
                              int32_t* ids, void* stream);
 
+/* ---- attention over packed prompts ----------------------------------------------------------
+ * What the model integrations do with a prompt before it is compressed (the reference attends with
+ * the framework's own attention, reskv/models/llama.py:25-170), for prompts of different lengths that
+ * lie one behind the other: out[i,h] = sum_j softmax_j(q[i,h].k[j,g] * scaling) v[j,g] over the tokens j of
+ * i's sequence, up to i itself if causal != 0; g = h / (q_heads / kv_heads), at most 128 query heads per
+ * KV head.
+ *
+ *   q            f16 (bf16 != 0: bf16) [total, q_heads, 128], k and v [total, kv_heads, 128]; rows of 128
+ *                dense, *_token / *_head elements between tokens / heads (positive multiples of 8), on
+ *                16-byte boundaries
+ *   cu_seqlens   i32 [sequences + 1] in device memory: sequence s holds tokens [cu[s], cu[s+1]); clamped to
+ *                [0, total], lengths may be 0
+ *   out          [total, q_heads, 128] of the same type, 16-byte aligned, lse f32 [total, q_heads] or NULL:
+ *                log of the sum of exponentials.  Rows of no sequence are left as they are.
+ * reskv_prompt_attention_status: RESKV_STATUS_* bits of all calls on the device so far (copies four bytes
+ * to the host and synchronises `stream`). */
+int reskv_prompt_attention(const void* q, const void* k, const void* v, const int32_t* cu_seqlens, int sequences, int total,
+                           int kv_heads, int q_heads, int bf16, int64_t q_token, int64_t q_head, int64_t k_token,
+                           int64_t k_head, int64_t v_token, int64_t v_head, float scaling, int causal, void* out, float* lse,
+                           void* stream);
+int reskv_prompt_attention_status(uint32_t* status, void* stream);
+
 /* ---- test and profiling hooks ---------------------------------------------------------
  * NOT part of the surface a production host binds: both calls set process-wide state without any
  * synchronisation (they change what every thread's next decode call does) and exist for the test suite

@@ -9,7 +9,7 @@ on first use.
 from .config import KernelPlan, ResKVConfig, ResKVKernelConfig
 
 __version__ = "0.1.0"
-__all__ = ["ResKVKernelConfig", "ResKVForCausalLM", "ResKVConfig", "KernelPlan", "compress", "attention"]
+__all__ = ["ResKVKernelConfig", "ResKVForCausalLM", "ResKVConfig", "KernelPlan", "compress", "attention", "prompt_attention"]
 
 
 def __getattr__(name):
@@ -21,6 +21,10 @@ def __getattr__(name):
         from ._attention import attention
 
         return attention
+    if name == "prompt_attention":
+        from .prompt import prompt_attention
+
+        return prompt_attention
     if name == "ResKVForCausalLM":  # needs transformers: imported on first use (reference __init__.py:18-21)
         from .models.hf_llama import ResKVForCausalLM
 

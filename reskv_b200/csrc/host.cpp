@@ -819,12 +819,84 @@ PyObject* py_ids_in_range(PyObject*, PyObject* ticket) {
     });
 }
 
+// ---- packed prompts ---------------------------------------------------------------------------------------------------
+// x[T,H,128] as the kernels read it: dense rows, strides of whole 16-byte pieces.  Anything else is copied.
+at::Tensor packed_rows(const at::Tensor& x) {
+    const bool fits = x.stride(2) == 1 && aligned16(x.const_data_ptr()) && (x.size(0) == 1 || (x.stride(0) > 0 && x.stride(0) % 8 == 0)) &&
+                      (x.size(1) == 1 || (x.stride(1) > 0 && x.stride(1) % 8 == 0)) && !x.is_neg();
+    return fits ? x : x.is_contiguous() ? x.clone() : x.contiguous();  // a dense tensor off a 16-byte boundary is moved
+}
+int64_t token_step(const at::Tensor& x) { return x.size(0) == 1 ? x.size(1) * 128 : x.stride(0); }
+int64_t head_step(const at::Tensor& x) { return x.size(1) == 1 ? 128 : x.stride(1); }
+
+// prompt_attention(query, key, value, cu_seqlens, scaling, causal, out, return_lse) -> out or (out, lse)
+PyObject* py_prompt_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        expect(n, 8);
+        at::Tensor x[3] = {tensor(o[0], "query"), tensor(o[1], "key"), tensor(o[2], "value")};
+        const at::Tensor cu = tensor(o[3], "cu_seqlens");
+        const double scaling = o[4] == Py_None ? 0.08838834764831845 : number(o[4]);  // 128 ** -0.5
+        const bool causal = o[5] == Py_True, stats = o[7] == Py_True;
+        at::Tensor out = optional_tensor(o[6], "out"), lse;
+        const at::ScalarType type = x[0].scalar_type();
+        for (const at::Tensor& t : x)
+            if (t.dim() != 3 || t.size(2) != 128 || t.scalar_type() != type || (type != at::kHalf && type != at::kBFloat16) || !t.is_cuda())
+                value_error("query, key and value must be FP16 or BF16 CUDA [tokens, heads, 128] of one type");
+        const int64_t total = x[0].size(0), nh = x[0].size(1), kh = x[1].size(1);
+        if (x[1].size(0) != total || x[1].sizes() != x[2].sizes()) value_error("query, key and value must have the same tokens, key and value the same heads");
+        if (kh < 1 || nh < 1 || nh % kh || nh / kh > 128) value_error("query heads must be a multiple of the KV heads, at most 128 per KV head");
+        if (total > 0x7fffffff) value_error("too many tokens for one call");
+        const c10::DeviceIndex dev = x[0].get_device();
+        for (const at::Tensor& t : {x[1], x[2], cu, out}) same_device(dev, t);
+        if (cu.dim() != 1 || cu.size(0) < 1 || cu.scalar_type() != at::kInt || cu.size(0) > 0x7fffffff)
+            value_error("cu_seqlens must be int32 [sequences + 1]");
+        if (!(scaling > 0.0) || !(scaling < 3.0e38)) value_error("scaling must be positive and finite");
+        if (out.defined() && (out.sizes() != x[0].sizes() || out.scalar_type() != type || !out.is_contiguous() || !aligned16(out.const_data_ptr())))
+            value_error("out must be contiguous, of the query's shape and type, on a 16-byte boundary");
+        if (c10::GradMode::is_enabled() && (x[0].requires_grad() || x[1].requires_grad() || x[2].requires_grad() || (out.defined() && out.requires_grad())))
+            value_error("prompt_attention is inference only: call it under torch.no_grad()");
+        {
+            const Unlocked free;
+            const at::AutoDispatchBelowADInplaceOrView plain;
+            const c10::cuda::CUDAGuard guard(dev);
+            if (!out.defined()) out = at::detail::empty_cuda({total, nh, 128}, type, x[0].device(), std::nullopt);
+            if (stats) lse = at::detail::empty_cuda({total, nh}, at::kFloat, x[0].device(), std::nullopt);
+            if (total > 0) {
+                for (at::Tensor& t : x) t = packed_rows(t);
+                const at::Tensor ends = cu.contiguous();
+                check(reskv_prompt_attention(x[0].const_data_ptr(), x[1].const_data_ptr(), x[2].const_data_ptr(),
+                                             static_cast<const int32_t*>(ends.const_data_ptr()), static_cast<int>(ends.size(0) - 1),
+                                             static_cast<int>(total), static_cast<int>(kh), static_cast<int>(nh), type == at::kBFloat16,
+                                             token_step(x[0]), head_step(x[0]), token_step(x[1]), head_step(x[1]), token_step(x[2]),
+                                             head_step(x[2]), static_cast<float>(scaling), causal, out.data_ptr(),
+                                             stats ? static_cast<float*>(lse.data_ptr()) : nullptr,
+                                             c10::cuda::getCurrentCUDAStream(dev).stream()));
+                if (ends.size(0) > 1) ++g_launches;
+                if (g_check_status) {
+                    uint32_t status = 0;
+                    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+                    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+                    check_cuda(cudaStreamIsCapturing(stream, &capture), "cudaStreamIsCapturing");
+                    if (capture == cudaStreamCaptureStatusNone) check(reskv_prompt_attention_status(&status, stream));
+                    if (status) throw Failure{PyExc_RuntimeError, "prompt_attention: a bounded wait ran out on the device"};
+                }
+            }
+        }
+        if (!stats) return THPVariable_Wrap(out);
+        PyObject* t = PyTuple_New(2);
+        PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(out));
+        PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(lse));
+        return t;
+    });
+}
+
 PyObject* py_launches(PyObject*, PyObject*) { return PyLong_FromLongLong(g_launches); }
 
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f))
 PyMethodDef g_methods[] = {
     {"decode", FAST(py_decode), METH_FASTCALL, "decode attention on given operands"},
     {"attention", FAST(py_attention), METH_FASTCALL, "decode attention on a compressed cache"},
+    {"prompt_attention", FAST(py_prompt_attention), METH_FASTCALL, "attention over packed prompts"},
     {"window_append", FAST(py_window_append), METH_FASTCALL, "append one token to the dense window"},
     {"encode", FAST(py_encode), METH_FASTCALL, "pack one side"},
     {"kmeans_pair", FAST(py_kmeans_pair), METH_FASTCALL, "cluster K and V in the same launch"},

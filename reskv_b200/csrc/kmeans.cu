@@ -30,6 +30,7 @@
 #include "common.cuh"
 #include "tensor_map.cuh"
 #include "tmem.cuh"
+#include "umma.cuh"
 
 namespace reskv {
 namespace {
@@ -514,41 +515,8 @@ constexpr int kUSumBuffers = 4;                // tile i of a segment adds to ac
 constexpr int kURun = 2;                       // segments of a unit that a CTA takes without a stop, accumulators of their own
 constexpr int kUChunkMax = 8192;               // most tokens per CTA (2048 per accumulator)
 
-// Shared-memory matrix descriptor, 128-byte swizzle, address bits [4, 18), leading / stride byte offsets.
-__device__ __forceinline__ uint64_t umma_desc(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
-    return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(lbo_bytes >> 4) << 16) |
-           (static_cast<uint64_t>(sbo_bytes >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-
-// FP16 x FP16 -> FP32, M = 128, N = n; a_mn: A is MN-major (the token tile read transposed).
-__host__ __device__ constexpr uint32_t umma_idesc(int n, bool a_mn) {
-    return (1u << 4) | (a_mn ? (1u << 15) : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
-}
-
-__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-// One arrival on `bar` once every MMA issued so far by the calling thread has completed.
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
 // Byte offset of 16-byte piece `piece` (0..7) of row `row` in a [rows][128 B] block with the 128-byte swizzle.
 __device__ __forceinline__ uint32_t sw128(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
-
-// True in exactly one lane of a converged warp (the same lane every time).
-__device__ __forceinline__ bool elect_one() {
-    uint32_t chosen;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(chosen));
-    return chosen != 0;
-}
 
 constexpr int kUWorkers = kUThreads - 32;  // everyone but the copying warp: these meet at the segment boundaries
 

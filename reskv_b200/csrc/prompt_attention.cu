@@ -1,0 +1,545 @@
+// Attention over whole prompts that lie one behind the other in packed tensors: for token i of a sequence and every query
+// head, out_i = sum_j softmax_j(q_i . k_j * scaling) v_j over the keys j <= i (causal) or over all keys of the sequence.
+#include <cuda_bf16.h>
+
+#include "tensor_map.cuh"
+#include "tmem.cuh"
+#include "umma.cuh"
+
+namespace reskv {
+namespace {
+
+constexpr int kPKeys = 128;                     // keys of a tile
+constexpr int kPHalf = 128 * 128;               // bytes of 128 rows x 64 coordinates
+constexpr int kPTile = 2 * kPHalf;              // 128 rows of 128 coordinates
+constexpr int kPStages = 5;                     // ring of K and V tiles
+constexpr int kPThreads = 384;                  // two softmax warpgroups; MMA warp, copying warp and two that idle
+// A row of scores is 128 registers of its thread.  The launch gives 168 a thread (the most for 384); the last warpgroup hands
+// back what the softmax warpgroups take: 2 x 208 + 88 = 3 x 168.
+constexpr int kPLaunchRegs = 168, kPSoftmaxRegs = 208, kPOtherRegs = 88;
+static_assert(2 * kPSoftmaxRegs + kPOtherRegs <= 3 * kPLaunchRegs, "the shares come out of the launch's registers");
+constexpr int kPSmem = 2 * kPTile + kPStages * kPTile + 1024;  // + room to start on a 1024-byte boundary
+constexpr uint32_t kPColS = 0, kPColO = 256;    // tensor memory: scores 2 x 128 columns, outputs 2 x 128
+constexpr float kPSlack = 8.f;                  // the running maximum lags by at most this (in powers of two)
+
+__device__ uint32_t g_prompt_status;  // RESKV_STATUS_* bits
+
+struct PromptParams {
+    const int* cu;      // [sequences + 1]
+    int sequences, total, kv_heads, group, tile_tokens;  // tile_tokens: tokens of 128 rows
+    const unsigned short* v;      // the values once more, for the outputs that infinities and NaN reach
+    int64_t v_token, v_head;      // elements between its tokens and heads
+    void* out;          // [total, query heads, 128]
+    float* lse;         // [total, query heads] or null
+    float scale_log2;
+    int causal;
+};
+
+// A work item: two row tiles of one sequence and KV head.
+struct PromptItem {
+    int start, len, token0, head, tiles0, tiles1;  // tiles0 / tiles1: key tiles that the first / second row tile needs
+};
+
+__device__ __forceinline__ int clamped(int x, int low, int high) { return x < low ? low : x > high ? high : x; }
+
+struct SequenceSpan {
+    int start, len;
+};
+__device__ __forceinline__ SequenceSpan span_of(const PromptParams& p, int s) {
+    const int a = clamped(p.cu[s], 0, p.total), b = clamped(p.cu[s + 1], a, p.total);
+    return {a, b - a};
+}
+
+// Number of (sequence, pair of row tiles) whose place in the sequence is `level` or behind it; whole warp.
+__device__ __forceinline__ int pairs_from(const PromptParams& p, int level, int lane) {
+    const int pair = 2 * p.tile_tokens;
+    int n = 0;
+    for (int s = lane; s < p.sequences; s += 32) {
+        const int tiles = (span_of(p, s).len + pair - 1) / pair;
+        n += tiles > level ? tiles - level : 0;
+    }
+    return __reduce_add_sync(0xffffffffu, n);
+}
+
+// Item `index`, items ordered by their place in their sequence, last ones first: with causal attention the longest ones.
+// tiles0 = 0 in the result: there is none.  Whole warp.
+__device__ PromptItem find_item(const PromptParams& p, int index, int lane) {
+    PromptItem it{};
+    const int pos = index / p.kv_heads, pair = 2 * p.tile_tokens;
+    int low = 0, high = (p.total + pair - 1) / pair;
+    if (pairs_from(p, 0, lane) <= pos) return it;
+    while (high - low > 1) {
+        const int mid = (low + high) >> 1;
+        if (pairs_from(p, mid, lane) > pos) low = mid; else high = mid;
+    }
+    int rest = pos - pairs_from(p, low + 1, lane);
+    for (int s0 = 0; s0 < p.sequences; s0 += 32) {
+        const SequenceSpan sp = s0 + lane < p.sequences ? span_of(p, s0 + lane) : SequenceSpan{0, 0};
+        const bool has = sp.len > low * pair;
+        const uint32_t mask = __ballot_sync(0xffffffffu, has);
+        const int count = __popc(mask);
+        if (rest >= count) {
+            rest -= count;
+            continue;
+        }
+        const int owner = __ffs(__ballot_sync(0xffffffffu, has && __popc(mask & ((1u << lane) - 1u)) == rest)) - 1;
+        it.start = __shfl_sync(0xffffffffu, sp.start, owner);
+        it.len = __shfl_sync(0xffffffffu, sp.len, owner);
+        it.head = index % p.kv_heads;
+        it.token0 = low * pair;
+        const int end0 = min(it.token0 + p.tile_tokens, it.len), end1 = min(it.token0 + pair, it.len);
+        it.tiles0 = ((p.causal ? end0 : it.len) + kPKeys - 1) / kPKeys;
+        it.tiles1 = end1 <= it.token0 + p.tile_tokens ? 0 : ((p.causal ? end1 : it.len) + kPKeys - 1) / kPKeys;
+        return it;
+    }
+    return it;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if (BF16)
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+template <bool BF16>
+__device__ __forceinline__ float unpack(unsigned short bits) {
+    return BF16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16) : __half2float(__ushort_as_half(bits));
+}
+
+// Whether one of the two 16-bit numbers is infinite or NaN.
+template <bool BF16>
+__device__ __forceinline__ bool non_finite(unsigned short bits) {
+    constexpr unsigned short mask = BF16 ? 0x7F80 : 0x7C00;
+    return (bits & mask) == mask;
+}
+
+// A value row (128 coordinates in two halves of 128 bytes) that some row of the tile may not see: `drop` clears it (a token
+// behind the sequence), otherwise its infinities and NaN are cleared, because a weight of 0 does not silence them.  The 16-byte
+// pieces are taken in an order that keeps the lanes on different banks.  Returns whether something non-finite was there.
+template <bool BF16>
+__device__ __forceinline__ bool tame_value_row(unsigned char* row, bool drop, int lane) {
+    uint32_t seen = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            uint4* at = reinterpret_cast<uint4*>(row + h * kPHalf + (((i + lane) & 7) << 4));
+            if (drop) {
+                *at = make_uint4(0, 0, 0, 0);
+            } else {
+                const uint4 v = *at;
+                constexpr uint32_t mask = BF16 ? 0x7F807F80u : 0x7C007C00u, one = BF16 ? 0x00800080u : 0x04000400u;
+                seen |= ((v.x & mask) + one) | ((v.y & mask) + one) | ((v.z & mask) + one) | ((v.w & mask) + one);
+            }
+        }
+    if (drop || !(seen & 0x80008000u)) return false;
+    for (int h = 0; h < 2; ++h)
+        for (int i = 0; i < 64; ++i) {
+            unsigned short* at = reinterpret_cast<unsigned short*>(row + h * kPHalf) + i;
+            if (non_finite<BF16>(*at)) *at = 0;
+        }
+    return true;
+}
+
+struct __align__(16) PromptShared {
+    uint64_t kv_full[kPStages], kv_empty[kPStages];
+    uint64_t q_full, q_empty, s_full[2], p_ready[2][2], o_done[2], item_full[2], item_empty[2], cancel;
+    uint4 cancel_reply;
+    PromptItem item[2];
+    int tamed[2];   // of an item: infinities or NaN were cleared in a tile of values
+    uint32_t tmem;
+};
+
+__device__ __forceinline__ bool wait_once(bool& lost, uint64_t* bar, uint32_t parity) {
+    if (!lost) lost = !mbar_wait(bar, parity);
+    return !lost;
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(kPThreads, 1)
+prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                        const __grid_constant__ CUtensorMap v_map) {
+    extern __shared__ unsigned char raw[];
+    __shared__ PromptShared sh;
+    unsigned char* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    unsigned char* qs = smem;                 // two row tiles
+    unsigned char* ring = smem + 2 * kPTile;  // K0 V0 K1 V1 ...
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rows = p.tile_tokens * p.group;
+    if (tid == 0) {
+        for (int s = 0; s < kPStages; ++s) mbar_init(&sh.kv_full[s], 1), mbar_init(&sh.kv_empty[s], 1);
+        mbar_init(&sh.q_full, 1), mbar_init(&sh.q_empty, 1), mbar_init(&sh.cancel, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.s_full[i], 1), mbar_init(&sh.o_done[i], 1);
+            mbar_init(&sh.p_ready[i][0], 128), mbar_init(&sh.p_ready[i][1], 128);
+            mbar_init(&sh.item_full[i], 1), mbar_init(&sh.item_empty[i], 257);  // softmax threads, MMA warp
+        }
+        mbar_fence_init();
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    bool lost = false;
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPOtherRegs));
+        if (warp == 9) {
+            // ---- copies, and the next item: the grid has a CTA for every item that there may be, and a CTA that has finished takes
+            // over one that has not started yet -------------------------------------------------------------------------------
+            int index = blockIdx.x, tile = 0;
+            for (int n = 0;; ++n) {
+                const int slot = n & 1;
+                const PromptItem it = find_item(p, index, lane);
+                if (n >= 2) wait_once(lost, &sh.item_empty[slot], ((n >> 1) - 1) & 1);
+                if (lane == 0) {
+                    sh.item[slot] = it;
+                    if (lost) sh.item[slot].tiles0 = 0;
+                    sh.tamed[slot] = 0;
+                    mbar_arrive(&sh.item_full[slot]);
+                }
+                if (it.tiles0 == 0 || lost) break;
+                if (n > 0) wait_once(lost, &sh.q_empty, (n - 1) & 1);
+                const int kv_tiles = max(it.tiles0, it.tiles1), row_tiles = it.tiles1 ? 2 : 1;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&sh.cancel, 16);
+                    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                                     smem_u32(&sh.cancel_reply)),
+                                 "r"(smem_u32(&sh.cancel))
+                                 : "memory");
+                    mbar_arrive_expect_tx(&sh.q_full, row_tiles * rows * 256);
+                    for (int i = 0; i < row_tiles; ++i)
+                        for (int h = 0; h < 2; ++h)
+                            tma_load_3d(qs + i * kPTile + h * kPHalf, &q_map, 64 * h, it.head * p.group, it.start + it.token0 + i * p.tile_tokens,
+                                        &sh.q_full);
+                }
+                for (int j = 0; j < 2 * kv_tiles; ++j, ++tile) {
+                    const int stage = tile % kPStages;
+                    if (tile >= kPStages) wait_once(lost, &sh.kv_empty[stage], (tile / kPStages - 1) & 1);
+                    if (lost) break;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&sh.kv_full[stage], kPTile);
+                        for (int h = 0; h < 2; ++h)
+                            tma_load_3d(ring + stage * kPTile + h * kPHalf, j & 1 ? &v_map : &k_map, 64 * h, it.head,
+                                        it.start + (j >> 1) * kPKeys, &sh.kv_full[stage]);
+                    }
+                    __syncwarp();
+                }
+                wait_once(lost, &sh.cancel, n & 1);
+                uint32_t taken, first;
+                asm volatile(
+                    "{\n\t.reg .b128 reply;\n\t.reg .pred p;\n\t"
+                    "ld.shared.b128 reply, [%2];\n\t"
+                    "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, reply;\n\t"
+                    "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+                    "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, reply;\n\t}"
+                    : "=r"(taken), "=r"(first)
+                    : "r"(smem_u32(&sh.cancel_reply))
+                    : "memory");
+                proxy_fence();  // the reply has been read before the next one is asked for
+                __syncwarp();
+                index = taken && !lost ? static_cast<int>(first) : 0x7fffffff;
+            }
+            if (lost) {  // no copy may land after the block's end
+                for (int t = tile > kPStages ? tile - kPStages : 0; t < tile; ++t) mbar_wait(&sh.kv_full[t % kPStages], (t / kPStages) & 1);
+            }
+        } else if (warp == 8) {
+            // ---- MMAs: per key tile and row tile scores = Q K^T, output += P V; the scores of the next key tile follow the output
+            // in turn, so a row tile's softmax runs beside the other's products -----------------------------------------------
+            const uint32_t score_idesc = umma_idesc(128, false, false, BF16), value_idesc = umma_idesc(128, false, true, BF16);
+            const uint64_t q0 = umma_desc(smem_u32(qs), 16, 1024), k0 = umma_desc(smem_u32(ring), 16, 1024);
+            const uint64_t v0 = umma_desc(smem_u32(ring), kPHalf, 1024);
+            int tile = 0;  // place in the ring
+            uint32_t made[2] = {0, 0};
+            const auto scores = [&](int i, int stage) {
+                if (elect_one()) {
+    #pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint64_t step = static_cast<uint64_t>(((ks >> 2) * kPHalf + (ks & 3) * 32) >> 4);
+                        umma_f16(tmem + kPColS + i * 128, q0 + static_cast<uint64_t>((i * kPTile) >> 4) + step,
+                                 k0 + static_cast<uint64_t>((stage * kPTile) >> 4) + step, score_idesc, ks > 0);
+                    }
+                    umma_commit(&sh.s_full[i]);
+                }
+                __syncwarp();
+            };
+            const auto values = [&](int i, int stage, int half, bool first) {
+                if (elect_one()) {
+    #pragma unroll
+                    for (int k4 = 0; k4 < 4; ++k4) {
+                        const int ks = half * 4 + k4;
+                        umma_f16_ta(tmem + kPColO + i * 128, tmem + kPColS + i * 128 + ks * 8,
+                                    v0 + static_cast<uint64_t>((stage * kPTile + ks * 2048) >> 4), value_idesc, !first || ks > 0);
+                    }
+                }
+                __syncwarp();
+            };
+            const auto commit = [&](uint64_t* bar) {
+                if (elect_one()) umma_commit(bar);
+                __syncwarp();
+            };
+            for (int n = 0;; ++n) {
+                const int slot = n & 1;
+                wait_once(lost, &sh.item_full[slot], (n >> 1) & 1);
+                const PromptItem it = sh.item[slot];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.item_empty[slot]);
+                if (it.tiles0 == 0 || lost) break;
+                const int kv_tiles = max(it.tiles0, it.tiles1);
+                wait_once(lost, &sh.q_full, n & 1);
+                wait_once(lost, &sh.kv_full[tile % kPStages], (tile / kPStages) & 1);
+                tc_fence_after();
+                scores(0, tile % kPStages);
+                if (it.tiles1) scores(1, tile % kPStages);
+                commit(&sh.kv_empty[tile % kPStages]);
+                if (kv_tiles == 1) commit(&sh.q_empty);
+                for (int j = 0; j < kv_tiles; ++j) {
+                    const int vt = tile + 2 * j + 1, kt = vt + 1, v_stage = vt % kPStages, k_stage = kt % kPStages;
+                    const bool more = j + 1 < kv_tiles;
+                    wait_once(lost, &sh.kv_full[v_stage], (vt / kPStages) & 1);
+                    if (more) wait_once(lost, &sh.kv_full[k_stage], (kt / kPStages) & 1);
+                    for (int i = 0; i < 2; ++i) {
+                        const int tiles = i ? it.tiles1 : it.tiles0;
+                        if (j >= tiles) continue;
+    #pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            wait_once(lost, &sh.p_ready[i][half], made[i] & 1);
+                            tc_fence_after();
+                            values(i, v_stage, half, j == 0);
+                        }
+                        ++made[i];
+                        if (j + 1 < tiles) scores(i, k_stage); else commit(&sh.o_done[i]);
+                    }
+                    commit(&sh.kv_empty[v_stage]);
+                    if (more) commit(&sh.kv_empty[k_stage]);
+                    if (j + 2 == kv_tiles) commit(&sh.q_empty);
+                }
+                tile += 2 * kv_tiles;
+            }
+            if (tile > 0) wait_once(lost, &sh.kv_empty[(tile - 1) % kPStages], ((tile - 1) / kPStages) & 1);  // the last commit has arrived
+        }
+    } else {
+        // ---- softmax and output: thread = row -----------------------------------------------------------------------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPSoftmaxRegs));
+        const int i = warp >> 2, row = tid & 127;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + lanes + kPColS + i * 128, o_at = tmem + lanes + kPColO + i * 128;
+        const int row_token = row / p.group, row_head = row - row_token * p.group;
+        const float scale = p.scale_log2, slack = kPSlack / scale;
+        uint32_t seen = 0, items = 0;
+        int tile = 0;
+        for (int n = 0;; ++n) {
+            const int slot = n & 1;
+            wait_once(lost, &sh.item_full[slot], (n >> 1) & 1);
+            const PromptItem it = sh.item[slot];
+            if (it.tiles0 == 0 || lost) break;
+            const int tiles = i ? it.tiles1 : it.tiles0, other = i ? it.tiles0 : it.tiles1;
+            const int first_token = it.token0 + i * p.tile_tokens, token = first_token + row_token;
+            const int limit = p.causal ? token : it.len - 1;  // last key that the row sees
+            float m = 0.f, l = 0.f;
+            for (int j = 0; j < tiles; ++j) {
+                wait_once(lost, &sh.s_full[i], seen & 1);
+                ++seen;
+                tc_fence_after();
+                float s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(s_at + c * 32, s[c]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld_wait(s[c]);
+                const bool masked = j * kPKeys + kPKeys > it.len || (p.causal && j * kPKeys + kPKeys - 1 > first_token);
+                if (masked) {
+                    const int last = limit - j * kPKeys;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) s[c][e] = c * 32 + e <= last ? s[c][e] : -INFINITY;
+                }
+                float top[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    top[c] = max_nan(s[c][0], s[c][1]);
+#pragma unroll
+                    for (int e = 2; e < 32; e += 2) top[c] = max3_nan(top[c], s[c][e], s[c][e + 1]);
+                }
+                const float most = max3_nan(max_nan(top[0], top[1]), top[2], top[3]);
+                if (j == 0) {
+                    m = most;
+                } else {
+                    // the output so far is at rest: the scores at hand were committed behind the last product
+                    const bool grows = !(most <= m + slack);
+                    if (__any_sync(0xffffffffu, grows)) {
+                        const float next = grows ? max_nan(m, most) : m, factor = grows ? fast_exp2((m - next) * scale) : 1.f;
+                        m = next, l *= factor;
+#pragma unroll 1
+                        for (int c = 0; c < 4; ++c) {
+                            float o[32];
+                            tmem_ld32(o_at + c * 32, o);
+                            tmem_ld_wait(o);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] *= factor;
+                            tmem_st32(o_at + c * 32, o);
+                        }
+                    }
+                }
+                // an infinite maximum: inf - inf, NaN for the whole row as in the formula
+                const float shift = m == INFINITY ? __int_as_float(0x7fffffff) : -m * scale;
+                float sum[2] = {0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float packed[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float a = fast_exp2(fmaf(s[c][e], scale, shift)), b = fast_exp2(fmaf(s[c][e + 1], scale, shift));
+                        sum[0] += a, sum[1] += b;
+                        packed[e / 2] = __uint_as_float(pack2<BF16>(a, b));
+                    }
+                    tmem_st16(s_at + c * 16, packed);
+                    if (c == 1) {
+                        tmem_st_wait();
+                        if (masked && (i == 0 || j >= other)) {
+                            const int vt = tile + 2 * j + 1, stage = vt % kPStages;
+                            wait_once(lost, &sh.kv_full[stage], (vt / kPStages) & 1);
+                            const bool behind = j * kPKeys + row >= it.len;
+                            if ((behind || p.causal) && tame_value_row<BF16>(ring + stage * kPTile + row * 128, behind, lane)) sh.tamed[slot] = 1;
+                            proxy_fence();
+                        }
+                        tc_fence_before();
+                        mbar_arrive(&sh.p_ready[i][0]);
+                    }
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&sh.p_ready[i][1]);
+                l += sum[0] + sum[1];
+            }
+            if (tiles) {
+                wait_once(lost, &sh.o_done[i], items & 1);
+                ++items;
+                tc_fence_after();
+                const bool live = row < rows && token < it.len && !lost;
+                const bool tamed = *static_cast<volatile int*>(&sh.tamed[slot]) != 0;
+                const int64_t at = (static_cast<int64_t>(it.start + token) * p.kv_heads + it.head) * p.group + row_head;
+                const float inv = 1.f / l;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    float o[32];
+                    tmem_ld32(o_at + c * 32, o);
+                    tmem_ld_wait(o);
+                    if (tamed && live) {  // what was cleared reaches the rows that see it
+                        for (int key = it.token0 / kPKeys * kPKeys; key <= limit; ++key) {
+                            const unsigned short* from = p.v + (it.start + key) * p.v_token + it.head * p.v_head + c * 32;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (non_finite<BF16>(from[e])) o[e] += unpack<BF16>(from[e]);
+                        }
+                    }
+                    if (live) {
+                        uint4* to = reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.out) + at * 128 + c * 32);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8)
+                            to[e / 8] = make_uint4(pack2<BF16>(o[e] * inv, o[e + 1] * inv), pack2<BF16>(o[e + 2] * inv, o[e + 3] * inv),
+                                                   pack2<BF16>(o[e + 4] * inv, o[e + 5] * inv), pack2<BF16>(o[e + 6] * inv, o[e + 7] * inv));
+                    }
+                }
+                tc_fence_before();
+                if (live && p.lse) p.lse[at] = m * scale * kLn2 + logf(l);
+            }
+            tile += 2 * max(it.tiles0, it.tiles1);
+            mbar_arrive(&sh.item_empty[slot]);
+        }
+    }
+    if (lost) atomicOr(&g_prompt_status, RESKV_STATUS_WAIT_TIMEOUT);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+int check_rows(const char* what, const void* x, int64_t token, int64_t head) {
+    if (!aligned16(x) || token % 8 || head % 8 || token <= 0 || head <= 0)
+        return fail(RESKV_ERR_INVALID, "prompt_attention: %s must start on a 16-byte boundary, its strides be positive multiples of 8 elements", what);
+    return check_device_pointer(x, "prompt_attention", what);
+}
+
+int rows_map(CUtensorMap* map, const void* x, int heads, int total, int64_t token, int64_t head, int box_heads, int box_tokens) {
+    const cuuint64_t dims[3] = {kHeadDim, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(total)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head) * 2, static_cast<cuuint64_t>(token) * 2};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+    return encode_tensor_map(map, x, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, "prompt_attention");
+}
+
+template <bool BF16>
+int launch(const PromptParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, unsigned items, cudaStream_t stream) {
+    static std::atomic<unsigned long long> done{0};
+    static const int registers = [] {
+        cudaFuncAttributes a{};
+        return cudaFuncGetAttributes(&a, prompt_attention_kernel<BF16>) == cudaSuccess ? a.numRegs : 0;
+    }();
+    if (registers != kPLaunchRegs)  // the softmax warps would wait for registers that nobody hands back
+        return fail(RESKV_ERR_CUDA, "prompt_attention: built with %d registers a thread, not %d", registers, kPLaunchRegs);
+    if (int rc = allow_smem(prompt_attention_kernel<BF16>, kPSmem, done, "cudaFuncSetAttribute(prompt_attention)")) return rc;
+    return check_cuda(launch_overlapped(prompt_attention_kernel<BF16>, dim3(items), kPThreads, kPSmem, stream, false, p, q, k, v),
+                      "prompt_attention launch");
+}
+
+}  // namespace
+}  // namespace reskv
+
+using namespace reskv;
+
+extern "C" int reskv_prompt_attention(const void* q, const void* k, const void* v, const int32_t* cu_seqlens, int sequences, int total,
+                                      int kv_heads, int q_heads, int bf16, int64_t q_token, int64_t q_head, int64_t k_token,
+                                      int64_t k_head, int64_t v_token, int64_t v_head, float scaling, int causal, void* out, float* lse,
+                                      void* stream) {
+    if (sequences < 0 || total < 0 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads)
+        return fail(RESKV_ERR_INVALID, "prompt_attention: %d sequences, %d tokens, %d query and %d KV heads", sequences, total, q_heads, kv_heads);
+    if (q_heads / kv_heads > 128) return fail(RESKV_ERR_LIMIT, "prompt_attention: more than 128 query heads per KV head");
+    if (!(scaling > 0.f) || !(scaling < 3.0e38f)) return fail(RESKV_ERR_INVALID, "prompt_attention: scaling must be positive and finite");
+    if (sequences == 0 || total == 0) return RESKV_OK;
+    if (!q || !k || !v || !cu_seqlens || !out) return fail(RESKV_ERR_INVALID, "prompt_attention: null pointer");
+    if (int rc = check_rows("q", q, q_token, q_head)) return rc;
+    if (int rc = check_rows("k", k, k_token, k_head)) return rc;
+    if (int rc = check_rows("v", v, v_token, v_head)) return rc;
+    if (!aligned16(out)) return fail(RESKV_ERR_INVALID, "prompt_attention: out must start on a 16-byte boundary");
+    if (int rc = check_device_pointer(out, "prompt_attention", "out")) return rc;
+    if (int rc = check_device_pointer(cu_seqlens, "prompt_attention", "cu_seqlens")) return rc;
+    PromptParams p{};
+    p.cu = cu_seqlens, p.sequences = sequences, p.total = total, p.kv_heads = kv_heads, p.group = q_heads / kv_heads;
+    p.tile_tokens = 128 / p.group;
+    p.v = static_cast<const unsigned short*>(v), p.v_token = v_token, p.v_head = v_head;
+    p.out = out, p.lse = lse, p.scale_log2 = scaling * kLog2e, p.causal = causal != 0;
+    CUtensorMap qm, km, vm;
+    if (int rc = rows_map(&qm, q, q_heads, total, q_token, q_head, p.group, p.tile_tokens)) return rc;
+    if (int rc = rows_map(&km, k, kv_heads, total, k_token, k_head, 1, kPKeys)) return rc;
+    if (int rc = rows_map(&vm, v, kv_heads, total, v_token, v_head, 1, kPKeys)) return rc;
+    // every sequence has at most one pair of row tiles that is not full
+    const int64_t items = (total / (2 * p.tile_tokens) + static_cast<int64_t>(sequences < total ? sequences : total)) * kv_heads;
+    if (items > 0x7ffffffe) return fail(RESKV_ERR_LIMIT, "prompt_attention: too many tokens for one call");
+    const auto st = static_cast<cudaStream_t>(stream);
+    return bf16 ? launch<true>(p, qm, km, vm, static_cast<unsigned>(items), st) : launch<false>(p, qm, km, vm, static_cast<unsigned>(items), st);
+}
+
+extern "C" int reskv_prompt_attention_status(uint32_t* status, void* stream) {
+    if (!status) return fail(RESKV_ERR_INVALID, "prompt_attention_status: null destination");
+    if (int rc = check_cuda(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)), "prompt_attention_status synchronize")) return rc;
+    return check_cuda(cudaMemcpyFromSymbol(status, g_prompt_status, sizeof(uint32_t)), "prompt_attention_status copy");
+}

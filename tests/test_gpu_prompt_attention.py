@@ -1,0 +1,242 @@
+"""``prompt_attention`` against the formula in 64 bits."""
+
+import pytest
+import torch
+
+from reskv_b200 import prompt_attention
+
+DEV = "cuda"
+
+
+def formula(q, k, v, ends, scaling=128**-0.5, causal=True):
+    """(out, lse, bound) in 64 bits; ``bound``: how far a kernel may be off that rounds weights and results once to the type.
+
+    With u half a step of the type and A = sum_j p_j |v_j|: the weights' rounding moves a result by at most u A, its own
+    rounding by u |o|.  An error e of a weight's exponential moves it by at most 2 e A (numerator and sum); e is at most 2^-13
+    for the exponential itself and |ds| for a score that is off by ds, where 128 products are added in FP32 with an error of
+    at most 128 * 2^-23 sum|q k|.  FP16 weights below 2^-14 are off by up to 2^-25 of the largest weight, in all 2^-25 sum|v|."""
+    u = torch.finfo(q.dtype).eps / 2
+    q, k, v = q.double(), k.double(), v.double()
+    heads, ratio = q.shape[1], q.shape[1] // k.shape[1]
+    out, bound = torch.zeros_like(q), torch.zeros_like(q)
+    lse = torch.zeros(q.shape[:2], dtype=torch.float64, device=q.device)
+    for a, b in zip(ends, ends[1:]):
+        if a == b:
+            continue
+        for h in range(heads):
+            qq, kk, vv = q[a:b, h], k[a:b, h // ratio], v[a:b, h // ratio]
+            s = qq @ kk.T * scaling
+            if causal:
+                s = s.masked_fill(torch.ones_like(s, dtype=torch.bool).triu(1), -torch.inf)
+            p = torch.softmax(s, -1)
+            ds = 128 * 2.0**-23 * scaling * (qq.abs() @ kk.abs().T).amax(-1, keepdim=True)
+            out[a:b, h], spread = p @ vv, p @ vv.abs()
+            lse[a:b, h] = torch.logsumexp(s, -1)
+            bound[a:b, h] = u * (spread + out[a:b, h].abs()) + 2 * spread * (2.0**-13 + ds) + 2.0**-25 * vv.abs().sum(0)
+    return out, lse, bound
+
+
+def inputs(lengths, kv_heads, ratio, dtype, seed=0, spread=1.5, behind=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    total = sum(lengths) + behind
+    x = torch.randn(total, kv_heads * (ratio + 2), 128, generator=g, device=DEV)
+    x[:, :kv_heads * ratio] *= spread
+    x = x.to(dtype)
+    ends = [0]
+    for t in lengths:
+        ends.append(ends[-1] + t)
+    cu = torch.tensor(ends, dtype=torch.int32, device=DEV)
+    h = kv_heads
+    return x[:, :h * ratio], x[:, h * ratio:h * (ratio + 1)], x[:, h * (ratio + 1):], ends, cu
+
+
+def assert_within(got, want, bound):
+    excess = ((got.double() - want).abs() - bound).max().item() if got.numel() else 0.0
+    assert excess <= 0, f"off by {(got.double() - want).abs().max().item():.3e}, {excess:.3e} too much"
+
+
+LENGTHS = [[1], [2, 1, 3], [127], [128], [129], [64, 65], [255, 256, 257], [300, 0, 17, 0], [1000], [31, 513, 128, 1, 700]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lengths", LENGTHS, ids=str)
+def test_lengths(lengths, dtype):
+    q, k, v, ends, cu = inputs(lengths, 2, 4, dtype)
+    got, lse = prompt_attention(q, k, v, cu, return_lse=True)
+    want, want_lse, bound = formula(q, k, v, ends)
+    assert got.shape == q.shape and got.dtype == dtype and got.is_contiguous()
+    assert_within(got, want, bound)
+    # the sum of exponentials: relative 2^-13 at most, scores off by 128 * 2^-23 * sum|q k| * scaling (< 2^-10 here)
+    assert (lse.double() - want_lse).abs().max().item() < 2e-3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("kv_heads,ratio", [(1, 1), (3, 1), (2, 2), (1, 3), (2, 5), (1, 7), (1, 8), (1, 12), (1, 40), (1, 128)])
+def test_head_layouts(kv_heads, ratio, causal):
+    q, k, v, ends, cu = inputs([45, 200, 1], kv_heads, ratio, torch.float16, seed=1)
+    assert_within(prompt_attention(q, k, v, cu, causal=causal), *formula(q, k, v, ends, causal=causal)[::2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scaling", [0.01, 1.0])
+def test_scaling(scaling):
+    q, k, v, ends, cu = inputs([400], 1, 4, torch.bfloat16, seed=2)
+    assert_within(prompt_attention(q, k, v, cu, scaling=scaling), *formula(q, k, v, ends, scaling=scaling)[::2])
+
+
+@pytest.mark.gpu
+def test_a_maximum_that_grows_with_every_key_tile():
+    """Scores rise along the keys, so that the running maximum and the output so far are rescaled again and again."""
+    q, k, v, ends, cu = inputs([900, 700], 1, 4, torch.float16, seed=3, spread=1.0)
+    rise = torch.linspace(0, 60, q.shape[0], device=DEV)[:, None]
+    k[:, 0, :] = (k[:, 0, :].float() * 0.1 + rise / 128).half()
+    q[:, :, :] = (q.float() * 0.05 + 10).half()
+    assert_within(prompt_attention(q, k, v, cu), *formula(q, k, v, ends)[::2])
+
+
+@pytest.mark.gpu
+def test_layouts_in_memory():
+    """Views, token-major and head-major, copies where rows cannot be read in place: the same numbers."""
+    q, k, v, ends, cu = inputs([77, 130], 2, 4, torch.float16, seed=4)
+    want = prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu)
+    assert torch.equal(prompt_attention(q, k, v, cu), want)
+    heads_first = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)]
+    assert torch.equal(prompt_attention(*heads_first, cu), want)
+    odd = torch.empty(q.numel() + 1, dtype=q.dtype, device=DEV)[1:].view(q.shape).copy_(q)
+    assert torch.equal(prompt_attention(odd, k, v, cu), want)
+    strided = torch.empty((*k.shape[:2], 256), dtype=k.dtype, device=DEV)[..., ::2].copy_(k)
+    assert torch.equal(prompt_attention(q, strided, v, cu), want)
+    one = k[:, :1].contiguous()
+    assert torch.equal(prompt_attention(q, one.expand(-1, 2, -1), one.expand(-1, 2, -1), cu),
+                       prompt_attention(q, one.repeat(1, 2, 1), one.repeat(1, 2, 1), cu))
+
+
+@pytest.mark.gpu
+def test_rows_behind_the_last_sequence_stay_and_do_not_count():
+    q, k, v, ends, cu = inputs([70, 33], 2, 4, torch.float16, seed=5, behind=40)
+    want = prompt_attention(q[:103], k[:103], v[:103], cu)
+    for x in (q, k, v):
+        x[103:] = float("nan")
+    v[110] = float("inf")
+    out = torch.full(q.shape, 7.0, dtype=q.dtype, device=DEV)
+    got = prompt_attention(q, k, v, cu, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    assert torch.equal(got[:103], want) and (got[103:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("ratio", [1, 4])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("side", ["key", "value"])
+def test_what_is_not_finite_counts_only_where_it_is_attended_to(dtype, ratio, bad, side):
+    """A later token's infinities and NaN do not reach the rows before it; the rows that see them have what the formula has."""
+    q, k, v, ends, cu = inputs([200, 150], 2, ratio, dtype, seed=6)
+    clean = prompt_attention(q, k, v, cu)
+    at = 131  # inside a key tile, seen by part of a row tile
+    (k if side == "key" else v)[at, 1, 5:9] = bad
+    got = prompt_attention(q, k, v, cu)
+    own = slice(ratio, 2 * ratio)  # the query heads of KV head 1
+    assert torch.equal(got[:at], clean[:at]) and torch.equal(got[200:], clean[200:]) and torch.equal(got[:, :ratio], clean[:, :ratio])
+    if side == "value":
+        seen = got[at:200, own]
+        assert torch.equal(seen[..., :5], clean[at:200, own, :5]) and torch.equal(seen[..., 9:], clean[at:200, own, 9:])
+        assert (seen[..., 5:9].isnan() if bad != bad else seen[..., 5:9] == bad).all()
+    else:
+        # a score of NaN or +inf: NaN.  -inf: a weight of 0
+        score = (q[at:200, own].double()[..., 5:9] * bad).sum(-1)
+        assert got[at:200, own][(score != score) | (score > 0)].isnan().all()
+        rest = score == -torch.inf
+        assert got[at:200, own][rest].isfinite().all()
+
+
+@pytest.mark.gpu
+def test_no_tokens_and_no_sequences():
+    q, k, v, _, cu = inputs([4], 1, 1, torch.float16)
+    assert prompt_attention(q[:0], k[:0], v[:0], cu[:1]).shape == (0, 1, 128)
+    out = torch.zeros_like(q, memory_format=torch.contiguous_format)
+    assert not prompt_attention(q, k, v, cu[:1], out=out).any()
+    assert not prompt_attention(q, k, v, torch.zeros(5, dtype=torch.int32, device=DEV), out=out).any()
+
+
+@pytest.mark.gpu
+def test_bounds_are_clamped():
+    q, k, v, ends, cu = inputs([40, 60], 1, 4, torch.float16, seed=7)
+    wild = torch.tensor([-5, 40, 2**31 - 1], dtype=torch.int32, device=DEV)
+    assert torch.equal(prompt_attention(q, k, v, wild), prompt_attention(q, k, v, cu))
+    back = torch.tensor([0, 100, 30], dtype=torch.int32, device=DEV)  # the second sequence has a negative length: none
+    assert torch.equal(prompt_attention(q, k, v, back), prompt_attention(q, k, v, cu[[0, 2]]))
+
+
+@pytest.mark.gpu
+def test_many_sequences_and_calls_in_a_row():
+    lengths = [(7 * i) % 90 for i in range(150)]
+    q, k, v, ends, cu = inputs(lengths, 2, 2, torch.float16, seed=8)
+    want = formula(q, k, v, ends)[::2]
+    first = prompt_attention(q, k, v, cu)
+    assert_within(first, *want)
+    for _ in range(20):
+        assert torch.equal(prompt_attention(q, k, v, cu), first)
+
+
+@pytest.mark.gpu
+def test_streams_and_a_captured_call():
+    q, k, v, ends, cu = inputs([500, 123], 2, 4, torch.float16, seed=9)
+    want = prompt_attention(q, k, v, cu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        here = prompt_attention(q, k, v, cu)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            there = prompt_attention(q, k, v, cu)
+    torch.cuda.synchronize()
+    assert torch.equal(here, want)
+    other, _, _, _, _ = inputs([500, 123], 2, 4, torch.float16, seed=10)
+    q.copy_(other)
+    graph.replay()
+    assert torch.equal(there, prompt_attention(q, k, v, cu))
+
+
+@pytest.mark.gpu
+def test_refusals():
+    q, k, v, _, cu = inputs([8], 2, 4, torch.float16)
+    bad = [
+        dict(query=q.float()), dict(query=q[..., :64]), dict(key=k[:7]), dict(value=v.bfloat16()), dict(key=k[:, :1]),
+        dict(query=q[:, :7]), dict(cu_seqlens=cu.long()), dict(cu_seqlens=cu[None]), dict(cu_seqlens=cu[:0]), dict(cu_seqlens=cu.cpu()),
+        dict(scaling=0.0), dict(scaling=-1.0), dict(scaling=float("nan")), dict(scaling=float("inf")),
+        dict(out=torch.empty(8, 8, 64, device=DEV)), dict(out=torch.empty(8, 8, 128, device=DEV)),
+        dict(out=torch.empty(8, 8, 256, dtype=torch.float16, device=DEV)[..., :128]), dict(key=k.cpu()),
+        dict(query=q.clone().requires_grad_()),
+    ]
+    for change in bad:
+        args = dict(query=q, key=k, value=v, cu_seqlens=cu) | change
+        with pytest.raises(ValueError):
+            prompt_attention(args.pop("query"), args.pop("key"), args.pop("value"), args.pop("cu_seqlens"), **args)
+    with pytest.raises(TypeError):
+        prompt_attention(q, k, None, cu)
+
+
+def test_the_library_refuses_bad_arguments_before_any_launch():
+    import numpy as np
+
+    from reskv_b200._extension import ERR_INVALID, ERR_LIMIT, library
+
+    lib = library()
+    x = np.zeros((4, 2, 128), np.float16)
+    cu = np.array([0, 4], np.int32)
+    assert x.ctypes.data % 16 == 0
+
+    def call(q=x.ctypes.data, kh=2, nh=2, step=256, scaling=0.1, total=4, sequences=1):
+        return lib.reskv_prompt_attention(q, x.ctypes.data, x.ctypes.data, cu.ctypes.data, sequences, total, kh, nh, 0, step, 128,
+                                          256, 128, 256, 128, scaling, 1, x.ctypes.data, None, None)
+
+    assert call(q=None) == ERR_INVALID and b"null" in lib.reskv_last_error()
+    assert call(nh=3) == ERR_INVALID and call(kh=0) == ERR_INVALID and call(sequences=-1) == ERR_INVALID
+    assert call(kh=1, nh=129) == ERR_LIMIT
+    assert call(scaling=0.0) == ERR_INVALID and call(scaling=float("nan")) == ERR_INVALID
+    assert call(step=129) == ERR_INVALID and call(q=x.ctypes.data + 2) == ERR_INVALID
+    assert call() == ERR_INVALID and b"prompt_attention: q" in lib.reskv_last_error()  # host memory
+    assert call(total=0) == 0 and call(sequences=0) == 0
