@@ -460,6 +460,45 @@ int reskv_prompt_attention(const void* q, const void* k, const void* v, const in
                            void* stream);
 int reskv_prompt_attention_status(uint32_t* status, void* stream);
 
+/* ---- 4-bit paged cache ------------------------------------------------------------------------
+ * No counterpart in the reference, whose caches hold one batch of equal lengths: keys (after RoPE) and values of
+ * sequences of different lengths in pages of 64 tokens, 4 bits per coordinate, one layer per call.
+ *
+ *   pages     u8 [page_count, kv_heads, 9216], 16-byte aligned: per KV head of a page four blocks of 16 tokens, each
+ *             keys then values: codes [16, 64], parameters [16, 4] of the model's type (f16, or bf16 if bf16 != 0):
+ *             scale of coordinates 0..63, of 64..127, offset of either.  csrc/paged_int4.cuh has the order of the codes.
+ *             offset = min, scale = (max - min) / 15 rounded to the type, code = round((x - offset) / scale) to the
+ *             nearest, ties to even, at most 15; 0 where the scale is 0.  The value is offset + scale * code.  A group
+ *             that holds an infinity or a NaN reads as NaN.
+ *   table     i32 [sequences, width]: page of the tokens [64 i, 64 i + 64) of a sequence
+ *   status    u32, device memory: a token outside the table or a page outside the pool sets
+ *             RESKV_STATUS_STATE_RANGE; such a token is not stored (write), not written (read), taken from page 0
+ *             (attention)
+ *
+ * reskv_paged_write: tokens [cu_seqlens[s], cu_seqlens[s+1]) of k and v (rows of 128 dense, strides in elements as for
+ * reskv_prompt_attention) become tokens starts[s], starts[s] + 1, ... of sequence s.  i32 [sequences + 1] and
+ * [sequences], device memory, cu_seqlens non-decreasing.  Tokens of no sequence are ignored.
+ * reskv_paged_read: the reverse, into dense [total, kv_heads, 128]; tokens of no sequence are left as they are.
+ * reskv_paged_attention: one query per sequence, q [sequences, q_heads, 128] (strides q_sequence, q_head), up to
+ * eight query heads per KV head, against tokens [0, lengths[s]) (clamped to the table); out [sequences, q_heads, 128]
+ * dense, lse f32 [sequences, q_heads] or NULL; length 0 gives zeros and -infinity.  The workspace is the call's own
+ * until it has run.
+ * reskv_copy_pages: pages src[i] -> dst[i] (HOST arrays) in each of `layers` pools that lie one behind the other,
+ * page_bytes a multiple of 16; all at once, so no page may be a destination twice or both source and destination. */
+int reskv_paged_write(const void* k, const void* v, int bf16, int64_t k_token, int64_t k_head, int64_t v_token,
+                      int64_t v_head, const int32_t* cu_seqlens, const int32_t* starts, const int32_t* table, int sequences,
+                      int width, int total, int kv_heads, void* pages, int page_count, uint32_t* status, void* stream);
+int reskv_paged_read(void* k, void* v, int bf16, const int32_t* cu_seqlens, const int32_t* starts, const int32_t* table,
+                     int sequences, int width, int total, int kv_heads, const void* pages, int page_count, uint32_t* status,
+                     void* stream);
+size_t reskv_paged_attention_workspace_bytes(int sequences, int width, int kv_heads);
+int reskv_paged_attention(const void* q, int bf16, int64_t q_sequence, int64_t q_head, const int32_t* lengths,
+                          const int32_t* table, int sequences, int width, int kv_heads, int q_heads, const void* pages,
+                          int page_count, float scaling, void* workspace, size_t workspace_bytes, void* out, float* lse,
+                          uint32_t* status, void* stream);
+int reskv_copy_pages(void* pages, int layers, int page_count, int64_t page_bytes, const int32_t* src, const int32_t* dst,
+                     int count, void* stream);
+
 /* ---- test and profiling hooks ---------------------------------------------------------
  * NOT part of the surface a production host binds: both calls set process-wide state without any
  * synchronisation (they change what every thread's next decode call does) and exist for the test suite

@@ -9,7 +9,8 @@ on first use.
 from .config import KernelPlan, ResKVConfig, ResKVKernelConfig
 
 __version__ = "0.1.0"
-__all__ = ["ResKVKernelConfig", "ResKVForCausalLM", "ResKVConfig", "KernelPlan", "compress", "attention", "prompt_attention"]
+__all__ = ["ResKVKernelConfig", "ResKVForCausalLM", "ResKVConfig", "KernelPlan", "compress", "attention", "prompt_attention",
+           "PagedInt4Cache"]
 
 
 def __getattr__(name):
@@ -25,6 +26,10 @@ def __getattr__(name):
         from .prompt import prompt_attention
 
         return prompt_attention
+    if name == "PagedInt4Cache":
+        from .paged import PagedInt4Cache
+
+        return PagedInt4Cache
     if name == "ResKVForCausalLM":  # needs transformers: imported on first use (reference __init__.py:18-21)
         from .models.hf_llama import ResKVForCausalLM
 

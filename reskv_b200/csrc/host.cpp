@@ -819,6 +819,12 @@ PyObject* py_ids_in_range(PyObject*, PyObject* ticket) {
     });
 }
 
+void refuse_gradients(std::initializer_list<at::Tensor> all, const char* who) {
+    if (!c10::GradMode::is_enabled()) return;
+    for (const at::Tensor& t : all)
+        if (t.defined() && t.requires_grad()) value_error(std::string(who) + " is inference only: call it under torch.no_grad()");
+}
+
 // ---- packed prompts ---------------------------------------------------------------------------------------------------
 // x[T,H,128] as the kernels read it: dense rows, strides of whole 16-byte pieces.  Anything else is copied.
 at::Tensor packed_rows(const at::Tensor& x) {
@@ -853,8 +859,7 @@ PyObject* py_prompt_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
         if (!(scaling > 0.0) || !(scaling < 3.0e38)) value_error("scaling must be positive and finite");
         if (out.defined() && (out.sizes() != x[0].sizes() || out.scalar_type() != type || !out.is_contiguous() || !aligned16(out.const_data_ptr())))
             value_error("out must be contiguous, of the query's shape and type, on a 16-byte boundary");
-        if (c10::GradMode::is_enabled() && (x[0].requires_grad() || x[1].requires_grad() || x[2].requires_grad() || (out.defined() && out.requires_grad())))
-            value_error("prompt_attention is inference only: call it under torch.no_grad()");
+        refuse_gradients({x[0], x[1], x[2], out}, "prompt_attention");
         {
             const Unlocked free;
             const at::AutoDispatchBelowADInplaceOrView plain;
@@ -890,6 +895,167 @@ PyObject* py_prompt_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
     });
 }
 
+// ---- 4-bit paged cache --------------------------------------------------------------------------------------------------
+// The pool [layers, pages, KV heads, 4, 2304] and the tables of a step, on one device.
+struct Pool {
+    at::Tensor pages, status;
+    int64_t layer, capacity, heads;
+    c10::DeviceIndex dev;
+    Pool(PyObject* pool, PyObject* index, PyObject* word) : pages(tensor(pool, "pages")), status(tensor(word, "status")), layer(integer(index)) {
+        if (pages.dim() != 5 || pages.scalar_type() != at::kByte || !pages.is_contiguous() || pages.size(3) != 4 || pages.size(4) != 2304 || !pages.is_cuda())
+            value_error("pages must be dense uint8 CUDA [layers, pages, KV heads, 4, 2304]");
+        if (layer < 0 || layer >= pages.size(0)) value_error("layer " + std::to_string(layer) + " of " + std::to_string(pages.size(0)));
+        capacity = pages.size(1), heads = pages.size(2), dev = pages.get_device();
+        same_device(dev, status);
+        if (status.numel() < 1 || status.scalar_type() != at::kInt) value_error("status must be an int32 tensor");
+    }
+    unsigned char* memory() const { return static_cast<unsigned char*>(pages.data_ptr()) + layer * capacity * heads * 9216; }
+    uint32_t* word() const { return static_cast<uint32_t*>(status.data_ptr()); }
+    // The tables of a step: int32, dense, on the pool's device.
+    at::Tensor table(PyObject* o, const char* what, int64_t dims) const {
+        at::Tensor t = tensor(o, what);
+        same_device(dev, t);
+        if (t.scalar_type() != at::kInt || t.dim() != dims || !t.is_contiguous()) value_error(std::string(what) + " must be dense int32");
+        return t;
+    }
+    void after(cudaStream_t stream) const {
+        if (!g_check_status) return;
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        check_cuda(cudaStreamIsCapturing(stream, &capture), "cudaStreamIsCapturing");
+        if (capture != cudaStreamCaptureStatusNone) return;
+        uint32_t status_word = 0;
+        check_cuda(cudaMemcpyAsync(&status_word, word(), sizeof(status_word), cudaMemcpyDeviceToHost, stream), "status copy");
+        check_cuda(cudaStreamSynchronize(stream), "status synchronize");
+        if (status_word) {
+            char text[80];
+            std::snprintf(text, sizeof(text), "paged cache: device status 0x%x", status_word);
+            throw Failure{PyExc_RuntimeError, text};
+        }
+    }
+};
+
+at::ScalarType model_type(const at::Tensor& x, const char* what) {
+    const at::ScalarType t = x.scalar_type();
+    if (t != at::kHalf && t != at::kBFloat16) value_error(std::string(what) + " must be FP16 or BF16");
+    return t;
+}
+
+// paged_write(pages, layer, status, key, value, cu_seqlens, starts, table)
+PyObject* py_paged_write(PyObject*, PyObject* const* o, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        expect(n, 8);
+        const Pool pool(o[0], o[1], o[2]);
+        at::Tensor k = tensor(o[3], "key"), v = tensor(o[4], "value");
+        const at::Tensor cu = pool.table(o[5], "cu_seqlens", 1), starts = pool.table(o[6], "starts", 1), table = pool.table(o[7], "table", 2);
+        const at::ScalarType type = model_type(k, "key");
+        same_device(pool.dev, k), same_device(pool.dev, v);
+        if (k.dim() != 3 || k.size(1) != pool.heads || k.size(2) != 128 || k.sizes() != v.sizes() || v.scalar_type() != type || k.size(0) > 0x7fffffff)
+            value_error("key and value must be [tokens, KV heads, 128] of one type");
+        if (cu.size(0) != starts.size(0) + 1 || table.size(0) != starts.size(0)) value_error("cu_seqlens, starts and table belong to different numbers of sequences");
+        refuse_gradients({k, v}, "paged_write");
+        {
+            const Unlocked free;
+            const at::AutoDispatchBelowADInplaceOrView plain;
+            const c10::cuda::CUDAGuard guard(pool.dev);
+            const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(pool.dev).stream();
+            if (k.size(0) > 0 && starts.size(0) > 0) {
+                k = packed_rows(k), v = packed_rows(v);
+                check(reskv_paged_write(k.const_data_ptr(), v.const_data_ptr(), type == at::kBFloat16, token_step(k), head_step(k), token_step(v),
+                                        head_step(v), static_cast<const int32_t*>(cu.const_data_ptr()), static_cast<const int32_t*>(starts.const_data_ptr()),
+                                        static_cast<const int32_t*>(table.const_data_ptr()), static_cast<int>(starts.size(0)),
+                                        static_cast<int>(table.size(1)), static_cast<int>(k.size(0)), static_cast<int>(pool.heads), pool.memory(),
+                                        static_cast<int>(pool.capacity), pool.word(), stream));
+                ++g_launches;
+                pool.after(stream);
+            }
+        }
+        return Py_NewRef(Py_None);
+    });
+}
+
+// paged_read(pages, layer, status, bf16, cu_seqlens, starts, table, tokens) -> (key, value)
+PyObject* py_paged_read(PyObject*, PyObject* const* o, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        expect(n, 8);
+        const Pool pool(o[0], o[1], o[2]);
+        const bool bf16 = o[3] == Py_True;
+        const at::Tensor cu = pool.table(o[4], "cu_seqlens", 1), starts = pool.table(o[5], "starts", 1), table = pool.table(o[6], "table", 2);
+        const int64_t total = integer(o[7]);
+        if (total < 0 || total > 0x7fffffff) value_error("too many tokens for one call");
+        if (cu.size(0) != starts.size(0) + 1 || table.size(0) != starts.size(0)) value_error("cu_seqlens, starts and table belong to different numbers of sequences");
+        at::Tensor k, v;
+        {
+            const Unlocked free;
+            const at::AutoDispatchBelowADInplaceOrView plain;
+            const c10::cuda::CUDAGuard guard(pool.dev);
+            const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(pool.dev).stream();
+            const at::ScalarType type = bf16 ? at::kBFloat16 : at::kHalf;
+            k = at::detail::empty_cuda({total, pool.heads, 128}, type, pool.pages.device(), std::nullopt);
+            v = at::detail::empty_cuda({total, pool.heads, 128}, type, pool.pages.device(), std::nullopt);
+            if (total > 0 && starts.size(0) > 0) {
+                check(reskv_paged_read(k.data_ptr(), v.data_ptr(), bf16, static_cast<const int32_t*>(cu.const_data_ptr()),
+                                       static_cast<const int32_t*>(starts.const_data_ptr()), static_cast<const int32_t*>(table.const_data_ptr()),
+                                       static_cast<int>(starts.size(0)), static_cast<int>(table.size(1)), static_cast<int>(total),
+                                       static_cast<int>(pool.heads), pool.memory(), static_cast<int>(pool.capacity), pool.word(), stream));
+                ++g_launches;
+                pool.after(stream);
+            }
+        }
+        PyObject* t = PyTuple_New(2);
+        PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(k));
+        PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(v));
+        return t;
+    });
+}
+
+// paged_attention(pages, layer, status, query, lengths, table, scaling, return_lse) -> out or (out, lse)
+PyObject* py_paged_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        expect(n, 8);
+        const Pool pool(o[0], o[1], o[2]);
+        at::Tensor q = tensor(o[3], "query");
+        const at::Tensor lengths = pool.table(o[4], "lengths", 1), table = pool.table(o[5], "table", 2);
+        const double scaling = o[6] == Py_None ? 0.08838834764831845 : number(o[6]);  // 128 ** -0.5
+        const bool stats = o[7] == Py_True;
+        const at::ScalarType type = model_type(q, "query");
+        same_device(pool.dev, q);
+        if (q.dim() != 3 || q.size(2) != 128 || q.size(0) != lengths.size(0) || table.size(0) != q.size(0))
+            value_error("query must be [sequences, query heads, 128], one row per sequence of the step");
+        if (q.size(1) < 1 || q.size(1) % pool.heads || q.size(1) / pool.heads > 8)
+            value_error("query heads must be a multiple of the KV heads, at most 8 per KV head");
+        if (!(scaling > 0.0) || !(scaling < 3.0e38)) value_error("scaling must be positive and finite");
+        if (q.size(0) * pool.heads > 0x7fffffff || table.size(1) > (1 << 24)) value_error("too many sequences or pages for one call");
+        refuse_gradients({q}, "paged_attention");
+        at::Tensor out, lse;
+        {
+            const Unlocked free;
+            const at::AutoDispatchBelowADInplaceOrView plain;
+            const c10::cuda::CUDAGuard guard(pool.dev);
+            const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(pool.dev).stream();
+            out = at::detail::empty_cuda(q.sizes(), type, q.device(), std::nullopt);
+            if (stats) lse = at::detail::empty_cuda({q.size(0), q.size(1)}, at::kFloat, q.device(), std::nullopt);
+            if (q.size(0) > 0) {
+                q = packed_rows(q);
+                const int sequences = static_cast<int>(q.size(0)), width = static_cast<int>(table.size(1)), heads = static_cast<int>(pool.heads);
+                const size_t need = reskv_paged_attention_workspace_bytes(sequences, width, heads);
+                const at::Tensor ws = at::detail::empty_cuda({static_cast<int64_t>(need)}, at::kByte, q.device(), std::nullopt);
+                check(reskv_paged_attention(q.const_data_ptr(), type == at::kBFloat16, token_step(q), head_step(q),
+                                            static_cast<const int32_t*>(lengths.const_data_ptr()), static_cast<const int32_t*>(table.const_data_ptr()),
+                                            sequences, width, heads, static_cast<int>(q.size(1)), pool.memory(), static_cast<int>(pool.capacity),
+                                            static_cast<float>(scaling), ws.data_ptr(), need, out.data_ptr(),
+                                            stats ? static_cast<float*>(lse.data_ptr()) : nullptr, pool.word(), stream));
+                g_launches += width > 0 ? 2 : 1;
+                pool.after(stream);
+            }
+        }
+        if (!stats) return THPVariable_Wrap(out);
+        PyObject* t = PyTuple_New(2);
+        PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(out));
+        PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(lse));
+        return t;
+    });
+}
+
 PyObject* py_launches(PyObject*, PyObject*) { return PyLong_FromLongLong(g_launches); }
 
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f))
@@ -897,6 +1063,9 @@ PyMethodDef g_methods[] = {
     {"decode", FAST(py_decode), METH_FASTCALL, "decode attention on given operands"},
     {"attention", FAST(py_attention), METH_FASTCALL, "decode attention on a compressed cache"},
     {"prompt_attention", FAST(py_prompt_attention), METH_FASTCALL, "attention over packed prompts"},
+    {"paged_write", FAST(py_paged_write), METH_FASTCALL, "tokens into a 4-bit paged cache"},
+    {"paged_read", FAST(py_paged_read), METH_FASTCALL, "values of tokens of a 4-bit paged cache"},
+    {"paged_attention", FAST(py_paged_attention), METH_FASTCALL, "one query per sequence against a 4-bit paged cache"},
     {"window_append", FAST(py_window_append), METH_FASTCALL, "append one token to the dense window"},
     {"encode", FAST(py_encode), METH_FASTCALL, "pack one side"},
     {"kmeans_pair", FAST(py_kmeans_pair), METH_FASTCALL, "cluster K and V in the same launch"},

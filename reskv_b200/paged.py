@@ -1,0 +1,303 @@
+"""Paged KV cache in 4 bits for sequences of different lengths.
+
+The compressed caches of this package hold one batch of equal lengths.  ``PagedInt4Cache`` is the cache of a server whose
+sequences come, grow, fork and go: keys (after RoPE) and values as 4-bit codes in pages of 64 tokens out of one pool for all
+layers, 144 bytes per token and KV head instead of 512.  The kernels are ``csrc/paged_store.cu`` and
+``csrc/paged_attention.cu``; the layout of a page is described in ``csrc/paged_int4.cuh``.
+
+A step of a model::
+
+    step = cache.extend(sequences, counts)          # room for the new tokens; tables on the device
+    for layer ...:
+        cache.write(layer, step, key, value)        # [new tokens, KV heads, 128], packed
+        out = cache.attend(layer, step, query)      # one query per sequence, or prompt_attention for whole prompts
+"""
+
+from __future__ import annotations
+
+
+import numpy as np
+import torch
+
+from ._extension import _stream, bound_library, check, device_index_of, host, require_device
+
+PAGE_TOKENS = 64
+_PAGE_HEAD = (4, 2304)  # blocks of 16 tokens, bytes of a block
+_TYPES = (torch.float16, torch.bfloat16)
+
+
+class PagedStep:
+    """Where the tokens of one step lie: made by ``PagedInt4Cache.extend`` and used for every layer of the step.
+
+    ``counts[i]`` tokens of ``sequences[i]`` are new, ``lengths[i]`` is its length with them; ``total`` is their sum over the
+    step.  ``cu_seqlens`` (int32, on the device) says which rows of the packed tensors belong to which sequence and serves
+    ``prompt_attention`` as it is."""
+
+    __slots__ = ("sequences", "counts", "lengths", "total", "cu_seqlens", "starts", "device_lengths", "table", "_whole", "_epoch", "_current")
+
+    def _everything(self):
+        """``(cu_seqlens, starts, tokens)`` of all tokens of the sequences, the earlier ones included."""
+        if self._whole is None:
+            ends = np.concatenate(([0], np.cumsum(self.lengths)))
+            if ends[-1] > 2**31 - 1:
+                raise ValueError("too many tokens for one call")
+            self._whole = (_upload(ends.astype(np.int32), self.table.device), torch.zeros_like(self.starts), int(ends[-1]))
+        return self._whole
+
+
+def _upload(numbers: np.ndarray, device) -> torch.Tensor:
+    """int32 numbers on the device, without waiting for the copy."""
+    pinned = torch.empty(numbers.size, dtype=torch.int32, pin_memory=True)
+    pinned.numpy()[:] = numbers.reshape(-1)
+    return pinned.to(device, non_blocking=True)
+
+
+class PagedInt4Cache:
+    """4-bit cache of ``layers`` layers with ``kv_heads`` heads of 128 in a pool of ``pages`` pages of 64 tokens.
+
+    Sequences are numbers given out by ``add`` and ``fork``.  A page that is full may be shared by forked sequences; a page
+    that still takes tokens belongs to one.  The calls launch on the current stream of the cache's device and do not wait for it;
+    a caller that uses several streams orders them itself.  The tables are the host's, so one thread at a time changes a cache.
+    """
+
+    def __init__(self, layers: int, kv_heads: int, pages: int, *, dtype: torch.dtype = torch.float16, device="cuda"):
+        for name, value in (("layers", layers), ("kv_heads", kv_heads), ("pages", pages)):
+            if type(value) is not int or value < 1:
+                raise ValueError(f"{name} must be a positive integer")
+        if dtype not in _TYPES:
+            raise ValueError("dtype must be torch.float16 or torch.bfloat16")
+        self.layers, self.kv_heads, self.capacity, self.dtype = layers, kv_heads, pages, dtype
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise ValueError("a paged cache lives on a CUDA device")
+        self.device = torch.device("cuda", device_index_of(self.device))
+        require_device(self.device.index)
+        self.pages = torch.empty((layers, pages, kv_heads, *_PAGE_HEAD), dtype=torch.uint8, device=self.device)
+        self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._lib = bound_library(self.device)
+        self._book = PageBook(pages)
+
+    # -- sequences -------------------------------------------------------------------------------------------------------------
+    @property
+    def free_pages(self) -> int:
+        return len(self._book.free)
+
+    def add(self, count: int = 1) -> list[int]:
+        """``count`` new, empty sequences."""
+        return self._book.add(count)
+
+    def length(self, sequence: int) -> int:
+        return self._book.of(sequence).length
+
+    def extend(self, sequences, counts) -> PagedStep:
+        """Room for ``counts[i]`` (or ``counts`` for each) more tokens of ``sequences[i]``, no sequence twice.  Earlier steps
+        of these sequences may not be used any more.  RuntimeError, and nothing changed, when the pool has too few pages."""
+        book = self._book
+        sequences, counts = list(sequences), [counts] * len(sequences) if type(counts) is int else list(counts)
+        entries = book.extend(sequences, counts)
+        step = PagedStep()
+        n, width = len(entries), max((len(e.pages) for e in entries), default=0)
+        step.sequences, step.counts, step.lengths = tuple(sequences), tuple(counts), tuple(e.length for e in entries)
+        step.total = sum(counts)
+        numbers = np.zeros(3 * n + 1 + n * width, np.int32)
+        np.cumsum(counts, out=numbers[1:n + 1])
+        numbers[2 * n + 1:3 * n + 1] = step.lengths
+        numbers[n + 1:2 * n + 1] = numbers[2 * n + 1:3 * n + 1] - np.asarray(counts, np.int32)
+        table = numbers[3 * n + 1:].reshape(n, width)
+        for row, e in zip(table, entries):
+            row[:len(e.pages)] = e.pages
+        there = _upload(numbers, self.device)
+        step.cu_seqlens, step.starts, step.device_lengths = there[:n + 1], there[n + 1:2 * n + 1], there[2 * n + 1:3 * n + 1]
+        step.table = there[3 * n + 1:].view(n, width)
+        step._whole, step._epoch, step._current = None, book.epoch, True
+        for e in entries:
+            e.supersede(step)
+        return step
+
+    def fork(self, sequences) -> list[int]:
+        """A new sequence with the tokens of each of ``sequences`` (one may be named several times).  Full pages are shared, a
+        partly filled last page is copied; steps of the forked sequences may not be used any more."""
+        new, pairs = self._book.fork(list(sequences))
+        self._copy(pairs)
+        return new
+
+    def free(self, sequences) -> None:
+        """Ends ``sequences``; pages that no other sequence shares go back to the pool."""
+        self._book.release(list(sequences))
+
+    def compact(self) -> int:
+        """Moves the pages in use to the front of the pool and returns their number.  No earlier step may be used any more."""
+        used, pairs = self._book.compact()
+        self._copy(pairs)
+        return used
+
+    # -- device ----------------------------------------------------------------------------------------------------------------
+    def _check(self, step: PagedStep) -> None:
+        if not isinstance(step, PagedStep):
+            raise TypeError(f"expected a PagedStep, got {type(step).__name__}")
+        if not step._current or step._epoch is not self._book.epoch:
+            raise ValueError("the step belongs to another cache, or its sequences have been extended, forked, freed or moved since")
+
+    def write(self, layer: int, step: PagedStep, key: torch.Tensor, value: torch.Tensor) -> None:
+        """Stores the step's new tokens: ``key`` (after RoPE) and ``value`` ``[step.total, KV heads, 128]`` of the cache's type."""
+        self._check(step)
+        if key.dtype != self.dtype or key.shape[0] != step.total:
+            raise ValueError(f"key and value must hold the step's {step.total} tokens in {self.dtype}")
+        host().paged_write(self.pages, layer, self._status, key, value, step.cu_seqlens, step.starts, step.table)
+
+    def read(self, layer: int, step: PagedStep, *, everything: bool = False):
+        """``(key, value)`` as the cache holds them: of the step's new tokens, or of all tokens of its sequences
+        (``everything``), packed ``[tokens, KV heads, 128]`` in the order of the step."""
+        self._check(step)
+        cu, starts, tokens = step._everything() if everything else (step.cu_seqlens, step.starts, step.total)
+        return host().paged_read(self.pages, layer, self._status, self.dtype == torch.bfloat16, cu, starts, step.table, tokens)
+
+    def attend(self, layer: int, step: PagedStep, query: torch.Tensor, *, scaling: float | None = None, return_lse: bool = False):
+        """One query per sequence of the step, ``[sequences, H, 128]`` after RoPE, against all of its tokens; ``H`` is up to
+        eight times the KV heads, ``scaling`` (positive) defaults to ``128**-0.5``.  Returns ``[sequences, H, 128]``, with
+        ``return_lse`` also FP32 ``[sequences, H]``, the logarithm of the sum of exponentials.  A sequence without tokens gets
+        zeros (and minus infinity)."""
+        self._check(step)
+        if query.dtype != self.dtype:
+            raise ValueError(f"query must be {self.dtype}")
+        return host().paged_attention(self.pages, layer, self._status, query, step.device_lengths, step.table, scaling, bool(return_lse))
+
+    def copy_pages(self, src, dst) -> None:
+        """Copies pages ``src[i]`` to ``dst[i]`` in all layers, all at once: no page may be a destination twice, or source and
+        destination.  What ``fork`` and ``compact`` use; the caller of this one answers for whose pages they are."""
+        src, dst = list(src), list(dst)
+        if len(src) != len(dst):
+            raise ValueError("as many sources as destinations are needed")
+        for page in (*src, *dst):
+            if type(page) is not int or not 0 <= page < self.capacity:
+                raise ValueError(f"page {page} of {self.capacity}")
+        self._copy(list(zip(src, dst)))
+
+    def _copy(self, pairs) -> None:
+        if not pairs:
+            return
+        numbers = np.array(pairs, dtype=np.int32).T.copy()
+        launches = -(-len(pairs) // 480)
+        check(self._lib.reskv_copy_pages(self.pages.data_ptr(), self.layers, self.capacity, self.pages.stride(1),
+                                         numbers[0].ctypes.data, numbers[1].ctypes.data, len(pairs), _stream(self.device)),
+              launches=launches)
+
+    def check(self) -> None:
+        """Waits for the device and raises if a kernel met a token or page outside its tables, or a wait that ran out."""
+        word = self._status.item()
+        if word:
+            raise RuntimeError(f"paged cache: device status 0x{word & 0xFFFFFFFF:x}")
+
+    @property
+    def nbytes(self) -> int:
+        return self.pages.nbytes
+
+
+class _Sequence:
+    __slots__ = ("pages", "length", "step")
+
+    def __init__(self, pages=(), length=0):
+        self.pages, self.length, self.step = list(pages), length, None
+
+    def supersede(self, step=None):
+        if self.step is not None:
+            self.step._current = False
+        self.step = step
+
+
+class PageBook:
+    """Which sequence holds which pages, and how often a page is held.  Host only."""
+
+    def __init__(self, pages: int):
+        self.free = list(range(pages - 1, -1, -1))  # taken from the end: the lowest numbers first
+        self.holders = [0] * pages
+        self.sequences: dict[int, _Sequence] = {}
+        self.epoch = object()  # steps made before the pages moved belong to another one
+        self._next = 0
+
+    def of(self, sequence: int) -> _Sequence:
+        entry = self.sequences.get(sequence) if type(sequence) is int else None
+        if entry is None:
+            raise ValueError(f"no sequence {sequence!r} in this cache")
+        return entry
+
+    def _new(self, entry: _Sequence) -> int:
+        self.sequences[self._next] = entry
+        self._next += 1
+        return self._next - 1
+
+    def _take(self) -> int:
+        page = self.free.pop()
+        self.holders[page] = 1
+        return page
+
+    def _need(self, pages: int) -> None:
+        if pages > len(self.free):
+            raise RuntimeError(f"out of pages: {pages} needed, {len(self.free)} free")
+
+    def add(self, count: int) -> list[int]:
+        if type(count) is not int or count < 0:
+            raise ValueError("count must be a non-negative integer")
+        return [self._new(_Sequence()) for _ in range(count)]
+
+    def extend(self, sequences, counts) -> list[_Sequence]:
+        entries = [self.of(s) for s in sequences]
+        if len(set(sequences)) != len(sequences):
+            raise ValueError("a sequence is named twice")
+        if len(counts) != len(entries) or any(type(c) is not int or c < 0 for c in counts):
+            raise ValueError("counts must be one non-negative integer per sequence")
+        if sum(counts) > 2**31 - 1 or any(e.length + c > 2**31 - PAGE_TOKENS for e, c in zip(entries, counts)):
+            raise ValueError("too many tokens")
+        more = [-(-(e.length + c) // PAGE_TOKENS) - len(e.pages) for e, c in zip(entries, counts)]
+        self._need(sum(more))
+        for e, c, m in zip(entries, counts, more):
+            e.pages.extend(self._take() for _ in range(m))
+            e.length += c
+        return entries
+
+    def fork(self, sequences):
+        """(new sequences, pages to copy)"""
+        entries = [self.of(s) for s in sequences]
+        self._need(sum(e.length % PAGE_TOKENS != 0 for e in entries))
+        new, pairs = [], []
+        for e in entries:
+            pages = list(e.pages)
+            shared = pages
+            if e.length % PAGE_TOKENS:
+                shared = pages[:-1]
+                pages[-1] = self._take()
+                pairs.append((e.pages[-1], pages[-1]))
+            for page in shared:
+                self.holders[page] += 1
+            e.supersede()
+            new.append(self._new(_Sequence(pages, e.length)))
+        return new, pairs
+
+    def release(self, sequences) -> None:
+        entries = [self.of(s) for s in sequences]
+        if len(set(sequences)) != len(sequences):
+            raise ValueError("a sequence is named twice")
+        for s, e in zip(sequences, entries):
+            e.supersede()
+            for page in reversed(e.pages):
+                self.holders[page] -= 1
+                if self.holders[page] == 0:
+                    self.free.append(page)
+            del self.sequences[s]
+
+    def compact(self):
+        """(pages in use, pages to copy)"""
+        pages = len(self.holders)
+        used = pages - len(self.free)
+        behind = [p for p in range(used, pages) if self.holders[p]]
+        room = [p for p in range(used) if not self.holders[p]]
+        pairs = list(zip(behind, room))
+        moved = dict(pairs)
+        for a, b in pairs:
+            self.holders[b], self.holders[a] = self.holders[a], 0
+        for e in self.sequences.values():
+            e.pages = [moved.get(p, p) for p in e.pages]
+            e.supersede()
+        self.free = list(range(pages - 1, used - 1, -1))
+        self.epoch = object()
+        return used, pairs

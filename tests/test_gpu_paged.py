@@ -1,0 +1,448 @@
+"""``PagedInt4Cache``: what it stores, and attention over it, against their definitions."""
+
+import numpy as np
+import pytest
+import torch
+
+from reskv_b200 import PagedInt4Cache, prompt_attention
+
+DEV = "cuda"
+TYPES = [torch.float16, torch.bfloat16]
+
+
+def stored(x):
+    """(value, scale, offset, code) per group of 64, FP32 from the definition: the quotient is rounded to FP32, then to the
+    nearest whole number."""
+    g = x.float().cpu().unflatten(-1, (2, 64))
+    low, high = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
+    scale = torch.from_numpy((high - low).numpy() / np.float32(15)).to(x.dtype).float()
+    with np.errstate(divide="ignore", invalid="ignore"):
+        code = np.rint((g - low).numpy() / scale.numpy())
+    code = torch.from_numpy(np.where(scale.numpy() > 0, np.minimum(code, 15), 0).astype(np.float32))
+    return low + scale * code, scale, low, code
+
+
+def values_of(x):
+    return stored(x)[0].flatten(-2).to(x.dtype).to(x.device)
+
+
+def vectors(tokens, heads, dtype, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(tokens, heads, 128, generator=g, device=DEV)
+    return (x * torch.where(torch.rand(heads, 128, generator=g, device=DEV) > 0.95, 5.0, 1.0) + 0.3).to(dtype)
+
+
+def fill(cache, lengths, seed=0, pieces=1):
+    """Sequences of these lengths, written in ``pieces`` steps -> (last step's sequences, keys and values of each)."""
+    seqs = cache.add(len(lengths))
+    k = [vectors(t, cache.kv_heads, cache.dtype, seed + 2 * i) for i, t in enumerate(lengths)]
+    v = [vectors(t, cache.kv_heads, cache.dtype, seed + 2 * i + 1) for i, t in enumerate(lengths)]
+    for piece in range(pieces):
+        cuts = [(t * piece // pieces, t * (piece + 1) // pieces) for t in lengths]
+        step = cache.extend(seqs, [b - a for a, b in cuts])
+        for layer in range(cache.layers):
+            cache.write(layer, step, *(torch.cat([x[a:b] for x, (a, b) in zip(side, cuts)]) for side in (k, v)))
+    return seqs, k, v
+
+
+def formula(q, k, v, scaling=128**-0.5):
+    """(out, lse, bound) in 64 bits for one query row [H, 128] and the stored keys and values of its sequence.
+
+    The weights times their token's scale are rounded to FP16 (half a step: 2^-11) in front of their product with the codes,
+    whose absolute sum is S = sum_j p_j (v_j - offset_j); those below FP16's normal numbers are off by 2^-25 where the largest
+    scale counts 2^14, so all together by less than 2^-38 T max(v - offset).  The result is rounded once (u).  A score is off by
+    at most ds: 128 products and their scaling in FP32, 130 * 2^-23 sum |q| (|offset| + 15 scale); that and 2^-20 for the
+    exponential and the sums of T weights (T 2^-24) count twice (numerator, sum) with A = sum_j p_j (|offset_j| + v_j - offset_j)."""
+    u = torch.finfo(q.dtype).eps / 2
+    heads, ratio = q.shape[0], q.shape[0] // k.shape[1]
+    q = q.double()
+    (kv, ks, kl, _), (vv, vs, vl, vc) = stored(k), stored(v)
+    to = lambda x: x.double().to(DEV)  # noqa: E731
+    key, value = to(kv).flatten(-2), to(vv).flatten(-2)
+    big = (to(kl).abs() + 15 * to(ks)).expand(-1, -1, 2, 64).flatten(-2)
+    above, below = (to(vs) * to(vc)).flatten(-2), to(vl).abs().expand(-1, -1, 2, 64).flatten(-2)
+    out, bound, lse = torch.zeros_like(q), torch.zeros_like(q), torch.zeros(heads, dtype=torch.float64, device=DEV)
+    t = key.shape[0]
+    for h in range(heads):
+        g = h // ratio
+        s = key[:, g] @ q[h] * scaling
+        p = torch.softmax(s, 0)
+        lse[h] = torch.logsumexp(s, 0)
+        out[h] = p @ value[:, g]
+        ds = 130 * 2.0**-23 * scaling * (big[:, g] @ q[h].abs()).max()
+        bound[h] = (2.0**-11 * (p @ above[:, g]) + u * out[h].abs() + 2 * (ds + 2.0**-20 + t * 2.0**-24) * (p @ (above + below)[:, g])
+                    + 2.0**-38 * t * above[:, g].amax(0) + 2.0**-25)
+    return out, lse, bound
+
+
+def assert_attends(cache, seqs, k, v, ratio, seed=50, layer=0, **kw):
+    step = cache.extend(seqs, 0)
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    q = torch.randn(len(seqs), cache.kv_heads * ratio, 128, generator=g, device=DEV).to(cache.dtype)
+    got, lse = cache.attend(layer, step, q, return_lse=True, **kw)
+    assert got.dtype == cache.dtype and got.shape == q.shape
+    for i in range(len(seqs)):
+        if len(k[i]) == 0:
+            assert not got[i].any() and (lse[i] == -torch.inf).all()
+            continue
+        want, want_lse, bound = formula(q[i], k[i], v[i], **kw)
+        undefined = want.isnan()  # values beyond the type's range were infinite before they were stored
+        assert torch.equal(got[i].isnan(), undefined)
+        err, bound = (got[i].double() - want).abs()[~undefined], bound[~undefined]
+        assert (err <= bound).all(), f"sequence {i}: off by {err.max():.3e}, {(err - bound).max():.3e} too much"
+        assert (lse[i].double() - want_lse).abs().max() < 1e-3
+    return got
+
+
+# ---- storing ------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kv_heads", [1, 3, 8])
+def test_what_is_written_is_read(dtype, kv_heads):
+    lengths = [1, 64, 65, 200, 0, 129]
+    cache = PagedInt4Cache(2, kv_heads, 16, dtype=dtype)
+    seqs, k, v = fill(cache, lengths, seed=3, pieces=3)
+    got = cache.read(1, cache.extend(seqs, 0), everything=True)
+    for x, side in zip(got, (k, v)):
+        assert x.dtype == dtype and torch.equal(x, torch.cat([values_of(y) for y in side]))
+    cache.check()
+
+
+@pytest.mark.gpu
+def test_read_gives_the_tokens_of_the_step():
+    cache = PagedInt4Cache(1, 2, 8)
+    seqs, k, v = fill(cache, [70, 10], seed=1)
+    step = cache.extend(seqs, [3, 60])
+    nk, nv = vectors(63, 2, torch.float16, 90), vectors(63, 2, torch.float16, 91)
+    cache.write(0, step, nk, nv)
+    got = cache.read(0, step)
+    assert torch.equal(got[0], values_of(nk)) and torch.equal(got[1], values_of(nv))
+    whole = cache.read(0, step, everything=True)[0]
+    assert torch.equal(whole, torch.cat([values_of(x) for x in (k[0], nk[:3], k[1], nk[3:])]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_at_the_edges(dtype):
+    """Constant rows, the largest and smallest numbers of the type, quotients on a half, signed zeros; NaN and infinities make
+    their group of 64 NaN and no other."""
+    info = torch.finfo(dtype)
+    x = torch.zeros(12, 1, 128)
+    x[1] = 3.5
+    x[2, 0, :64], x[2, 0, 64:] = info.max / 2, -info.max / 2
+    x[2, 0, ::2] *= -0.5
+    x[3, 0, 1] = info.smallest_normal * info.eps  # the smallest subnormal
+    x[4] = torch.linspace(0, 15, 128)
+    x[5, 0, :64] = torch.arange(64) / 4  # with 15.75 as the largest: a scale of 1.05
+    x[6, 0, :64] = (torch.arange(64) / 2).clamp(max=15)  # scale 1: halves go to the even code
+    x[7, 0, 64:] = -0.0
+    x[8, 0, 0] = torch.nan
+    x[9, 0, 100] = torch.inf
+    x[10, 0, 3] = -torch.inf
+    x[11] = torch.randn(128, generator=torch.Generator().manual_seed(0)) * 1e-4
+    x = x.to(dtype).to(DEV)
+    cache = PagedInt4Cache(1, 1, 1, dtype=dtype)
+    step = cache.extend(cache.add(1), 12)
+    cache.write(0, step, x, x.flip(0))
+    k, v = cache.read(0, step)
+    assert torch.equal(k[:8], values_of(x[:8])) and torch.equal(k[11], values_of(x[11:])[0])
+    assert torch.equal(v[4:], values_of(x[:8].flip(0))) and torch.equal(v[0], k[11])
+    for row, group in ((8, 0), (9, 1), (10, 0)):
+        bad, good = (k[row, 0, 64 * i:64 * i + 64] for i in (group, 1 - group))
+        assert bad.isnan().all() and not good.any()
+
+
+@pytest.mark.gpu
+def test_layouts_in_memory():
+    """Views of a fused projection, head-major and misaligned tensors are stored alike."""
+    cache = PagedInt4Cache(1, 2, 4)
+    fused = torch.randn(100, 8, 128, device=DEV).half()
+    k, v = fused[:, 4:6], fused[:, 6:]
+    step = cache.extend(cache.add(1), 100)
+
+    def after(key, value):
+        cache.pages.zero_()
+        cache.write(0, step, key, value)
+        return cache.pages.clone()
+
+    want = after(k.contiguous(), v.contiguous())
+    assert torch.equal(after(k, v), want)
+    assert torch.equal(after(k.transpose(0, 1).contiguous().transpose(0, 1), v), want)
+    odd = torch.empty(k.numel() + 1, dtype=k.dtype, device=DEV)[1:].view(k.shape).copy_(k)
+    assert torch.equal(after(odd, v), want)
+    one = k[:, :1].contiguous()
+    assert torch.equal(after(one.expand(-1, 2, -1), v), after(one.repeat(1, 2, 1), v))
+
+
+@pytest.mark.gpu
+def test_rows_behind_the_step_and_other_pages_stay():
+    cache = PagedInt4Cache(1, 2, 6)
+    cache.pages.fill_(17)
+    seqs = cache.add(2)
+    step = cache.extend(seqs, [5, 70])
+    more = vectors(90, 2, torch.float16, 5)
+    from reskv_b200._extension import host
+
+    # tensors longer than the step (a padded batch): the tokens behind the last sequence are ignored
+    host().paged_write(cache.pages, 0, cache._status, more, more, step.cu_seqlens, step.starts, step.table)
+    assert torch.equal(cache.read(0, step)[0], values_of(more[:75]))
+    assert (cache.pages[0, 3:] == 17).all()
+    assert (cache.pages[0, 0, :, 1:] == 17).all()  # the blocks of the first page behind its five tokens
+    k, v = host().paged_read(cache.pages, 0, cache._status, False, step.cu_seqlens, step.starts, step.table, 75)
+    assert torch.equal(k, cache.read(0, step)[0])
+    cache.check()
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------------
+LENGTHS = [[1], [15, 16, 17], [63, 64, 65], [128, 0, 129], [300], [1000, 3, 777], [5000, 1, 130, 64, 2222]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths", LENGTHS, ids=str)
+def test_lengths(lengths, dtype):
+    cache = PagedInt4Cache(1, 2, sum(-(-t // 64) for t in lengths), dtype=dtype)
+    assert_attends(cache, *fill(cache, lengths, seed=7), 4)
+    cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_heads,ratio", [(1, 1), (3, 2), (2, 3), (1, 5), (2, 7), (8, 8)])
+def test_head_layouts(kv_heads, ratio):
+    cache = PagedInt4Cache(2, kv_heads, 40)
+    assert_attends(cache, *fill(cache, [600, 77, 1], seed=11), ratio, layer=1)
+
+
+@pytest.mark.gpu
+def test_many_short_sequences():
+    """More units than there are CTAs: shares that hold several units, or parts of two."""
+    lengths = [(37 * i) % 190 for i in range(120)]
+    cache = PagedInt4Cache(1, 4, sum(-(-t // 64) for t in lengths))
+    assert_attends(cache, *fill(cache, lengths, seed=13), 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("key_size,value_size,scaling", [(1.0, 1e-4, 0.1), (1.0, 2000.0, 0.1), (100.0, 1.0, 0.01), (1e-3, 1.0, 30.0)])
+def test_magnitudes(dtype, key_size, value_size, scaling):
+    cache = PagedInt4Cache(1, 1, 20, dtype=dtype)
+    seqs = cache.add(2)
+    k = [vectors(t, 1, torch.float32, i).mul(key_size).to(dtype) for i, t in enumerate((500, 90))]
+    v = [vectors(t, 1, torch.float32, 5 + i).mul(value_size).to(dtype) for i, t in enumerate((500, 90))]
+    v[0][100:] *= 16  # scales that grow along the sequence
+    cache.write(0, cache.extend(seqs, [500, 90]), torch.cat(k), torch.cat(v))
+    assert_attends(cache, seqs, k, v, 4, scaling=scaling)
+
+
+@pytest.mark.gpu
+def test_a_maximum_that_grows_along_the_sequence():
+    cache = PagedInt4Cache(1, 1, 40)
+    seqs = cache.add(1)
+    k = vectors(2000, 1, torch.float16, 1) * 0.1 + torch.linspace(0, 4, 2000, device=DEV)[:, None, None].half()
+    v = vectors(2000, 1, torch.float16, 2)
+    cache.write(0, cache.extend(seqs, 2000), k, v)
+    step = cache.extend(seqs, 0)
+    q = torch.full((1, 4, 128), 0.5, dtype=torch.float16, device=DEV)
+    want, _, bound = formula(q[0], k, v)
+    assert ((cache.attend(0, step, q)[0].double() - want).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+def test_what_lies_behind_a_sequence_counts_for_nothing():
+    """Uninitialised parts of pages hold whatever was there: NaN scales, infinities."""
+    cache = PagedInt4Cache(1, 2, 8)
+    cache.pages.view(torch.int16).fill_(0x7E01)  # FP16 NaN in every parameter
+    seqs, k, v = fill(cache, [100, 7, 130], seed=17)
+    assert_attends(cache, seqs, k, v, 4)
+
+
+@pytest.mark.gpu
+def test_a_nan_reaches_its_sequence_and_head_only():
+    cache = PagedInt4Cache(1, 2, 8)
+    seqs, k, v = fill(cache, [100, 130], seed=19)
+    q = torch.randn(2, 8, 128, device=DEV).half()
+    clean = cache.attend(0, cache.extend(seqs, 0), q)
+    step = cache.extend(seqs, [1, 1])
+    nk, nv = vectors(2, 2, torch.float16, 1), vectors(2, 2, torch.float16, 2)
+    nk[0, 1, 3] = torch.nan
+    cache.write(0, step, nk, nv)
+    got = cache.attend(0, step, q)
+    assert got[0, 4:].isnan().all() and got[0, :4].isfinite().all() and got[1].isfinite().all()
+    assert clean.isfinite().all()
+    step = cache.extend(seqs, [1, 1])
+    nk[0, 1, 3], nv[1, 0, 100] = 0, torch.inf
+    cache.write(0, step, nk, nv)
+    got = cache.attend(0, step, q)
+    assert got[1, :4, 64:].isnan().all() and got[1, :4, :64].isfinite().all() and got[1, 4:].isfinite().all()
+
+
+@pytest.mark.gpu
+def test_query_layouts_streams_and_a_captured_call():
+    cache = PagedInt4Cache(1, 2, 40)
+    seqs, k, v = fill(cache, [1500, 20], seed=23)
+    step = cache.extend(seqs, 0)
+    fused = torch.randn(2, 12, 128, device=DEV).half()
+    q = fused[:, :8]
+    want = cache.attend(0, step, q.contiguous())
+    assert torch.equal(cache.attend(0, step, q), want)
+    assert torch.equal(cache.attend(0, step, q.transpose(0, 1).contiguous().transpose(0, 1)), want)
+    for _ in range(10):
+        assert torch.equal(cache.attend(0, step, q), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        here = cache.attend(0, step, q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            there = cache.attend(0, step, q)
+    torch.cuda.synchronize()
+    assert torch.equal(here, want)
+    fused.copy_(torch.randn_like(fused))
+    graph.replay()
+    assert torch.equal(there, cache.attend(0, step, q))
+
+
+@pytest.mark.gpu
+def test_pages_outside_the_pool_set_the_status_and_touch_nothing():
+    from reskv_b200._extension import host
+
+    cache = PagedInt4Cache(1, 1, 2)
+    cache.pages.fill_(3)
+    seqs = cache.add(1)
+    step = cache.extend(seqs, 70)
+    x = vectors(70, 1, torch.float16, 1)
+    for table in ([[0, 2]], [[0, -1]]):
+        bad = torch.tensor(table, dtype=torch.int32, device=DEV)
+        with pytest.raises(RuntimeError, match="status 0x2"):
+            host().paged_write(cache.pages, 0, cache._status, x, x, step.cu_seqlens, step.starts, bad)
+            cache.check()
+        assert (cache.pages[0, 1] == 3).all()
+        cache._status.zero_()
+        with pytest.raises(RuntimeError, match="status 0x2"):
+            host().paged_attention(cache.pages, 0, cache._status, x[:1], step.device_lengths, bad, None, False)
+            cache.check()
+        cache._status.zero_()
+    far = torch.tensor([200], dtype=torch.int32, device=DEV)  # tokens behind the table
+    with pytest.raises(RuntimeError, match="status 0x2"):
+        host().paged_read(cache.pages, 0, cache._status, False, step.cu_seqlens, far, step.table, 70)
+        cache.check()
+    cache._status.zero_()
+
+
+# ---- pages ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("layers,kv_heads,pages,pairs", [(1, 1, 2, 1), (3, 2, 40, 17), (2, 1, 1200, 600)])
+def test_copy_pages(layers, kv_heads, pages, pairs):
+    cache = PagedInt4Cache(layers, kv_heads, pages)
+    cache.pages.copy_(torch.randint(0, 256, cache.pages.shape, device=DEV, dtype=torch.uint8))
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(1)).tolist()
+    src, dst = order[:pairs], order[pairs:2 * pairs]
+    src[-1] = src[0]  # a source may serve several destinations
+    want = cache.pages.clone()
+    want[:, dst] = want[:, src]
+    cache.copy_pages(src, dst)
+    assert torch.equal(cache.pages, want)
+    cache.copy_pages([], [])
+
+
+@pytest.mark.gpu
+def test_forked_sequences_go_their_own_ways_and_survive_a_compaction():
+    cache = PagedInt4Cache(2, 2, 30)
+    seqs, k, v = fill(cache, [130, 64, 300], seed=29)
+    children = cache.fork([seqs[0], seqs[0], seqs[1]])
+    everyone = [seqs[0], seqs[2], *children]
+    ks, vs = [k[0], k[2], k[0], k[0], k[1]], [v[0], v[2], v[0], v[0], v[1]]
+    cache.free([seqs[1]])
+    for turn in range(3):
+        step = cache.extend(everyone, [1, 60, 2, 1, 3])
+        nk, nv = vectors(67, 2, torch.float16, 100 + turn), vectors(67, 2, torch.float16, 200 + turn)
+        for layer in range(2):
+            cache.write(layer, step, nk, nv)
+        at = np.concatenate(([0], np.cumsum(step.counts)))
+        ks = [torch.cat((x, nk[a:b])) for x, a, b in zip(ks, at, at[1:])]
+        vs = [torch.cat((x, nv[a:b])) for x, a, b in zip(vs, at, at[1:])]
+        if turn == 1:
+            before = cache.attend(1, step, torch.ones(5, 4, 128, dtype=torch.float16, device=DEV))
+            used = cache.compact()
+            assert used == cache.capacity - cache.free_pages
+            assert max(max(e.pages) for e in cache._book.sequences.values()) == used - 1
+            with pytest.raises(ValueError, match="moved"):
+                cache.attend(1, step, torch.ones(5, 4, 128, dtype=torch.float16, device=DEV))
+            again = cache.attend(1, cache.extend(everyone, 0), torch.ones(5, 4, 128, dtype=torch.float16, device=DEV))
+            assert (again - before).abs().max() < 2e-3  # other shares, another order of the sums
+    for layer in range(2):
+        assert_attends(cache, everyone, ks, vs, 4, layer=layer)
+    cache.free(everyone)
+    assert cache.free_pages == cache.capacity
+    cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_prompts_then_tokens(dtype):
+    """A batch as a server has it: packed prompts are attended to and stored, then every sequence takes tokens; each step's
+    attention is that over the stored values."""
+    cache = PagedInt4Cache(1, 2, 20, dtype=dtype)
+    seqs, lengths = cache.add(3), [200, 33, 64]
+    step = cache.extend(seqs, lengths)
+    q, k, v = vectors(297, 8, dtype, 1), vectors(297, 2, dtype, 2), vectors(297, 2, dtype, 3)
+    cache.write(0, step, k, v)
+    stored_k, stored_v = cache.read(0, step)
+    full = prompt_attention(q, stored_k, stored_v, step.cu_seqlens)
+    last = [t - 1 for t in step.cu_seqlens[1:].tolist()]
+    one = cache.attend(0, step, q[last])
+    u = torch.finfo(dtype).eps
+    # the prompt's attention reads the stored values rounded to the type and rounds its weights to it: a few steps of the type
+    assert (one.double() - full[last].double()).abs().max() <= 8 * u * stored_v.abs().max().double()
+    ks, vs = [list(x.split(lengths)) for x in (k, v)]
+    for turn in range(3):
+        step = cache.extend(seqs, 1)
+        nk, nv = vectors(3, 2, dtype, 10 + turn), vectors(3, 2, dtype, 20 + turn)
+        cache.write(0, step, nk, nv)
+        ks, vs = [torch.cat((x, y[None])) for x, y in zip(ks, nk)], [torch.cat((x, y[None])) for x, y in zip(vs, nv)]
+        assert_attends(cache, seqs, ks, vs, 4, seed=60 + turn)
+
+
+@pytest.mark.gpu
+def test_refusals():
+    for args in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (1, True, 1), (1.0, 1, 1)):
+        with pytest.raises(ValueError):
+            PagedInt4Cache(*args)
+    with pytest.raises(ValueError):
+        PagedInt4Cache(1, 1, 1, dtype=torch.float32)
+    with pytest.raises(ValueError):
+        PagedInt4Cache(1, 1, 1, device="cpu")
+    cache = PagedInt4Cache(1, 2, 4)
+    seqs = cache.add(2)
+    step = cache.extend(seqs, [3, 4])
+    x, q = vectors(7, 2, torch.float16, 1), vectors(2, 8, torch.float16, 2)
+    for key, value in ((x[:6], x[:6]), (x.bfloat16(), x.bfloat16()), (x, x[:6]), (x, x.float()), (x[:, :1], x[:, :1]), (x[..., :64], x[..., :64]),
+                       (x.cpu(), x.cpu()), (x.clone().requires_grad_(), x)):
+        with pytest.raises(ValueError):
+            cache.write(0, step, key, value)
+    for layer in (-1, 1):
+        with pytest.raises(ValueError):
+            cache.write(layer, step, x, x)
+    for bad in (q[:1], q.float(), q[:, :3], q[..., :64], vectors(2, 18, torch.float16, 2), q.cpu(), q.clone().requires_grad_()):
+        with pytest.raises(ValueError):
+            cache.attend(0, step, bad)
+    for scaling in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            cache.attend(0, step, q, scaling=scaling)
+    with pytest.raises(TypeError):
+        cache.attend(0, None, q)
+    other = PagedInt4Cache(1, 2, 4)
+    with pytest.raises(ValueError, match="another cache"):
+        other.attend(0, step, q)
+    for src, dst in (([0], [4]), ([0], []), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([0.0], [1])):
+        with pytest.raises(ValueError):
+            cache.copy_pages(src, dst)
+    cache.extend([seqs[0]], 1)  # the older step is out of date now
+    with pytest.raises(ValueError, match="extended"):
+        cache.write(0, step, x, x)
+    with pytest.raises(RuntimeError, match="out of pages"):
+        cache.extend([seqs[0]], 1000)
+    step = cache.extend(seqs, 1)
+    cache.fork([seqs[0]])
+    with pytest.raises(ValueError):
+        cache.write(0, step, x[:2], x[:2])
