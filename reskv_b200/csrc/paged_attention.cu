@@ -9,9 +9,11 @@
 // its 144 bytes take to arrive.
 //
 // Work: the pages of all (sequence, KV head) units lie end to end and every CTA takes an equal share; a unit that lies in one
-// CTA is finished there, the parts of the others are added by a second kernel.  Eight warps take a segment's blocks of 16 tokens
-// in turn, each through a ring of its own (one bulk copy of 2304 bytes per block) with a running softmax of its own; they meet
+// CTA is finished there, the parts of the others are added by a second kernel.  Eight warps take a segment's chunks of 32 tokens
+// in turn, each through a ring of its own (one bulk copy of 4608 bytes per chunk) with a running softmax of its own; they meet
 // in shared memory at a segment's end.
+#include <algorithm>
+
 #include "paged_int4.cuh"
 
 namespace reskv {
@@ -19,11 +21,16 @@ namespace {
 
 constexpr int kPaWarps = 8;
 constexpr int kPaThreads = kPaWarps * 32;
-constexpr int kPaStages = 4;
+constexpr int kPaStages = 2;
+constexpr int kChunkBlocks = 2, kChunkTokens = kChunkBlocks * kBlockTokens, kChunkBytes = kChunkBlocks * kBlockBytes;  // a warp's turn
 constexpr int kPaPerSm = 2;                       // CTAs of an SM
-constexpr int kPaLeast = 2;                       // pages of a share, at least: one block for every warp
+constexpr int kPageChunks = kPageTokens / kChunkTokens;
+constexpr int kPaCharge = 3;                      // a segment costs as much as that many pages besides its own
+constexpr int kPaLeast = 2 * kPaCharge;           // a share is at least that long
 constexpr int kPaSumBytes = kPaWarps * kPagedGroup * kHeadDim * 4;
-constexpr int kPaSmem = kPaWarps * kPaStages * kBlockBytes + kPaSumBytes;
+constexpr int kPaSmem = kPaWarps * kPaStages * kChunkBytes + kPaSumBytes;
+constexpr float kCodeMiddle = 7.5f;
+constexpr int kPaSlack = 5;
 constexpr int kPartialFloats = kPagedGroup * (kHeadDim + 2);  // of a part: outputs [8][128], maxima [8], sums [8]
 
 struct PagedParams {
@@ -47,53 +54,63 @@ __device__ __forceinline__ int length_of(const PagedParams& p, int s) {
 }
 __device__ __forceinline__ int pages_of(int length) { return (length + kPageTokens - 1) / kPageTokens; }
 
-// How the pages of all units, laid end to end, are dealt out; the same for both kernels.
+// How the work is dealt out; the same for both kernels.  All units are laid end to end, each with its pages behind a charge of
+// kPaCharge (what a segment costs besides them: the query, the first block's latency, the meeting of the warps), and every CTA
+// takes an equal stretch.
 struct Shares {
-    int64_t pages;
+    int64_t all;
     int ctas;
-    __device__ __forceinline__ int64_t begin(int cta) const { return cta * pages / ctas; }
-    __device__ __forceinline__ int owner(int64_t page) const { return static_cast<int>(((page + 1) * ctas - 1) / pages); }
+    __device__ __forceinline__ int64_t begin(int cta) const { return cta * all / ctas; }
+    __device__ __forceinline__ int owner(int64_t place) const { return static_cast<int>(((place + 1) * ctas - 1) / all); }
 };
-__device__ __forceinline__ Shares shares_of(const PagedParams& p, int lane) {
+__device__ __forceinline__ int stretch_of(int length) { return length > 0 ? pages_of(length) + kPaCharge : 0; }
+__device__ __forceinline__ Shares shares_of(const PagedParams& p, int64_t of_one_head) {
+    const int64_t all = of_one_head * p.heads, most = (all + kPaLeast - 1) / kPaLeast;
+    return {all, static_cast<int>(most < p.ctas ? most : p.ctas)};
+}
+__device__ __forceinline__ Shares count_shares(const PagedParams& p, int lane) {
     int64_t n = 0;
-    for (int s = lane; s < p.sequences; s += 32) n += pages_of(length_of(p, s));
+    for (int s = lane; s < p.sequences; s += 32) n += stretch_of(length_of(p, s));
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
-    n *= p.heads;
-    const int64_t most = (n + kPaLeast - 1) / kPaLeast;
-    return {n, static_cast<int>(most < p.ctas ? most : p.ctas)};
+    return shares_of(p, n);
 }
 
-// A unit's consecutive pages inside a share, one segment after the other.
+// The segments of a share, one after the other: consecutive pages of a unit.
 struct Segments {
     int sequence, head, length, first, last;
-    int64_t left;  // pages of the share behind this segment
-    // The segment that holds page `page` of all; whole warp.
-    __device__ __forceinline__ void start(const PagedParams& p, int64_t page, int64_t count, int lane) {
+    int64_t left;  // of the share behind this segment
+    // From place `place` on, `count` long; whole warp.  The first segment may be empty (first == last).
+    __device__ __forceinline__ void start(const PagedParams& p, int64_t place, int64_t count, int lane) {
         int64_t before = 0;
+        left = -1;
         for (int s0 = 0; s0 < p.sequences; s0 += 32) {
             const int n = s0 + lane < p.sequences ? length_of(p, s0 + lane) : 0;
-            const int64_t mine = static_cast<int64_t>(pages_of(n)) * p.heads;
+            const int64_t mine = static_cast<int64_t>(stretch_of(n)) * p.heads;
             int64_t upto = mine;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
                 const int64_t other = __shfl_up_sync(0xffffffffu, upto, off);
                 if (lane >= off) upto += other;
             }
-            const uint32_t mask = __ballot_sync(0xffffffffu, before + upto > page);
+            const uint32_t mask = __ballot_sync(0xffffffffu, before + upto > place);
             if (mask) {
                 const int owner = __ffs(mask) - 1;
                 length = __shfl_sync(0xffffffffu, n, owner);
-                const int64_t at = page - (before + __shfl_sync(0xffffffffu, upto - mine, owner));
-                const int per = pages_of(length);
-                sequence = s0 + owner, head = static_cast<int>(at / per), first = static_cast<int>(at - static_cast<int64_t>(head) * per);
-                last = static_cast<int64_t>(per - first) < count ? per : first + static_cast<int>(count);
-                left = count - (last - first);
+                const int64_t at = place - (before + __shfl_sync(0xffffffffu, upto - mine, owner));
+                const int per = stretch_of(length);
+                sequence = s0 + owner, head = static_cast<int>(at / per);
+                take(static_cast<int>(at - static_cast<int64_t>(head) * per), count);
                 return;
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
         }
-        left = -1;  // not reached: the page lies in some sequence
+    }
+    // What `count` from offset `from` of the unit's stretch on holds of it.
+    __device__ __forceinline__ void take(int from, int64_t count) {
+        const int per = stretch_of(length), to = per - from < count ? per : from + static_cast<int>(count);
+        first = from > kPaCharge ? from - kPaCharge : 0, last = to > kPaCharge ? to - kPaCharge : 0;
+        left = count - (to - from);
     }
     __device__ __forceinline__ bool next(const PagedParams& p) {
         if (left <= 0) return false;
@@ -104,15 +121,12 @@ struct Segments {
                 length = length_of(p, sequence);
             } while (length == 0);
         }
-        first = 0;
-        const int per = pages_of(length);
-        last = per < left ? per : static_cast<int>(left);
-        left -= last;
+        take(0, left);
         return true;
     }
-    __device__ __forceinline__ int first_block() const { return first * (kPageTokens / kBlockTokens); }
-    __device__ __forceinline__ int last_block() const {
-        const int all = (length + kBlockTokens - 1) / kBlockTokens, end = last * (kPageTokens / kBlockTokens);
+    __device__ __forceinline__ int first_chunk() const { return first * kPageChunks; }
+    __device__ __forceinline__ int last_chunk() const {
+        const int all = (length + kChunkTokens - 1) / kChunkTokens, end = last * kPageChunks;
         return all < end ? all : end;
     }
 };
@@ -123,14 +137,57 @@ __device__ __forceinline__ int clamped(int x, int low, int high) { return x < lo
 
 __device__ __forceinline__ void ctas_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kPaThreads) : "memory"); }
 
+// mma_16816 with nothing to add to.
+__device__ __forceinline__ void mma_16816_start(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Tokens' offsets (a0: token g, a1: token g + 8, groups 0 and 1, the same in every lane of a quad) times the parts of the sums of q
+// that the lanes of a quad hold, in the type of the model.
 template <bool BF16>
-__device__ __forceinline__ uint32_t larger_pair(uint32_t a, uint32_t b) {
-    uint32_t r;
+__device__ __forceinline__ void mma_offsets(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
     if (BF16)
-        asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
     else
-        asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
+}
+
+// An 8 x 8 matrix of 16-bit numbers, two of a row per lane, with rows and columns exchanged.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// Two FP32 numbers per instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
+}
+
+struct Requests {
+    Segments segment;           // behind the one that is being requested; left < 0: none
+    const int* entry;           // in the table, of the chunk after the next
+    const unsigned char* base;  // of the head and the chunk's place in page 0
+    int chunks, page;           // left to request of the segment (-1: none at all), page of the next one
+};
+
+// The warp's next segment, in shared memory; whole warp.
+__device__ __forceinline__ bool next_segment(const PagedParams& p, Segments& at, int lane) {
+    bool any = false;
+    __syncwarp();
+    if (lane == 0) any = at.next(p);
+    return __shfl_sync(0xffffffffu, any, 0);
 }
 
 template <bool BF16>
@@ -138,9 +195,11 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint64_t bar_full[kPaWarps][kPaStages];
     __shared__ float s_max[kPaWarps][kPagedGroup], s_sum[kPaWarps][kPagedGroup], s_top[kPagedGroup];
+    __shared__ Segments s_at[kPaWarps];
+    __shared__ Requests s_ahead[kPaWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    unsigned char* ring = smem + warp * kPaStages * kBlockBytes;
-    float* sums = reinterpret_cast<float*>(smem + kPaWarps * kPaStages * kBlockBytes);  // [warp][head][128]
+    unsigned char* ring = smem + warp * kPaStages * kChunkBytes;
+    float* sums = reinterpret_cast<float*>(smem + kPaWarps * kPaStages * kChunkBytes);  // [warp][head][128]
     if (lane == 0) {
         for (int s = 0; s < kPaStages; ++s) mbar_init(&bar_full[warp][s], 1);
         mbar_fence_init();
@@ -148,52 +207,70 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
     __syncwarp();
     wait_for_previous_launch();
     let_next_launch_start();
-    const Shares shares = shares_of(p, lane);
+    const Shares shares = count_shares(p, lane);
     if (static_cast<int>(blockIdx.x) >= shares.ctas) return;
     const int64_t begin = shares.begin(blockIdx.x), count = shares.begin(blockIdx.x + 1) - begin;
-    Segments at;  // being worked on
-    at.start(p, begin, count, lane);
-    Segments ahead = at;  // being requested
-    int ahead_block = ahead.first_block() + warp, ahead_end = ahead.last_block();
-    bool more = true, lost = false;
-    int page = -1;
-    const auto look = [&] {  // the page of the block that is requested next
-        while (more && ahead_block >= ahead_end) {
-            more = ahead.next(p);
-            ahead_block = ahead.first_block() + warp, ahead_end = ahead.last_block();
+    // A warp's places in its list of segments, the one that is worked on and the one whose chunks are requested, are in shared
+    // memory: registers are scarce.
+    Segments& at = s_at[warp];
+    Requests& ahead = s_ahead[warp];
+    {
+        Segments first{};
+        first.start(p, begin, count, lane);
+        if (lane == 0) at = first, ahead.segment = first, ahead.chunks = 0;
+        __syncwarp();
+    }
+    // Requests run ahead of the work (lane 0).  A warp's chunks are kPaWarps apart, so they lie at the same place of their pages.
+    // The number of the next page is under way into shared memory while a chunk is worked on.
+    const auto look = [&] {
+        while (ahead.chunks == 0) {
+            if (ahead.segment.left < 0) {
+                ahead.chunks = -1;
+                return;
+            }
+            const int first = ahead.segment.first_chunk() + warp, end = ahead.segment.last_chunk();
+            if (end > first) {
+                ahead.chunks = (end - first + kPaWarps - 1) / kPaWarps;
+                ahead.entry = p.table + static_cast<int64_t>(ahead.segment.sequence) * p.width + first / kPageChunks;
+                ahead.base = p.pages + static_cast<int64_t>(ahead.segment.head) * kPageHeadBytes + (first & (kPageChunks - 1)) * kChunkBytes;
+            }
+            if (!ahead.segment.next(p)) ahead.segment.left = -1;
         }
-        if (more) page = p.table[static_cast<int64_t>(ahead.sequence) * p.width + ahead_block / (kPageTokens / kBlockTokens)];
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&ahead.page)), "l"(ahead.entry) : "memory");
+        ahead.entry += kPaWarps / kPageChunks;
     };
     const auto request = [&](int stage) {
-        if (!more) return;
-        if (page < 0 || page >= p.page_count) {
-            if (lane == 0) atomicOr(p.status, RESKV_STATUS_STATE_RANGE);
+        if (ahead.chunks < 0) return;
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        int page = *static_cast<volatile int*>(&ahead.page);
+        if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.page_count)) {
+            atomicOr(p.status, RESKV_STATUS_STATE_RANGE);
             page = 0;
         }
-        if (lane == 0) {
-            mbar_arrive_expect_tx(&bar_full[warp][stage], kBlockBytes);
-            bulk_g2s(ring + stage * kBlockBytes, p.pages + (static_cast<int64_t>(page) * p.heads + ahead.head) * kPageHeadBytes +
-                                                     (ahead_block & (kPageTokens / kBlockTokens - 1)) * kBlockBytes,
-                     kBlockBytes, &bar_full[warp][stage]);
-        }
-        ahead_block += kPaWarps;
+        mbar_arrive_expect_tx(&bar_full[warp][stage], kChunkBytes);
+        bulk_g2s(ring + stage * kChunkBytes, ahead.base + page * (static_cast<int64_t>(p.heads) * kPageHeadBytes), kChunkBytes, &bar_full[warp][stage]);
+        --ahead.chunks;
         look();
     };
-    look();
-#pragma unroll
-    for (int s = 0; s < kPaStages; ++s) request(s);
+    bool lost = false;
+    if (lane == 0) {
+        look();
+#pragma unroll 1
+        for (int s = 0; s < kPaStages; ++s) request(s);
+    }
 
-    // rows of a block that this lane's columns 2t, 2t + 1 of the scores stand for: a score tile's column n is row
-    // n / 2 (n even) or 4 + (n / 2 ^ 1) (n odd) of its eight
-    const int row_even = t, row_odd = 4 + (t ^ 1), key_row = (g >> 1) ^ (g & 1 ? 5 : 0);
+    // Row n of a tile of eight tokens is row n / 2 (n even) or 4 + (n / 2 ^ 1) (n odd) of the block's eight: the rows that the lanes
+    // of a quad read together (tokens 2t, 2t + 1 of the contraction with the values) lie on different banks.
+    const int row_even = t, row_odd = 4 + (t ^ 1), own_row = (g >> 1) ^ (g & 1 ? 5 : 0);
     int stage = 0, phase = 0;
     bool first_segment = true;
-    for (bool any = true; any; any = at.next(p), first_segment = false) {
+    for (bool any = true; any; any = next_segment(p, at, lane)) {
+        if (at.first == at.last) continue;
         // ---- the query: head g's coordinates 32 j + 8 t .. + 7, scaled by a power of two that makes the largest about 2^9 ------
-        uint32_t q_low[4][2], q_high[4][2];
-        float q_sum[2] = {0.f, 0.f}, q_scale;
+        uint32_t q_low[4][2], q_high[4][2], q_sums;
+        float q_scale[2];  // of heads 2t, 2t + 1: of the scores as they come from the products
         {
-            float v[4][8], top = 0.f;
+            float v[4][8], top = 0.f, sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint4 raw = make_uint4(0, 0, 0, 0);
@@ -204,16 +281,16 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
                 for (int e = 0; e < 4; ++e) {
                     v[j][2 * e] = low_of<BF16>(pairs[e]), v[j][2 * e + 1] = high_of<BF16>(pairs[e]);
                     top = fmaxf(top, fmaxf(fabsf(v[j][2 * e]), fabsf(v[j][2 * e + 1])));
-                    q_sum[j >> 1] += v[j][2 * e] + v[j][2 * e + 1];
+                    sum[j >> 1] += v[j][2 * e] + v[j][2 * e + 1];
                 }
             }
 #pragma unroll
             for (int off = 1; off < 4; off <<= 1) {
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-                q_sum[0] += __shfl_xor_sync(0xffffffffu, q_sum[0], off);
-                q_sum[1] += __shfl_xor_sync(0xffffffffu, q_sum[1], off);
+                sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], off);
+                sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], off);
             }
-            const int up = clamped(9 - exponent_of(top), -118, 100);
+            const int up = clamped(9 - exponent_of(top), -100, 100);
             const float by = power_of_two(up);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -222,149 +299,201 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
                     q_low[j][e] = pack2<false>(v[j][2 * e] * by, v[j][2 * e + 4] * by);
                     q_high[j][e] = pack2<false>(v[j][2 * e + 1] * by * 0.0625f, v[j][2 * e + 5] * by * 0.0625f);
                 }
-            q_scale = p.scale_log2 * power_of_two(24) / by;
-            q_sum[0] *= p.scale_log2, q_sum[1] *= p.scale_log2;
+            // A quarter of the sums (below 2^14), against the offsets: the lanes of a quad hold what one 16-bit number leaves of
+            // them (FP16: two parts, BF16: three), each against the same offsets
+            sum[0] *= 0.25f * by, sum[1] *= 0.25f * by;
+            q_sums = 0;
+#pragma unroll
+            for (int part = 0; part < (BF16 ? 3 : 2); ++part) {
+                const uint32_t pair = pack2<BF16>(sum[0], sum[1]);
+                if (t == part) q_sums = pair;
+                sum[0] -= low_of<BF16>(pair), sum[1] -= high_of<BF16>(pair);
+            }
+            const float mine = 4.f * p.scale_log2 / by;
+            q_scale[0] = __shfl_sync(0xffffffffu, mine, 8 * t), q_scale[1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
         }
 
-        float m = -INFINITY, l = 0.f, flat[2] = {0.f, 0.f};  // of head g: maximum, sum, sum of p * offset
-        float acc[8][4];                                    // outputs: rows = coordinates, columns = heads 2t, 2t + 1
+        // Of heads 2t and 2t + 1, over the lane's tokens: sums of p, per group of p * offset, and of what p * scale lost when it
+        // was rounded.  They and the outputs are in units of 2^-unit_up, which keeps p * scale where FP16 is exact to half a step.
+        // m may lag behind the maximum by kPaSlack powers of two: fewer rescalings.
+        float m[2] = {-INFINITY, -INFINITY}, shift[2] = {INFINITY, INFINITY};  // shift: unit_up - m * q_scale
+        float most_power = 0.f, unit_limit = -1.f;                             // the largest power of two that a p may get; scale
+        int unit_up = 0;
+        float2 l = make_float2(0.f, 0.f), flat[2] = {l, l}, lost_weight[2] = {l, l};
+        float acc[8][4];  // rows = coordinates, columns = heads 2t, 2t + 1
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-        float value_scale = 1.f, scale_limit = -1.f;        // p * scale * value_scale stays in FP16's range up to that scale
-        const int end = at.last_block();
-        for (int block = at.first_block() + warp; block < end; block += kPaWarps) {
+        const int end = at.last_chunk(), start = at.first_chunk() + warp;
+        int tokens = at.length - start * kChunkTokens;  // from this chunk on
+        for (int chunks = end - start; chunks > 0; chunks -= kPaWarps, tokens -= kPaWarps * kChunkTokens) {
             if (!lost) lost = !mbar_wait(&bar_full[warp][stage], phase);
-            const unsigned char* keys = ring + stage * kBlockBytes;
-            const unsigned char* values = keys + kBlockSide;
-            // ---- scores of 2 x 8 tokens ---------------------------------------------------------------------------------
-            float s[2][2];
-            const int tokens = at.length - block * kBlockTokens;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint4 w = *reinterpret_cast<const uint4*>(keys + (8 * i + key_row) * 64 + 16 * t);
-                const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-                float c[2][4];
+            for (int b = 0; b < kChunkBlocks; ++b) {
+                unsigned char* keys = ring + stage * kChunkBytes + b * kBlockBytes + own_row * 64 + 16 * t;
+                unsigned char* values = ring + stage * kChunkBytes + b * kBlockBytes + kBlockSide;
+                unsigned char* own = values + kBlockCodes + own_row * 8;  // parameters of the lane's tokens: here and 64 bytes on
+                const int live = tokens - b * kBlockTokens;
+                if (live <= 0) break;
+                // ---- scores: rows = tokens g, g + 8, columns = heads: (scale . (q . code) 2^22 + offset . sum(q) / 4) * q_scale ----
+                float s[4];
+                {
+                    const uint4 w0 = *reinterpret_cast<const uint4*>(keys), w1 = *reinterpret_cast<const uint4*>(keys + 8 * 64);
+                    const uint32_t words[2][4] = {{w0.x, w0.y, w0.z, w0.w}, {w1.x, w1.y, w1.z, w1.w}};
+                    const uint2 param[2] = {*reinterpret_cast<const uint2*>(own - kBlockSide), *reinterpret_cast<const uint2*>(own - kBlockSide + 64)};
+                    float c[2][4], offsets[4];
+                    mma_offsets<BF16>(offsets, param[0].y, param[1].y, q_sums);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float(&d)[4] = c[j >> 1];
-                    if ((j & 1) == 0) d[0] = d[1] = d[2] = d[3] = 0.f;
-                    const uint32_t next = words[j] >> 8;
-                    mma_16816(d, q_low[j][0], 0u, q_high[j][0], 0u, words[j] & 0x000F000Fu, words[j] & 0x00F000F0u);
-                    mma_16816(d, q_low[j][1], 0u, q_high[j][1], 0u, next & 0x000F000Fu, next & 0x00F000F0u);
+                    for (int j = 0; j < 4; ++j) {
+                        float(&d)[4] = c[j >> 1];
+                        const uint32_t x = words[0][j], y = words[1][j], x8 = x >> 8, y8 = y >> 8;
+                        if (j & 1)
+                            mma_16816(d, x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q_low[j][0], q_high[j][0]);
+                        else
+                            mma_16816_start(d, x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q_low[j][0], q_high[j][0]);
+                        mma_16816(d, x8 & 0x000F000Fu, y8 & 0x000F000Fu, x8 & 0x00F000F0u, y8 & 0x00F000F0u, q_low[j][1], q_high[j][1]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float scale0 = low_of<BF16>(param[i].x), scale1 = high_of<BF16>(param[i].x);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            s[2 * i + h] = fmaf(fmaf(c[0][2 * i + h], scale0, c[1][2 * i + h] * scale1), 1 << 22, offsets[2 * i + h]);
+                    }
                 }
-                const unsigned char* params = keys + kBlockCodes + 64 * i;
-                const uint2 even = *reinterpret_cast<const uint2*>(params + 8 * row_even), odd = *reinterpret_cast<const uint2*>(params + 8 * row_odd);
-                s[i][0] = (c[0][0] * low_of<BF16>(even.x) + c[1][0] * high_of<BF16>(even.x)) * q_scale +
-                          (q_sum[0] * low_of<BF16>(even.y) + q_sum[1] * high_of<BF16>(even.y));
-                s[i][1] = (c[0][1] * low_of<BF16>(odd.x) + c[1][1] * high_of<BF16>(odd.x)) * q_scale +
-                          (q_sum[0] * low_of<BF16>(odd.y) + q_sum[1] * high_of<BF16>(odd.y));
-            }
-            uint2 params[2][2];
+                if (live < kBlockTokens) {  // behind the sequence's end: whatever lies there counts for nothing
+                    __syncwarp();
+                    if (lane < kBlockTokens && lane >= live) {
+                        *reinterpret_cast<uint2*>(values + kBlockCodes + lane * 8) = make_uint2(0, 0);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next copy to this place comes behind it
+                    }
+                    __syncwarp();
+                    if (own_row >= live) s[0] = s[1] = -INFINITY;
+                    if (own_row + 8 >= live) s[2] = s[3] = -INFINITY;
+                }
+                float scale[2][2], offset[2][2];  // [token][group]
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                params[i][0] = *reinterpret_cast<const uint2*>(values + kBlockCodes + 8 * (8 * i + row_even));
-                params[i][1] = *reinterpret_cast<const uint2*>(values + kBlockCodes + 8 * (8 * i + row_odd));
-            }
-            if (tokens < kBlockTokens) {  // behind the sequence's end: whatever lies there counts for nothing
+                for (int i = 0; i < 2; ++i) {
+                    const uint2 param = *reinterpret_cast<const uint2*>(own + 64 * i);
+                    scale[i][0] = low_of<BF16>(param.x), scale[i][1] = high_of<BF16>(param.x);
+                    offset[i][0] = low_of<BF16>(param.y), offset[i][1] = high_of<BF16>(param.y);
+                }
+                // ---- running softmax; the unit follows the largest scale (BF16: or 2^-30 of an offset, so that a sum of offsets stays
+                // in range where all scales are 0) ------------------------------------------------------------------------------------
+                float most = fmaxf(fmaxf(scale[0][0], scale[0][1]), fmaxf(scale[1][0], scale[1][1]));
+                if (BF16) most = fmaxf(most, 0x1p-30f * fmaxf(fmaxf(fabsf(offset[0][0]), fabsf(offset[0][1])), fmaxf(fabsf(offset[1][0]), fabsf(offset[1][1]))));
+                float power[4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < 4; ++i) power[i] = fmaf(s[i], q_scale[i & 1], shift[i & 1]);
+                if (__any_sync(0xffffffffu, fmaxf(fmaxf(power[0], power[1]), fmaxf(power[2], power[3])) > most_power || most > unit_limit)) {
+                    float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        if (8 * i + (e ? row_odd : row_even) >= tokens) s[i][e] = -INFINITY, params[i][e] = make_uint2(0, 0);
-            }
-            // ---- running softmax --------------------------------------------------------------------------------------------
-            float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            if (__any_sync(0xffffffffu, top > m)) {
-                const float next = fmaxf(m, top), factor = m == next ? 1.f : fast_exp2(m - next);
-                m = next, l *= factor, flat[0] *= factor, flat[1] *= factor;
-                const float f0 = __shfl_sync(0xffffffffu, factor, 8 * t), f1 = __shfl_sync(0xffffffffu, factor, 8 * t + 4);
+                    for (int off = 4; off < 32; off <<= 1) {
+                        top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
+                        top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+                    }
+                    float change = 1.f;
+                    if (most > unit_limit) {  // the same in every lane
+                        const int e = clamped(exponent_of(most), -60, 100);
+                        const int now = 14 - kPaSlack - e;  // a scale up to 2^(e + 1) times a p up to 2^kPaSlack, 2^15 at most
+                        if (unit_limit >= 0.f) change = power_of_two(clamped(now - unit_up, -126, 126));  // else: nothing summed up yet
+                        unit_up = now, most_power = static_cast<float>(now + kPaSlack), unit_limit = power_of_two(e + 1);
+                    }
+                    float factor[2];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[i][0] *= f0, acc[i][1] *= f1, acc[i][2] *= f0, acc[i][3] *= f1;
-            }
-            // ---- the scales of the values: a power of two keeps p * scale where FP16 is exact to half a step -------------------
-            {
-                const uint32_t pair = larger_pair<BF16>(larger_pair<BF16>(params[0][0].x, params[0][1].x), larger_pair<BF16>(params[1][0].x, params[1][1].x));
-                float most = fmaxf(low_of<BF16>(pair), high_of<BF16>(pair));
-                if (__any_sync(0xffffffffu, most > scale_limit)) {
-                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                    const int e = clamped(exponent_of(most), -100, 126);
-                    const float now = power_of_two(14 - e > 126 ? 126 : 14 - e), change = scale_limit < 0.f ? 0.f : now / value_scale;
-                    value_scale = now, scale_limit = power_of_two(e + 1 > 127 ? 127 : e + 1);
-                    if (scale_limit < 0.f) scale_limit = 0.f;
+                    for (int h = 0; h < 2; ++h) {
+                        const float next = fmaxf(m[h], top[h]);
+                        factor[h] = (m[h] == next ? 1.f : fast_exp2((m[h] - next) * q_scale[h])) * change;
+                        m[h] = next;
+                        shift[h] = static_cast<float>(unit_up) - next * q_scale[h];
+                        power[h] = fmaf(s[h], q_scale[h], shift[h]), power[2 + h] = fmaf(s[2 + h], q_scale[h], shift[h]);
+                    }
+                    l.x *= factor[0], l.y *= factor[1];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[i][0] *= change, acc[i][1] *= change, acc[i][2] *= change, acc[i][3] *= change;
+                    for (int i = 0; i < 2; ++i) {
+                        flat[i].x *= factor[0], flat[i].y *= factor[1];
+                        lost_weight[i].x *= factor[0], lost_weight[i].y *= factor[1];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) acc[i][0] *= factor[0], acc[i][1] *= factor[1], acc[i][2] *= factor[0], acc[i][3] *= factor[1];
+                }
+                // ---- weights: rows = tokens, turned round for the contraction over them --------------------------------------------
+                uint32_t weights[2][2];  // [group][half of the block's tokens]
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float2 weight = make_float2(fast_exp2(power[2 * i]), fast_exp2(power[2 * i + 1]));
+                    l = add2(l, weight);
+#pragma unroll
+                    for (int group = 0; group < 2; ++group) {
+                        const float2 w = make_float2(weight.x * scale[i][group], weight.y * scale[i][group]);
+                        const uint32_t pair = pack2<false>(w.x, w.y);
+                        weights[group][i] = transposed(pair);
+                        lost_weight[group] = add2(lost_weight[group], make_float2(w.x - low_of<false>(pair), w.y - high_of<false>(pair)));
+                        flat[group].x = fmaf(weight.x, offset[i][group], flat[group].x), flat[group].y = fmaf(weight.y, offset[i][group], flat[group].y);
+                    }
+                }
+                // ---- outputs --------------------------------------------------------------------------------------------------------
+                uint2 rows[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = 8 * (i >> 1) + (i & 1 ? row_odd : row_even);
+                    rows[i] = *reinterpret_cast<const uint2*>(values + row * 64 + 8 * (g ^ ((row >> 1 & 1) << 2)));
+                }
+#pragma unroll
+                for (int group = 0; group < 2; ++group) {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {  // bytes 0, 1 and 2, 3 of the words
+                        const uint32_t pick = half ? 0x7632u : 0x5410u;
+                        const uint32_t x = __byte_perm(group ? rows[0].y : rows[0].x, group ? rows[1].y : rows[1].x, pick), x8 = x >> 8;
+                        const uint32_t y = __byte_perm(group ? rows[2].y : rows[2].x, group ? rows[3].y : rows[3].x, pick), y8 = y >> 8;
+                        mma_16816(acc[group * 4 + half * 2], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, weights[group][0], weights[group][1]);
+                        mma_16816(acc[group * 4 + half * 2 + 1], x8 & 0x000F000Fu, x8 & 0x00F000F0u, y8 & 0x000F000Fu, y8 & 0x00F000F0u, weights[group][0], weights[group][1]);
+                    }
                 }
             }
-            uint32_t weights[2][2];  // [group][half of the tokens]
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float p0 = fast_exp2(s[i][0] - m), p1 = fast_exp2(s[i][1] - m);
-                l += p0 + p1;
-                const float n0 = p0 * value_scale, n1 = p1 * value_scale;
-                weights[0][i] = pack2<false>(n0 * low_of<BF16>(params[i][0].x), n1 * low_of<BF16>(params[i][1].x));
-                weights[1][i] = pack2<false>(n0 * high_of<BF16>(params[i][0].x), n1 * high_of<BF16>(params[i][1].x));
-                flat[0] = fmaf(p0, low_of<BF16>(params[i][0].y), fmaf(p1, low_of<BF16>(params[i][1].y), flat[0]));
-                flat[1] = fmaf(p0, high_of<BF16>(params[i][0].y), fmaf(p1, high_of<BF16>(params[i][1].y), flat[1]));
-            }
-            // ---- outputs ------------------------------------------------------------------------------------------------------
-            uint2 rows[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 8 * (i >> 1) + (i & 1 ? row_odd : row_even);
-                rows[i] = *reinterpret_cast<const uint2*>(values + row * 64 + 8 * (g ^ ((row >> 1 & 1) << 2)));
-            }
-#pragma unroll
-            for (int group = 0; group < 2; ++group)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {  // bytes 0, 1 and 2, 3 of the words
-                    const uint32_t pick = half ? 0x7632u : 0x5410u;
-                    const uint32_t a = __byte_perm(group ? rows[0].y : rows[0].x, group ? rows[1].y : rows[1].x, pick);
-                    const uint32_t b = __byte_perm(group ? rows[2].y : rows[2].x, group ? rows[3].y : rows[3].x, pick);
-                    const uint32_t a8 = a >> 8, b8 = b >> 8;
-                    mma_16816(acc[group * 4 + half * 2], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, weights[group][0], weights[group][1]);
-                    mma_16816(acc[group * 4 + half * 2 + 1], a8 & 0x000F000Fu, a8 & 0x00F000F0u, b8 & 0x000F000Fu, b8 & 0x00F000F0u, weights[group][0], weights[group][1]);
-                }
             __syncwarp();
-            request(stage);
+            if (lane == 0) request(stage);
             if (++stage == kPaStages) stage = 0, phase ^= 1;
         }
         // ---- the warps' parts of the segment ------------------------------------------------------------------------------------
+        const auto over_tokens = [](float2 x) {
 #pragma unroll
-        for (int off = 1; off < 4; off <<= 1) {
-            l += __shfl_xor_sync(0xffffffffu, l, off);
-            flat[0] += __shfl_xor_sync(0xffffffffu, flat[0], off), flat[1] += __shfl_xor_sync(0xffffffffu, flat[1], off);
-        }
-        if (t == 0) s_max[warp][g] = m;
+            for (int off = 4; off < 32; off <<= 1)
+                x.x += __shfl_xor_sync(0xffffffffu, x.x, off), x.y += __shfl_xor_sync(0xffffffffu, x.y, off);
+            return x;
+        };
+        l = over_tokens(l);
+        m[0] *= q_scale[0], m[1] *= q_scale[1];  // from here on in powers of two
+        if (g == 0) s_max[warp][2 * t] = m[0], s_max[warp][2 * t + 1] = m[1];
         ctas_sync();
-        const int active = min(kPaWarps, end - at.first_block());
-        float top = s_max[0][g];
-        for (int w = 1; w < active; ++w) top = fmaxf(top, s_max[w][g]);
+        const int active = min(kPaWarps, end - at.first_chunk());
+        float top[2] = {s_max[0][2 * t], s_max[0][2 * t + 1]};
+        for (int w = 1; w < active; ++w) top[0] = fmaxf(top[0], s_max[w][2 * t]), top[1] = fmaxf(top[1], s_max[w][2 * t + 1]);
         if (warp < active) {
-            const float weight = m == top ? 1.f : fast_exp2(m - top);
-            if (t == 0) s_sum[warp][g] = l * weight;
-            const float w0 = __shfl_sync(0xffffffffu, weight, 8 * t), w1 = __shfl_sync(0xffffffffu, weight, 8 * t + 4);
-            float flats[2][2];
+            const float unit = power_of_two(-unit_up);
+            const float weight[2] = {m[0] == top[0] ? 1.f : fast_exp2(m[0] - top[0]), m[1] == top[1] ? 1.f : fast_exp2(m[1] - top[1])};
+            if (g == 0) s_sum[warp][2 * t] = l.x * unit * weight[0], s_sum[warp][2 * t + 1] = l.y * unit * weight[1];
+            // A value is offset + kCodeMiddle * scale + (code - kCodeMiddle) * scale.  What the weights lost when they were rounded
+            // counts for the middle's part too, where it would weigh most, and is given back to it.
+            float base[2][2];  // [group][head]
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                flats[i][0] = __shfl_sync(0xffffffffu, flat[i], 8 * t), flats[i][1] = __shfl_sync(0xffffffffu, flat[i], 8 * t + 4);
-            const float unit = 1.f / value_scale;
-            float* mine = sums + warp * kPagedGroup * kHeadDim;
+            for (int i = 0; i < 2; ++i) {
+                const float2 f = over_tokens(flat[i]), r = over_tokens(lost_weight[i]);
+                base[i][0] = fmaf(r.x, kCodeMiddle, f.x) * unit, base[i][1] = fmaf(r.y, kCodeMiddle, f.y) * unit;
+            }
+            float* mine = sums + warp * kPagedGroup * kHeadDim + 2 * t * kHeadDim;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int d = (i >> 2) * 64 + 8 * g + (i & 3) * 2;
                 constexpr float low = 1 << 24, high = 1 << 20;  // of codes in the low and in the next nibbles
-                if (2 * t < p.group)
-                    *reinterpret_cast<float2*>(mine + 2 * t * kHeadDim + d) =
-                        make_float2(fmaf(acc[i][0] * low, unit, flats[i >> 2][0]) * w0, fmaf(acc[i][2] * high, unit, flats[i >> 2][0]) * w0);
-                if (2 * t + 1 < p.group)
-                    *reinterpret_cast<float2*>(mine + (2 * t + 1) * kHeadDim + d) =
-                        make_float2(fmaf(acc[i][1] * low, unit, flats[i >> 2][1]) * w1, fmaf(acc[i][3] * high, unit, flats[i >> 2][1]) * w1);
+                const int d = (i >> 2) * 64 + 8 * g + (i & 3) * 2;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (2 * t + h < p.group)
+                        *reinterpret_cast<float2*>(mine + h * kHeadDim + d) = make_float2(fmaf(acc[i][h] * low, unit, base[i >> 2][h]) * weight[h],
+                                                                                       fmaf(acc[i][2 + h] * high, unit, base[i >> 2][h]) * weight[h]);
             }
         }
-        if (warp == 0 && t == 0) s_top[g] = top;
+        if (warp == 0 && g == 0) s_top[2 * t] = top[0], s_top[2 * t + 1] = top[1];
         ctas_sync();
         const bool whole = at.first == 0 && at.last == pages_of(at.length);
         float* part = p.parts + (2 * static_cast<int64_t>(blockIdx.x) + (first_segment ? 0 : 1)) * kPartialFloats;
@@ -389,6 +518,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
             }
         }
         // the next segment's sums and s_top are written behind its first barrier
+        first_segment = false;
     }
     if (lost) {  // no copy may land after the block's end
         for (int s = 0; s < kPaStages; ++s) mbar_wait(&bar_full[warp][s], s < stage ? phase ^ 1 : phase);
@@ -396,31 +526,38 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
     }
 }
 
-// Adds the parts of a unit that lies in several CTAs; a unit without tokens gets zeros.  Warp = query head.
+// Adds the parts of a unit that lies in several CTAs; a unit without tokens gets zeros.  Bound by latency: `split` warps per query
+// head take the parts in turn, and meet in shared memory.
 template <bool BF16>
-__global__ void __launch_bounds__(kPagedGroup * 32) paged_merge_kernel(const PagedParams p) {
-    const int lane = threadIdx.x & 31, head = threadIdx.x >> 5, unit = blockIdx.x;
+__global__ void __launch_bounds__(1024) paged_merge_kernel(const PagedParams p, int split) {
+    __shared__ float4 s_out[32][32];
+    __shared__ float s_total[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = warp / split, turn = warp - head * split, unit = blockIdx.x;
     wait_for_previous_launch();
     let_next_launch_start();
     const int sequence = unit / p.heads, kv_head = unit - sequence * p.heads;
     const int length = length_of(p, sequence);
     const int64_t row = static_cast<int64_t>(sequence) * p.heads * p.group + kv_head * p.group + head;
     if (length == 0) {
-        *reinterpret_cast<uint2*>(p.out + row * kHeadDim + 4 * lane) = make_uint2(0, 0);
-        if (p.lse && lane == 0) p.lse[row] = -INFINITY;
+        if (turn == 0) *reinterpret_cast<uint2*>(p.out + row * kHeadDim + 4 * lane) = make_uint2(0, 0);
+        if (p.lse && threadIdx.x % (32 * split) == 0) p.lse[row] = -INFINITY;
         return;
     }
-    const Shares shares = shares_of(p, lane);
-    int64_t before = 0;
-    for (int s = lane; s < sequence; s += 32) before += pages_of(length_of(p, s));
+    int64_t all = 0, before = 0;
+    for (int s = lane; s < p.sequences; s += 32) {
+        const int n = stretch_of(length_of(p, s));
+        all += n, before += s < sequence ? n : 0;
+    }
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) before += __shfl_xor_sync(0xffffffffu, before, off);
-    const int per = pages_of(length);
+    for (int off = 16; off > 0; off >>= 1)
+        all += __shfl_xor_sync(0xffffffffu, all, off), before += __shfl_xor_sync(0xffffffffu, before, off);
+    const Shares shares = shares_of(p, all);
+    const int per = stretch_of(length);
     const int64_t a = before * p.heads + static_cast<int64_t>(kv_head) * per;
-    const int from = shares.owner(a), to = shares.owner(a + per - 1);
+    const int from = shares.owner(a + kPaCharge), to = shares.owner(a + per - 1);
     if (from == to) return;
     const int count = to - from + 1;
-    const int skip = shares.begin(from) == a ? 0 : 1;  // the unit begins behind another one in its first CTA: that CTA's second part
+    const int skip = shares.begin(from) < a ? 1 : 0;  // the last page of another unit lies in front of it in its first CTA: that CTA's second part
     const float* parts = p.parts + 2 * static_cast<int64_t>(from) * kPartialFloats;
     const auto part = [&](int i) { return parts + (2 * i + (i == 0 ? skip : 0)) * kPartialFloats; };
     float top = -INFINITY;
@@ -429,14 +566,24 @@ __global__ void __launch_bounds__(kPagedGroup * 32) paged_merge_kernel(const Pag
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     float total = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < count; ++i) {
+#pragma unroll 4
+    for (int i = turn; i < count; i += split) {
         const float* from_part = part(i);
         const float m = from_part[kPagedGroup * kHeadDim + head], l = from_part[kPagedGroup * (kHeadDim + 1) + head];
         const float4 x = *reinterpret_cast<const float4*>(from_part + head * kHeadDim + 4 * lane);
         const float weight = m == top ? 1.f : fast_exp2(m - top);
         sum.x = fmaf(x.x, weight, sum.x), sum.y = fmaf(x.y, weight, sum.y), sum.z = fmaf(x.z, weight, sum.z), sum.w = fmaf(x.w, weight, sum.w);
         total = fmaf(l, weight, total);
+    }
+    if (split > 1) {
+        s_out[warp][lane] = sum;
+        if (lane == 0) s_total[warp] = total;
+        __syncthreads();
+        if (turn > 0) return;
+        for (int w = 1; w < split; ++w) {
+            const float4 x = s_out[warp + w][lane];
+            sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w, total += s_total[warp + w];
+        }
     }
     const float inv = 1.f / total;
     *reinterpret_cast<uint2*>(p.out + row * kHeadDim + 4 * lane) =
@@ -446,7 +593,7 @@ __global__ void __launch_bounds__(kPagedGroup * 32) paged_merge_kernel(const Pag
 
 // CTAs of the first kernel for as many pages as there may be.
 int paged_ctas(int sequences, int width, int heads) {
-    const int64_t most = (static_cast<int64_t>(sequences) * width * heads + kPaLeast - 1) / kPaLeast, room = kPaPerSm * sm_count();
+    const int64_t most = (static_cast<int64_t>(sequences) * (width + kPaCharge) * heads + kPaLeast - 1) / kPaLeast, room = kPaPerSm * sm_count();
     return static_cast<int>(most < room ? most : room);
 }
 
@@ -458,7 +605,8 @@ int launch(const PagedParams& p, cudaStream_t stream) {
         if (int rc = check_cuda(launch_overlapped(paged_attention_kernel<BF16>, dim3(static_cast<unsigned>(p.ctas)), kPaThreads, kPaSmem, stream, true, p),
                                 "paged_attention launch"))
             return rc;
-    return check_cuda(launch_overlapped(paged_merge_kernel<BF16>, dim3(static_cast<unsigned>(p.sequences * p.heads)), p.group * 32, 0, stream, true, p),
+    const int units = p.sequences * p.heads, split = units <= sm_count() && 32 / p.group > 1 ? std::min(8, 32 / p.group) : 1;
+    return check_cuda(launch_overlapped(paged_merge_kernel<BF16>, dim3(static_cast<unsigned>(units)), p.group * split * 32, 0, stream, true, p, split),
                       "paged_attention merge launch");
 }
 
