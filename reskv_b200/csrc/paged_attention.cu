@@ -4,7 +4,7 @@
 // The codes go to the tensor cores as they are: four bits in a 16-bit lane are a subnormal FP16 number, code * 2^-24 in the low
 // nibble, code * 2^-20 in the next one, exactly; scales and offsets enter outside of the product,
 //     q . k_j   = sum_groups scale_j,g * (q_g . code_j,g) + offset_j,g * sum(q_g)
-//     sum p v   = sum_j (p_j scale_j,g) code_j,g + sum_j p_j offset_j,g
+//     sum p v   = sum_j (p_j scale_j,g) (code_j,g - 8) + sum_j p_j (offset_j,g + 8 scale_j,g)
 // with p * scale rounded to FP16 once as the product's operand.  Bound by the cache's bytes as long as a token costs less than
 // its 144 bytes take to arrive.
 //
@@ -29,7 +29,8 @@ constexpr int kPaCharge = 3;                      // a segment costs as much as 
 constexpr int kPaLeast = 2 * kPaCharge;           // a share is at least that long
 constexpr int kPaSumBytes = kPaWarps * kPagedGroup * kHeadDim * 4;
 constexpr int kPaSmem = kPaWarps * kPaStages * kChunkBytes + kPaSumBytes;
-constexpr float kCodeMiddle = 7.5f;
+constexpr float kCodeMiddle = 8.f;
+constexpr uint32_t kMinusMiddleLow = 0x80088008u, kMinusMiddleHigh = 0x80808080u;  // pairs of -8 * 2^-24 and -8 * 2^-20
 constexpr int kPaSlack = 5;
 constexpr int kPartialFloats = kPagedGroup * (kHeadDim + 2);  // of a part: outputs [8][128], maxima [8], sums [8]
 
@@ -164,15 +165,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
-}
-
-// Two FP32 numbers per instruction.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
 }
 
 struct Requests {
@@ -313,13 +305,13 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
             q_scale[0] = __shfl_sync(0xffffffffu, mine, 8 * t), q_scale[1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
         }
 
-        // Of heads 2t and 2t + 1, over the lane's tokens: sums of p, per group of p * offset, and of what p * scale lost when it
-        // was rounded.  They and the outputs are in units of 2^-unit_up, which keeps p * scale where FP16 is exact to half a step.
+        // Of heads 2t and 2t + 1, over the lane's tokens: sums of p and per group of p * middle.  They and the outputs are in units of
+        // 2^-unit_up, which keeps p * scale where FP16 is exact to half a step.
         // m may lag behind the maximum by kPaSlack powers of two: fewer rescalings.
         float m[2] = {-INFINITY, -INFINITY}, shift[2] = {INFINITY, INFINITY};  // shift: unit_up - m * q_scale
         float most_power = 0.f, unit_limit = -1.f;                             // the largest power of two that a p may get; scale
         int unit_up = 0;
-        float2 l = make_float2(0.f, 0.f), flat[2] = {l, l}, lost_weight[2] = {l, l};
+        float2 l = make_float2(0.f, 0.f), flat[2] = {l, l};
         float acc[8][4];  // rows = coordinates, columns = heads 2t, 2t + 1
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
@@ -396,7 +388,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
                     if (most > unit_limit) {  // the same in every lane
                         const int e = clamped(exponent_of(most), -60, 100);
                         const int now = 14 - kPaSlack - e;  // a scale up to 2^(e + 1) times a p up to 2^kPaSlack, 2^15 at most
-                        if (unit_limit >= 0.f) change = power_of_two(clamped(now - unit_up, -126, 126));  // else: nothing summed up yet
+                        change = power_of_two(clamped(now - unit_up, -126, 126));
                         unit_up = now, most_power = static_cast<float>(now + kPaSlack), unit_limit = power_of_two(e + 1);
                     }
                     float factor[2];
@@ -412,7 +404,6 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         flat[i].x *= factor[0], flat[i].y *= factor[1];
-                        lost_weight[i].x *= factor[0], lost_weight[i].y *= factor[1];
                     }
 #pragma unroll
                     for (int i = 0; i < 8; ++i) acc[i][0] *= factor[0], acc[i][1] *= factor[1], acc[i][2] *= factor[0], acc[i][3] *= factor[1];
@@ -425,14 +416,15 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
                     l = add2(l, weight);
 #pragma unroll
                     for (int group = 0; group < 2; ++group) {
-                        const float2 w = make_float2(weight.x * scale[i][group], weight.y * scale[i][group]);
-                        const uint32_t pair = pack2<false>(w.x, w.y);
-                        weights[group][i] = transposed(pair);
-                        lost_weight[group] = add2(lost_weight[group], make_float2(w.x - low_of<false>(pair), w.y - high_of<false>(pair)));
-                        flat[group].x = fmaf(weight.x, offset[i][group], flat[group].x), flat[group].y = fmaf(weight.y, offset[i][group], flat[group].y);
+                        weights[group][i] = transposed(pack2<false>(weight.x * scale[i][group], weight.y * scale[i][group]));
+                        const float middle = fmaf(scale[i][group], kCodeMiddle, offset[i][group]);
+                        flat[group].x = fmaf(weight.x, middle, flat[group].x), flat[group].y = fmaf(weight.y, middle, flat[group].y);
                     }
                 }
-                // ---- outputs --------------------------------------------------------------------------------------------------------
+                // ---- outputs: a value is offset + 8 scale (its middle) + (code - 8) scale.  With the codes alone the sum would be many times
+                // the result, most of it taken back by the offsets, and its rounding with it.
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mma_16816(acc[i], kMinusMiddleLow, kMinusMiddleHigh, kMinusMiddleLow, kMinusMiddleHigh, weights[i >> 2][0], weights[i >> 2][1]);
                 uint2 rows[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -473,13 +465,11 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
             const float unit = power_of_two(-unit_up);
             const float weight[2] = {m[0] == top[0] ? 1.f : fast_exp2(m[0] - top[0]), m[1] == top[1] ? 1.f : fast_exp2(m[1] - top[1])};
             if (g == 0) s_sum[warp][2 * t] = l.x * unit * weight[0], s_sum[warp][2 * t + 1] = l.y * unit * weight[1];
-            // A value is offset + kCodeMiddle * scale + (code - kCodeMiddle) * scale.  What the weights lost when they were rounded
-            // counts for the middle's part too, where it would weigh most, and is given back to it.
             float base[2][2];  // [group][head]
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float2 f = over_tokens(flat[i]), r = over_tokens(lost_weight[i]);
-                base[i][0] = fmaf(r.x, kCodeMiddle, f.x) * unit, base[i][1] = fmaf(r.y, kCodeMiddle, f.y) * unit;
+                const float2 f = over_tokens(flat[i]);
+                base[i][0] = f.x * unit, base[i][1] = f.y * unit;
             }
             float* mine = sums + warp * kPagedGroup * kHeadDim + 2 * t * kHeadDim;
 #pragma unroll

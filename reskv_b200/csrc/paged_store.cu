@@ -2,9 +2,10 @@
 //
 // Storing: of a token's vector of one head, every group of 64 coordinates becomes offset = min, scale = (max - min) / 15
 // rounded to the model's type, code = round((x - offset) / scale) to the nearest, ties to even, at most 15 (0 where the scale
-// is 0).  512 bytes of K and V become 144.  Bound by bytes: half a warp holds a row (16 bytes a lane), the other half the same
-// row of the other side; extremes meet in three shuffles, every lane writes the word of its eight coordinates.  Several rows
-// are requested before the first is used.
+// is 0).  512 bytes of K and V become 144.  Bound by bytes, and close to that by instructions.  Eight lanes hold a row of one side,
+// eight coordinates of either group each, four rows (K and V of two heads) to a warp; extremes of both groups travel together as
+// 16-bit pairs; a code is the low bits of (x - offset) * (1 / scale) + 1.5 * 2^23, and only where that lies within 1e-5 of a half
+// the division itself decides.  A block first looks up where its tokens go, while their rows are on the way.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -14,8 +15,8 @@
 namespace reskv {
 namespace {
 
-constexpr int kRowsAtOnce = 4;       // (token, head) rows of a warp that are in flight together
-constexpr int kStoreThreads = 256;
+constexpr int kStoreWarps = 8, kStoreThreads = kStoreWarps * 32;
+constexpr int kPairsAtOnce = 4;  // pairs of (token, head) rows of a warp, where there are enough of them
 
 struct StoreParams {
     PagedPlace at;
@@ -27,135 +28,184 @@ struct StoreParams {
     uint32_t* status;
 };
 
-// Sequence of token i and its number in it; false: in none.  Whole warp.
-__device__ __forceinline__ bool place_of(const PagedPlace& at, int token, int lane, int& sequence, int& number) {
-    int before = 0;  // ends that lie at the token or in front of it
-    for (int s = lane; s < at.sequences; s += 32) before += at.cu[s + 1] <= token;
-    sequence = __reduce_add_sync(0xffffffffu, before);
-    if (sequence >= at.sequences) return false;
-    number = at.starts[sequence] + token - at.cu[sequence];
-    return token >= at.cu[sequence];
-}
-
-// Block of the pool that holds token `number` of a sequence for one head, and its row there; null (and a status bit): outside
-// the table or the pool.
-__device__ __forceinline__ unsigned char* block_of(const StoreParams& p, int sequence, int number, int head, int lane) {
-    const int slot = number / kPageTokens;
-    const bool inside = number >= 0 && slot < p.at.width;
-    const int page = inside ? p.at.table[static_cast<int64_t>(sequence) * p.at.width + slot] : -1;
-    if (page < 0 || page >= p.at.pages) {
-        if (lane == 0) atomicOr(p.status, RESKV_STATUS_STATE_RANGE);
-        return nullptr;
+// Where token i goes: byte of its block in the pool for head 0 (below 0: nowhere), and row of the block.
+struct TokenPlace {
+    int64_t block;
+    int row;
+};
+__device__ __forceinline__ TokenPlace place_of(const StoreParams& p, int token) {
+    int low = 0, high = p.at.sequences;  // the number of sequences that end at the token or in front of it
+    while (low < high) {
+        const int mid = (low + high) >> 1;
+        if (p.at.cu[mid + 1] <= token) low = mid + 1; else high = mid;
     }
-    return p.pages + (static_cast<int64_t>(page) * p.heads + head) * kPageHeadBytes + (number / kBlockTokens & 3) * kBlockBytes;
+    if (low >= p.at.sequences || token < p.at.cu[low]) return {-1, 0};
+    const int number = p.at.starts[low] + token - p.at.cu[low], slot = number / kPageTokens;
+    const int page = number >= 0 && slot < p.at.width ? p.at.table[static_cast<int64_t>(low) * p.at.width + slot] : -1;
+    if (page < 0 || page >= p.at.pages) {  // outside the table or the pool
+        atomicOr(p.status, RESKV_STATUS_STATE_RANGE);
+        return {-1, 0};
+    }
+    return {static_cast<int64_t>(page) * p.heads * kPageHeadBytes + (number / kBlockTokens & 3) * kBlockBytes, number & (kBlockTokens - 1)};
 }
 
-__device__ __forceinline__ float min_nan(float a, float b) {
-    float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+// The larger / smaller numbers of two pairs, NaN if one of the two is.
+template <bool BF16>
+__device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if (BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+template <bool BF16>
+__device__ __forceinline__ uint32_t min_pair(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if (BF16) asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 
-template <bool BF16, bool WRITE>
+// Codes of eight numbers; `scale` as stored, `low` the offset.
+template <bool BF16>
+__device__ __forceinline__ uint32_t codes_of(const uint4& x, float low, float scale) {
+    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: a sum with it is rounded to a whole number
+    constexpr float kNormal = BF16 ? 0x1p-126f : 0x1p-14f;
+    const uint32_t pairs[4] = {x.x, x.y, x.z, x.w};
+    float inverse, far = 0.f;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(scale));
+    const float2 minus_low = make_float2(-low, -low), inverses = make_float2(inverse, inverse), up = make_float2(kRound, kRound),
+                 down = make_float2(-kRound, -kRound);
+    float2 above[4];
+    uint32_t word = 0;
+#pragma unroll
+    for (int e = 3; e >= 0; --e) {
+        above[e] = add2(make_float2(low_of<BF16>(pairs[e]), high_of<BF16>(pairs[e])), minus_low);
+        const float2 quotient = mul2(above[e], inverses), rounded = add2(quotient, up), whole = add2(rounded, down);
+        far = max_nan(far, max_nan(fabsf(quotient.x - whole.x), fabsf(quotient.y - whole.y)));
+        word = (word * 16u + __float_as_uint(rounded.y)) * 16u + __float_as_uint(rounded.x);  // the constant part goes below
+    }
+    word -= 0x4B400000u * 0x11111111u;
+    // By the reciprocal a quotient is off by less than 1e-5.  A quotient that near to a half, a scale that rounding has made much
+    // smaller than it should be (below the normal numbers, 0) and what is not finite: by the division.
+    if (far <= 0.49999f && scale >= kNormal) return word;
+    word = 0;
+#pragma unroll
+    for (int e = 7; e >= 0; --e) {
+        const float code = fminf(fmaxf(rintf((e & 1 ? above[e >> 1].y : above[e >> 1].x) / scale), 0.f), 15.f);  // a NaN becomes 0:
+        word = word * 16u + (scale > 0.f ? static_cast<uint32_t>(code) : 0u);                                   // the scale says it
+    }
+    return word;
+}
+
+// x / 15 as IEEE division rounds it (x finite): the quotient by the reciprocal, corrected by its remainder.
+__device__ __forceinline__ float fifteenth(float x) {
+    constexpr float kInverse = 1.f / 15.f;
+    const float q = x * kInverse;
+    return fmaf(fmaf(-15.f, q, x), kInverse, q);
+}
+
+template <bool BF16, bool WRITE, int PAIRS>
 __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const StoreParams p) {
+    constexpr int kRows = kStoreWarps * 2 * PAIRS;  // of a block
+    __shared__ TokenPlace places[kRows];
     wait_for_previous_launch();
     let_next_launch_start();
-    const int lane = threadIdx.x & 31, side = lane >> 4, c = lane & 15;
-    const int64_t rows = static_cast<int64_t>(p.total) * p.heads;
-    const int64_t first = (static_cast<int64_t>(blockIdx.x) * (kStoreThreads / 32) + (threadIdx.x >> 5)) * kRowsAtOnce;
-    if (first >= rows) return;
-    int token = static_cast<int>(first / p.heads), head = static_cast<int>(first - static_cast<int64_t>(token) * p.heads);
-    unsigned char* row_at[kRowsAtOnce];
-    int block_row[kRowsAtOnce];
-    uint4 x[kRowsAtOnce];
-    int tokens[kRowsAtOnce], heads[kRowsAtOnce];
-    if (WRITE) {
-        int t = token, h = head;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side = lane >> 3 & 1, c = lane & 7;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows;
+    const int token0 = static_cast<int>(first / p.heads), head0 = static_cast<int>(first - static_cast<int64_t>(token0) * p.heads);
+    // a warp's pairs of rows lie next to each other
+    int token[PAIRS], head[PAIRS];
+    uint4 x[PAIRS][2];
+    {
+        const int row = warp * PAIRS * 2 + (lane >> 4);
+        int t = token0 + (head0 + row) / p.heads, h = (head0 + row) % p.heads;
 #pragma unroll
-        for (int r = 0; r < kRowsAtOnce; ++r) {
-            if (first + r < rows)
-                x[r] = *reinterpret_cast<const uint4*>(side ? p.v + t * p.v_token + h * p.v_head + 8 * c : p.k + t * p.k_token + h * p.k_head + 8 * c);
-            if (++h == p.heads) h = 0, ++t;
+        for (int i = 0; i < PAIRS; ++i) {
+            token[i] = t < p.total ? t : -1, head[i] = h;
+            if (WRITE && token[i] >= 0) {
+                const uint4* from = reinterpret_cast<const uint4*>(side ? p.v + t * p.v_token + h * p.v_head : p.k + t * p.k_token + h * p.k_head);
+                x[i][0] = from[c], x[i][1] = from[8 + c];
+            }
+            for (h += 2; h >= p.heads; h -= p.heads) ++t;
         }
     }
-    int known = -1, sequence = 0, number = 0;
-    bool placed = false;
+    for (int i = threadIdx.x; i < kRows && token0 + i < p.total && i <= (head0 + kRows - 1) / p.heads; i += kStoreThreads)
+        places[i] = place_of(p, token0 + i);
+    __syncthreads();
+    unsigned char* block[PAIRS];  // of the row's side, or null
+    int row[PAIRS];
 #pragma unroll
-    for (int r = 0; r < kRowsAtOnce; ++r) {
-        row_at[r] = nullptr;
-        tokens[r] = token, heads[r] = head;
-        if (first + r < rows) {
-            if (token != known) placed = place_of(p.at, token, lane, sequence, number), known = token;
-            if (placed) row_at[r] = block_of(p, sequence, number, head, lane);
-            block_row[r] = number & (kBlockTokens - 1);
-        }
-        if (++head == p.heads) head = 0, ++token;
+    for (int i = 0; i < PAIRS; ++i) {
+        block[i] = nullptr, row[i] = 0;
+        if (token[i] < 0) continue;
+        const TokenPlace to = places[token[i] - token0];
+        if (to.block >= 0) block[i] = p.pages + to.block + static_cast<int64_t>(head[i]) * kPageHeadBytes + side * kBlockSide;
+        row[i] = to.row;
     }
     if (WRITE) {
 #pragma unroll
-        for (int r = 0; r < kRowsAtOnce; ++r) {
-            if (!row_at[r]) continue;
-            const uint32_t* pairs = reinterpret_cast<const uint32_t*>(&x[r]);
-            float v[8];
+        for (int i = 0; i < PAIRS; ++i) {
+            // (group 0, group 1) extremes; rows without a place take part in the exchange with whatever they hold
+            if (token[i] < 0) x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);
+            uint32_t top[2], bottom[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[2 * e] = low_of<BF16>(pairs[e]), v[2 * e + 1] = high_of<BF16>(pairs[e]);
-            float low = v[0], high = v[0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) low = min_nan(low, v[e]), high = max_nan(high, v[e]);
+            for (int group = 0; group < 2; ++group) {
+                const uint4& v = x[i][group];
+                top[group] = max_pair<BF16>(max_pair<BF16>(v.x, v.y), max_pair<BF16>(v.z, v.w));
+                bottom[group] = min_pair<BF16>(min_pair<BF16>(v.x, v.y), min_pair<BF16>(v.z, v.w));
+            }
+            uint32_t high = max_pair<BF16>(__byte_perm(top[0], top[1], 0x5410), __byte_perm(top[0], top[1], 0x7632));
+            uint32_t low = min_pair<BF16>(__byte_perm(bottom[0], bottom[1], 0x5410), __byte_perm(bottom[0], bottom[1], 0x7632));
 #pragma unroll
             for (int off = 1; off < 8; off <<= 1) {
-                low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, off));
-                high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, off));
+                high = max_pair<BF16>(high, __shfl_xor_sync(0xffffffffu, high, off));
+                low = min_pair<BF16>(low, __shfl_xor_sync(0xffffffffu, low, off));
             }
-            const unsigned short scale_bits = narrow<BF16>((high - low) / 15.f);
-            const float scale = widen<BF16>(scale_bits);
-            uint32_t word = 0;
-            const float inverse = __frcp_rn(scale);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                // by the reciprocal (off by less than 1e-5), unless that lies so near to a half that the quotient has to decide;
-                // a NaN (of an infinite or NaN group) becomes 0 here: the group's values are NaN by its scale
-                const float above = v[e] - low, quotient = above * inverse;
-                float code = rintf(quotient);
-                if (!(fabsf(quotient - code) <= 0.4999f)) code = rintf(above / scale);
-                code = fminf(fmaxf(code, 0.f), 15.f);
-                word |= (scale > 0.f ? static_cast<uint32_t>(code) : 0u) << (4 * e);
+            if (!block[i]) continue;
+            const float low0 = low_of<BF16>(low), low1 = high_of<BF16>(low);
+            const uint32_t scales = pack2<BF16>(fifteenth(low_of<BF16>(high) - low0), fifteenth(high_of<BF16>(high) - low1));
+            const uint32_t w0 = codes_of<BF16>(x[i][0], low0, low_of<BF16>(scales)), w1 = codes_of<BF16>(x[i][1], low1, high_of<BF16>(scales));
+            if (side) {
+                *reinterpret_cast<uint2*>(block[i] + value_word(row[i], c)) = make_uint2(w0, w1);
+            } else {
+                *reinterpret_cast<uint32_t*>(block[i] + key_word(row[i], c)) = w0;
+                *reinterpret_cast<uint32_t*>(block[i] + key_word(row[i], c + 8)) = w1;
             }
-            unsigned char* codes = row_at[r] + side * kBlockSide;
-            *reinterpret_cast<uint32_t*>(codes + (side ? value_word(block_row[r], c) : key_word(block_row[r], c))) = word;
-            if ((c & 7) == 0) {
-                unsigned short* params = reinterpret_cast<unsigned short*>(codes + kBlockCodes + block_row[r] * 8);
-                params[c >> 3] = scale_bits;
-                params[2 + (c >> 3)] = narrow<BF16>(low);
-            }
+            if (c == 0) *reinterpret_cast<uint2*>(block[i] + kBlockCodes + row[i] * 8) = make_uint2(scales, low);
         }
     } else {
-        uint32_t word[kRowsAtOnce];
-        uint2 params[kRowsAtOnce];
+        uint2 words[PAIRS], params[PAIRS];
 #pragma unroll
-        for (int r = 0; r < kRowsAtOnce; ++r) {
-            if (!row_at[r]) continue;
-            const unsigned char* codes = row_at[r] + side * kBlockSide;
-            word[r] = *reinterpret_cast<const uint32_t*>(codes + (side ? value_word(block_row[r], c) : key_word(block_row[r], c)));
-            params[r] = *reinterpret_cast<const uint2*>(codes + kBlockCodes + block_row[r] * 8);
+        for (int i = 0; i < PAIRS; ++i) {
+            if (!block[i]) continue;
+            if (side)
+                words[i] = *reinterpret_cast<const uint2*>(block[i] + value_word(row[i], c));
+            else
+                words[i] = make_uint2(*reinterpret_cast<const uint32_t*>(block[i] + key_word(row[i], c)),
+                                      *reinterpret_cast<const uint32_t*>(block[i] + key_word(row[i], c + 8)));
+            params[i] = *reinterpret_cast<const uint2*>(block[i] + kBlockCodes + row[i] * 8);
         }
 #pragma unroll
-        for (int r = 0; r < kRowsAtOnce; ++r) {
-            if (!row_at[r]) continue;
-            const float scale = c < 8 ? low_of<BF16>(params[r].x) : high_of<BF16>(params[r].x);
-            const float low = c < 8 ? low_of<BF16>(params[r].y) : high_of<BF16>(params[r].y);
-            uint4 y;
-            uint32_t* pairs = reinterpret_cast<uint32_t*>(&y);
+        for (int i = 0; i < PAIRS; ++i) {
+            if (!block[i]) continue;
+            uint4* to = reinterpret_cast<uint4*>((side ? p.v_out : p.k_out) + (static_cast<int64_t>(token[i]) * p.heads + head[i]) * 128);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                pairs[e] = pack2<BF16>(fmaf(scale, static_cast<float>(word[r] >> (8 * e) & 15u), low),
-                                       fmaf(scale, static_cast<float>(word[r] >> (8 * e + 4) & 15u), low));
-            *reinterpret_cast<uint4*>((side ? p.v_out : p.k_out) + (static_cast<int64_t>(tokens[r]) * p.heads + heads[r]) * 128 + 8 * c) = y;
+            for (int group = 0; group < 2; ++group) {
+                const float scale = group ? high_of<BF16>(params[i].x) : low_of<BF16>(params[i].x);
+                const float low = group ? high_of<BF16>(params[i].y) : low_of<BF16>(params[i].y);
+                const uint32_t word = group ? words[i].y : words[i].x;
+                const float2 scales = make_float2(scale, scale), lows = make_float2(low, low), down = make_float2(-8388608.f, -8388608.f);
+                uint4 y;
+                uint32_t* pairs = reinterpret_cast<uint32_t*>(&y);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {  // codes as the low bits of 2^23 + code
+                    const float2 code = add2(make_float2(__uint_as_float((word >> (8 * e) & 15u) | 0x4B000000u),
+                                                         __uint_as_float((word >> (8 * e + 4) & 15u) | 0x4B000000u)), down);
+                    const float2 v = fma2(scales, code, lows);
+                    pairs[e] = pack2<BF16>(v.x, v.y);
+                }
+                to[8 * group + c] = y;
+            }
         }
     }
 }
@@ -199,14 +249,20 @@ int check_place(const char* who, const int32_t* cu, const int32_t* starts, const
     return width > 0 ? check_device_pointer(table, who, "table") : RESKV_OK;
 }
 
+template <bool BF16, bool WRITE, int PAIRS>
+int launch_store(const StoreParams& p, cudaStream_t stream) {
+    constexpr int per = kStoreWarps * 2 * PAIRS;
+    const int64_t blocks = (static_cast<int64_t>(p.total) * p.heads + per - 1) / per;
+    if (blocks > 0x7fffffff) return fail(RESKV_ERR_LIMIT, "paged cache: too many tokens for one call");
+    return check_cuda(launch_overlapped(paged_store_kernel<BF16, WRITE, PAIRS>, dim3(static_cast<unsigned>(blocks)), kStoreThreads, 0, stream, true, p),
+                      WRITE ? "paged_write launch" : "paged_read launch");
+}
+// One pair of rows per warp as long as that leaves SMs without a block.
 template <bool WRITE>
 int run_store(const StoreParams& p, int bf16, cudaStream_t stream) {
-    const int64_t rows = static_cast<int64_t>(p.total) * p.heads, per = kRowsAtOnce * (kStoreThreads / 32), blocks = (rows + per - 1) / per;
-    if (blocks > 0x7fffffff) return fail(RESKV_ERR_LIMIT, "paged cache: too many tokens for one call");
-    const dim3 grid(static_cast<unsigned>(blocks));
-    return check_cuda(bf16 ? launch_overlapped(paged_store_kernel<true, WRITE>, grid, kStoreThreads, 0, stream, true, p)
-                           : launch_overlapped(paged_store_kernel<false, WRITE>, grid, kStoreThreads, 0, stream, true, p),
-                      WRITE ? "paged_write launch" : "paged_read launch");
+    const bool many = static_cast<int64_t>(p.total) * p.heads > static_cast<int64_t>(sm_count()) * kStoreWarps * 2;
+    return bf16 ? many ? launch_store<true, WRITE, kPairsAtOnce>(p, stream) : launch_store<true, WRITE, 1>(p, stream)
+                : many ? launch_store<false, WRITE, kPairsAtOnce>(p, stream) : launch_store<false, WRITE, 1>(p, stream);
 }
 
 }  // namespace
