@@ -25,12 +25,12 @@ constexpr int kPaStages = 2;
 constexpr int kChunkBlocks = 2, kChunkTokens = kChunkBlocks * kBlockTokens, kChunkBytes = kChunkBlocks * kBlockBytes;  // a warp's turn
 constexpr int kPaPerSm = 2;                       // CTAs of an SM
 constexpr int kPageChunks = kPageTokens / kChunkTokens;
-constexpr int kPaCharge = 3;                      // a segment costs as much as that many pages besides its own
-constexpr int kPaLeast = 2 * kPaCharge;           // a share is at least that long
+constexpr int kPaCharge = 8;                      // a segment costs as much as that many pages besides its own
+constexpr int kPaLeast = 4;                       // a share is at least that long (a unit of one page: two CTAs' worth)
 constexpr int kPaSumBytes = kPaWarps * kPagedGroup * kHeadDim * 4;
 constexpr int kPaSmem = kPaWarps * kPaStages * kChunkBytes + kPaSumBytes;
 constexpr float kCodeMiddle = 8.f;
-constexpr uint32_t kMinusMiddleLow = 0x80088008u, kMinusMiddleHigh = 0x80808080u;  // pairs of -8 * 2^-24 and -8 * 2^-20
+constexpr uint32_t kMiddleLow = 0x80088008u, kMiddleHigh = 0x80808080u;  // pairs of -8 * 2^-24 and -8 * 2^-20
 constexpr int kPaSlack = 5;
 constexpr int kPartialFloats = kPagedGroup * (kHeadDim + 2);  // of a part: outputs [8][128], maxima [8], sums [8]
 
@@ -56,60 +56,74 @@ __device__ __forceinline__ int length_of(const PagedParams& p, int s) {
 __device__ __forceinline__ int pages_of(int length) { return (length + kPageTokens - 1) / kPageTokens; }
 
 // How the work is dealt out; the same for both kernels.  All units are laid end to end, each with its pages behind a charge of
-// kPaCharge (what a segment costs besides them: the query, the first block's latency, the meeting of the warps), and every CTA
-// takes an equal stretch.
-struct Shares {
-    int64_t all;
-    int ctas;
-    __device__ __forceinline__ int64_t begin(int cta) const { return cta * all / ctas; }
-    __device__ __forceinline__ int owner(int64_t place) const { return static_cast<int>(((place + 1) * ctas - 1) / all); }
-};
+// kPaCharge (what a segment costs besides them: the query, the first chunk's latency, the meeting of the warps), and every CTA
+// takes an equal stretch (the first `extra` one more).  The host refuses what does not fit 31 bits.
 __device__ __forceinline__ int stretch_of(int length) { return length > 0 ? pages_of(length) + kPaCharge : 0; }
-__device__ __forceinline__ Shares shares_of(const PagedParams& p, int64_t of_one_head) {
-    const int64_t all = of_one_head * p.heads, most = (all + kPaLeast - 1) / kPaLeast;
-    return {all, static_cast<int>(most < p.ctas ? most : p.ctas)};
-}
-__device__ __forceinline__ Shares count_shares(const PagedParams& p, int lane) {
-    int64_t n = 0;
-    for (int s = lane; s < p.sequences; s += 32) n += stretch_of(length_of(p, s));
+struct Shares {
+    int ctas, each, extra;
+    __device__ __forceinline__ Shares(const PagedParams& p, int all) {
+        ctas = min(p.ctas, (all + kPaLeast - 1) / kPaLeast);
+        each = ctas ? all / ctas : 0, extra = all - each * ctas;
+    }
+    __device__ __forceinline__ int begin(int cta) const { return cta * each + min(cta, extra); }
+    __device__ __forceinline__ int owner(int place) const {
+        const int longer = extra * (each + 1);
+        return place < longer ? place / (each + 1) : extra + (place - longer) / each;
+    }
+};
+
+// The stretches of the sequences, one after the other, of one head.
+struct Lengths {
+    int mine, upto, all;  // of the lane's sequence among the first 32: its length, the stretches up to its end; all stretches
+    __device__ __forceinline__ Lengths(const PagedParams& p, int lane) {
+        mine = lane < p.sequences ? length_of(p, lane) : 0;
+        upto = running_sum(stretch_of(mine), lane);
+        all = __shfl_sync(0xffffffffu, upto, 31);
+        if (p.sequences > 32) {
+            int rest = 0;
+            for (int s = 32 + lane; s < p.sequences; s += 32) rest += stretch_of(length_of(p, s));
+            all += __reduce_add_sync(0xffffffffu, rest);
+        }
+    }
+    static __device__ __forceinline__ int running_sum(int x, int lane) {
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
-    return shares_of(p, n);
-}
+        for (int off = 1; off < 32; off <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, x, off);
+            if (lane >= off) x += other;
+        }
+        return x;
+    }
+};
 
 // The segments of a share, one after the other: consecutive pages of a unit.
 struct Segments {
     int sequence, head, length, first, last;
-    int64_t left;  // of the share behind this segment
+    int left;  // of the share behind this segment
     // From place `place` on, `count` long; whole warp.  The first segment may be empty (first == last).
-    __device__ __forceinline__ void start(const PagedParams& p, int64_t place, int64_t count, int lane) {
-        int64_t before = 0;
+    __device__ __forceinline__ void start(const PagedParams& p, const Lengths& known, int place, int count, int lane) {
+        int before = 0, n = known.mine, upto = known.upto;
         left = -1;
         for (int s0 = 0; s0 < p.sequences; s0 += 32) {
-            const int n = s0 + lane < p.sequences ? length_of(p, s0 + lane) : 0;
-            const int64_t mine = static_cast<int64_t>(stretch_of(n)) * p.heads;
-            int64_t upto = mine;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const int64_t other = __shfl_up_sync(0xffffffffu, upto, off);
-                if (lane >= off) upto += other;
+            if (s0 > 0) {
+                n = s0 + lane < p.sequences ? length_of(p, s0 + lane) : 0;
+                upto = Lengths::running_sum(stretch_of(n), lane);
             }
-            const uint32_t mask = __ballot_sync(0xffffffffu, before + upto > place);
+            const uint32_t mask = __ballot_sync(0xffffffffu, (before + upto) * p.heads > place);
             if (mask) {
                 const int owner = __ffs(mask) - 1;
                 length = __shfl_sync(0xffffffffu, n, owner);
-                const int64_t at = place - (before + __shfl_sync(0xffffffffu, upto - mine, owner));
                 const int per = stretch_of(length);
-                sequence = s0 + owner, head = static_cast<int>(at / per);
-                take(static_cast<int>(at - static_cast<int64_t>(head) * per), count);
+                const int at = place - (before + __shfl_sync(0xffffffffu, upto, owner) - per) * p.heads;
+                sequence = s0 + owner, head = at / per;
+                take(at - head * per, count);
                 return;
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
         }
     }
     // What `count` from offset `from` of the unit's stretch on holds of it.
-    __device__ __forceinline__ void take(int from, int64_t count) {
-        const int per = stretch_of(length), to = per - from < count ? per : from + static_cast<int>(count);
+    __device__ __forceinline__ void take(int from, int count) {
+        const int per = stretch_of(length), to = min(per, from + count);
         first = from > kPaCharge ? from - kPaCharge : 0, last = to > kPaCharge ? to - kPaCharge : 0;
         left = count - (to - from);
     }
@@ -160,6 +174,15 @@ __device__ __forceinline__ void mma_offsets(float (&c)[4], uint32_t a0, uint32_t
                      : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
 }
 
+// The larger numbers of two pairs (a NaN counts for nothing).
+template <bool BF16>
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if (BF16) asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
 // An 8 x 8 matrix of 16-bit numbers, two of a row per lane, with rows and columns exchanged.
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t y;
@@ -169,9 +192,11 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 
 struct Requests {
     Segments segment;           // behind the one that is being requested; left < 0: none
-    const int* entry;           // in the table, of the chunk after the next
+    const int* entry;           // in the table, of the chunk that is looked up next
     const unsigned char* base;  // of the head and the chunk's place in page 0
-    int chunks, page;           // left to request of the segment (-1: none at all), page of the next one
+    int chunks;                 // left to look up of the segment (-1: none at all)
+    int page[kPaStages];        // looked up: pages, and `base` (null: there is no further chunk)
+    const unsigned char* at[kPaStages];
 };
 
 // The warp's next segment, in shared memory; whole warp.
@@ -199,26 +224,27 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
     __syncwarp();
     wait_for_previous_launch();
     let_next_launch_start();
-    const Shares shares = count_shares(p, lane);
+    const Lengths lengths(p, lane);
+    const Shares shares(p, lengths.all * p.heads);
     if (static_cast<int>(blockIdx.x) >= shares.ctas) return;
-    const int64_t begin = shares.begin(blockIdx.x), count = shares.begin(blockIdx.x + 1) - begin;
+    const int begin = shares.begin(blockIdx.x), count = shares.begin(blockIdx.x + 1) - begin;
     // A warp's places in its list of segments, the one that is worked on and the one whose chunks are requested, are in shared
     // memory: registers are scarce.
     Segments& at = s_at[warp];
     Requests& ahead = s_ahead[warp];
     {
         Segments first{};
-        first.start(p, begin, count, lane);
+        first.start(p, lengths, begin, count, lane);
         if (lane == 0) at = first, ahead.segment = first, ahead.chunks = 0;
         __syncwarp();
     }
     // Requests run ahead of the work (lane 0).  A warp's chunks are kPaWarps apart, so they lie at the same place of their pages.
-    // The number of the next page is under way into shared memory while a chunk is worked on.
-    const auto look = [&] {
+    // The numbers of the next two pages are under way into shared memory while a chunk is worked on.
+    const auto look = [&](int slot) {
         while (ahead.chunks == 0) {
             if (ahead.segment.left < 0) {
                 ahead.chunks = -1;
-                return;
+                break;
             }
             const int first = ahead.segment.first_chunk() + warp, end = ahead.segment.last_chunk();
             if (end > first) {
@@ -228,25 +254,32 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
             }
             if (!ahead.segment.next(p)) ahead.segment.left = -1;
         }
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&ahead.page)), "l"(ahead.entry) : "memory");
-        ahead.entry += kPaWarps / kPageChunks;
+        ahead.at[slot] = nullptr;
+        if (ahead.chunks > 0) {
+            ahead.at[slot] = ahead.base;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&ahead.page[slot])), "l"(ahead.entry) : "memory");
+            ahead.entry += kPaWarps / kPageChunks;
+            --ahead.chunks;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    const auto request = [&](int stage) {
-        if (ahead.chunks < 0) return;
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        int page = *static_cast<volatile int*>(&ahead.page);
+    const auto request = [&](int stage) {  // page slots and stages go round together
+        const unsigned char* from = ahead.at[stage];
+        if (!from) return;
+        asm volatile("cp.async.wait_group %0;" ::"n"(kPaStages - 1) : "memory");
+        int page = *static_cast<volatile int*>(&ahead.page[stage]);
         if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.page_count)) {
             atomicOr(p.status, RESKV_STATUS_STATE_RANGE);
             page = 0;
         }
         mbar_arrive_expect_tx(&bar_full[warp][stage], kChunkBytes);
-        bulk_g2s(ring + stage * kChunkBytes, ahead.base + page * (static_cast<int64_t>(p.heads) * kPageHeadBytes), kChunkBytes, &bar_full[warp][stage]);
-        --ahead.chunks;
-        look();
+        bulk_g2s(ring + stage * kChunkBytes, from + page * (static_cast<int64_t>(p.heads) * kPageHeadBytes), kChunkBytes, &bar_full[warp][stage]);
+        look(stage);
     };
     bool lost = false;
     if (lane == 0) {
-        look();
+#pragma unroll 1
+        for (int s = 0; s < kPaStages; ++s) look(s);
 #pragma unroll 1
         for (int s = 0; s < kPaStages; ++s) request(s);
     }
@@ -308,9 +341,8 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
         // Of heads 2t and 2t + 1, over the lane's tokens: sums of p and per group of p * middle.  They and the outputs are in units of
         // 2^-unit_up, which keeps p * scale where FP16 is exact to half a step.
         // m may lag behind the maximum by kPaSlack powers of two: fewer rescalings.
-        float m[2] = {-INFINITY, -INFINITY}, shift[2] = {INFINITY, INFINITY};  // shift: unit_up - m * q_scale
-        float most_power = 0.f, unit_limit = -1.f;                             // the largest power of two that a p may get; scale
-        int unit_up = 0;
+        float shift[2] = {INFINITY, INFINITY};  // unit_up - m * q_scale
+        float unit_up = 0.f, unit_limit = -1.f;
         float2 l = make_float2(0.f, 0.f), flat[2] = {l, l};
         float acc[8][4];  // rows = coordinates, columns = heads 2t, 2t + 1
 #pragma unroll
@@ -319,112 +351,134 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
         int tokens = at.length - start * kChunkTokens;  // from this chunk on
         for (int chunks = end - start; chunks > 0; chunks -= kPaWarps, tokens -= kPaWarps * kChunkTokens) {
             if (!lost) lost = !mbar_wait(&bar_full[warp][stage], phase);
+            unsigned char* const chunk = ring + stage * kChunkBytes;
+            // ---- scores: rows = tokens g, g + 8 of a block, columns = heads: (scale . (q . code) 2^22 + offset . sum(q) / 4) * q_scale ----
+            float s[kChunkBlocks][4];
 #pragma unroll
             for (int b = 0; b < kChunkBlocks; ++b) {
-                unsigned char* keys = ring + stage * kChunkBytes + b * kBlockBytes + own_row * 64 + 16 * t;
-                unsigned char* values = ring + stage * kChunkBytes + b * kBlockBytes + kBlockSide;
-                unsigned char* own = values + kBlockCodes + own_row * 8;  // parameters of the lane's tokens: here and 64 bytes on
-                const int live = tokens - b * kBlockTokens;
-                if (live <= 0) break;
-                // ---- scores: rows = tokens g, g + 8, columns = heads: (scale . (q . code) 2^22 + offset . sum(q) / 4) * q_scale ----
-                float s[4];
-                {
-                    const uint4 w0 = *reinterpret_cast<const uint4*>(keys), w1 = *reinterpret_cast<const uint4*>(keys + 8 * 64);
-                    const uint32_t words[2][4] = {{w0.x, w0.y, w0.z, w0.w}, {w1.x, w1.y, w1.z, w1.w}};
-                    const uint2 param[2] = {*reinterpret_cast<const uint2*>(own - kBlockSide), *reinterpret_cast<const uint2*>(own - kBlockSide + 64)};
-                    float c[2][4], offsets[4];
-                    mma_offsets<BF16>(offsets, param[0].y, param[1].y, q_sums);
+                const unsigned char* keys = chunk + b * kBlockBytes + own_row * 64 + 16 * t;
+                const unsigned char* own = chunk + b * kBlockBytes + kBlockCodes + own_row * 8;
+                const uint4 w0 = *reinterpret_cast<const uint4*>(keys), w1 = *reinterpret_cast<const uint4*>(keys + 8 * 64);
+                const uint32_t words[2][4] = {{w0.x, w0.y, w0.z, w0.w}, {w1.x, w1.y, w1.z, w1.w}};
+                const uint2 param[2] = {*reinterpret_cast<const uint2*>(own), *reinterpret_cast<const uint2*>(own + 64)};
+                float c[2][4], offsets[4];
+                mma_offsets<BF16>(offsets, param[0].y, param[1].y, q_sums);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float(&d)[4] = c[j >> 1];
-                        const uint32_t x = words[0][j], y = words[1][j], x8 = x >> 8, y8 = y >> 8;
-                        if (j & 1)
-                            mma_16816(d, x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q_low[j][0], q_high[j][0]);
-                        else
-                            mma_16816_start(d, x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q_low[j][0], q_high[j][0]);
-                        mma_16816(d, x8 & 0x000F000Fu, y8 & 0x000F000Fu, x8 & 0x00F000F0u, y8 & 0x00F000F0u, q_low[j][1], q_high[j][1]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float scale0 = low_of<BF16>(param[i].x), scale1 = high_of<BF16>(param[i].x);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            s[2 * i + h] = fmaf(fmaf(c[0][2 * i + h], scale0, c[1][2 * i + h] * scale1), 1 << 22, offsets[2 * i + h]);
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    float(&d)[4] = c[j >> 1];
+                    const uint32_t x = words[0][j], y = words[1][j], x8 = x >> 8, y8 = y >> 8;
+                    if (j & 1)
+                        mma_16816(d, x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q_low[j][0], q_high[j][0]);
+                    else
+                        mma_16816_start(d, x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q_low[j][0], q_high[j][0]);
+                    mma_16816(d, x8 & 0x000F000Fu, y8 & 0x000F000Fu, x8 & 0x00F000F0u, y8 & 0x00F000F0u, q_low[j][1], q_high[j][1]);
                 }
-                if (live < kBlockTokens) {  // behind the sequence's end: whatever lies there counts for nothing
-                    __syncwarp();
-                    if (lane < kBlockTokens && lane >= live) {
-                        *reinterpret_cast<uint2*>(values + kBlockCodes + lane * 8) = make_uint2(0, 0);
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next copy to this place comes behind it
-                    }
-                    __syncwarp();
-                    if (own_row >= live) s[0] = s[1] = -INFINITY;
-                    if (own_row + 8 >= live) s[2] = s[3] = -INFINITY;
-                }
-                float scale[2][2], offset[2][2];  // [token][group]
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const uint2 param = *reinterpret_cast<const uint2*>(own + 64 * i);
-                    scale[i][0] = low_of<BF16>(param.x), scale[i][1] = high_of<BF16>(param.x);
-                    offset[i][0] = low_of<BF16>(param.y), offset[i][1] = high_of<BF16>(param.y);
+                    const float scale0 = low_of<BF16>(param[i].x), scale1 = high_of<BF16>(param[i].x);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        s[b][2 * i + h] = fmaf(fmaf(c[0][2 * i + h], scale0, c[1][2 * i + h] * scale1), 1 << 22, offsets[2 * i + h]);
                 }
-                // ---- running softmax; the unit follows the largest scale (BF16: or 2^-30 of an offset, so that a sum of offsets stays
-                // in range where all scales are 0) ------------------------------------------------------------------------------------
-                float most = fmaxf(fmaxf(scale[0][0], scale[0][1]), fmaxf(scale[1][0], scale[1][1]));
-                if (BF16) most = fmaxf(most, 0x1p-30f * fmaxf(fmaxf(fabsf(offset[0][0]), fabsf(offset[0][1])), fmaxf(fabsf(offset[1][0]), fabsf(offset[1][1]))));
-                float power[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) power[i] = fmaf(s[i], q_scale[i & 1], shift[i & 1]);
-                if (__any_sync(0xffffffffu, fmaxf(fmaxf(power[0], power[1]), fmaxf(power[2], power[3])) > most_power || most > unit_limit)) {
-                    float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
-#pragma unroll
-                    for (int off = 4; off < 32; off <<= 1) {
-                        top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
-                        top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
-                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-                    }
-                    float change = 1.f;
-                    if (most > unit_limit) {  // the same in every lane
-                        const int e = clamped(exponent_of(most), -60, 100);
-                        const int now = 14 - kPaSlack - e;  // a scale up to 2^(e + 1) times a p up to 2^kPaSlack, 2^15 at most
-                        change = power_of_two(clamped(now - unit_up, -126, 126));
-                        unit_up = now, most_power = static_cast<float>(now + kPaSlack), unit_limit = power_of_two(e + 1);
-                    }
-                    float factor[2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float next = fmaxf(m[h], top[h]);
-                        factor[h] = (m[h] == next ? 1.f : fast_exp2((m[h] - next) * q_scale[h])) * change;
-                        m[h] = next;
-                        shift[h] = static_cast<float>(unit_up) - next * q_scale[h];
-                        power[h] = fmaf(s[h], q_scale[h], shift[h]), power[2 + h] = fmaf(s[2 + h], q_scale[h], shift[h]);
-                    }
-                    l.x *= factor[0], l.y *= factor[1];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        flat[i].x *= factor[0], flat[i].y *= factor[1];
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[i][0] *= factor[0], acc[i][1] *= factor[1], acc[i][2] *= factor[0], acc[i][3] *= factor[1];
+            }
+            if (tokens < kChunkTokens) {  // behind the sequence's end: whatever lies there counts for nothing
+                __syncwarp();
+                if (lane >= tokens) {
+                    *reinterpret_cast<uint2*>(chunk + (lane >> 4) * kBlockBytes + kBlockSide + kBlockCodes + (lane & 15) * 8) = make_uint2(0, 0);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next copy to this place comes behind it
                 }
+                __syncwarp();
+#pragma unroll
+                for (int b = 0; b < kChunkBlocks; ++b) {
+                    if (16 * b + own_row >= tokens) s[b][0] = s[b][1] = -INFINITY;
+                    if (16 * b + own_row + 8 >= tokens) s[b][2] = s[b][3] = -INFINITY;
+                }
+            }
+            // ---- running softmax; the unit follows the largest scale (BF16: or 2^-30 of an offset, so that a sum of offsets stays in
+            // range where all scales are 0) ----------------------------------------------------------------------------------------
+            uint2 params[kChunkBlocks][2];  // of the lane's tokens: scales, offsets
+#pragma unroll
+            for (int b = 0; b < kChunkBlocks; ++b)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    params[b][i] = *reinterpret_cast<const uint2*>(chunk + b * kBlockBytes + kBlockSide + kBlockCodes + (own_row + 8 * i) * 8);
+            float most;
+            {
+                const uint32_t pair = larger<BF16>(larger<BF16>(params[0][0].x, params[0][1].x), larger<BF16>(params[1][0].x, params[1][1].x));
+                most = fmaxf(low_of<BF16>(pair), high_of<BF16>(pair));
+                if (BF16) {
+                    constexpr uint32_t kPlus = 0x7FFF7FFFu;
+                    const uint32_t off = larger<BF16>(larger<BF16>(params[0][0].y & kPlus, params[0][1].y & kPlus), larger<BF16>(params[1][0].y & kPlus, params[1][1].y & kPlus));
+                    most = fmaxf(most, 0x1p-30f * fmaxf(low_of<BF16>(off), high_of<BF16>(off)));
+                }
+            }
+            float power[kChunkBlocks][4], highest = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < kChunkBlocks; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) power[b][i] = fmaf(s[b][i], q_scale[i & 1], shift[i & 1]), highest = fmaxf(highest, power[b][i]);
+            if (__any_sync(0xffffffffu, highest > unit_up + kPaSlack || most > unit_limit)) {
+                float top[2] = {fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])), fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]))};
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) {
+                    top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
+                    top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
+                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+                }
+                float up = unit_up;
+                if (most > unit_limit) {  // the same in every lane
+                    const int e = clamped(exponent_of(most), -60, 100);
+                    up = 14 - kPaSlack - e;  // a scale up to 2^(e + 1) times a p up to 2^kPaSlack, 2^15 at most
+                    unit_limit = power_of_two(e + 1);
+                }
+                const float change = power_of_two(clamped(static_cast<int>(up - unit_up), -126, 126));
+                float factor[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float before = unit_up - shift[h], next = fmaxf(before, top[h] * q_scale[h]);
+                    factor[h] = (before == next ? 1.f : fast_exp2(before - next)) * change;
+                    shift[h] = up - next;
+                }
+                unit_up = up;
+#pragma unroll
+                for (int b = 0; b < kChunkBlocks; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) power[b][i] = fmaf(s[b][i], q_scale[i & 1], shift[i & 1]);
+                l.x *= factor[0], l.y *= factor[1];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) flat[i].x *= factor[0], flat[i].y *= factor[1];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i][0] *= factor[0], acc[i][1] *= factor[1], acc[i][2] *= factor[0], acc[i][3] *= factor[1];
+            }
+            float eights[2][4];
+#pragma unroll
+            for (int b = 0; b < kChunkBlocks; ++b) {
+                const unsigned char* values = chunk + b * kBlockBytes + kBlockSide;
                 // ---- weights: rows = tokens, turned round for the contraction over them --------------------------------------------
                 uint32_t weights[2][2];  // [group][half of the block's tokens]
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float2 weight = make_float2(fast_exp2(power[2 * i]), fast_exp2(power[2 * i + 1]));
+                    const float2 weight = make_float2(fast_exp2(power[b][2 * i]), fast_exp2(power[b][2 * i + 1]));
                     l = add2(l, weight);
 #pragma unroll
                     for (int group = 0; group < 2; ++group) {
-                        weights[group][i] = transposed(pack2<false>(weight.x * scale[i][group], weight.y * scale[i][group]));
-                        const float middle = fmaf(scale[i][group], kCodeMiddle, offset[i][group]);
+                        const float scale = group ? high_of<BF16>(params[b][i].x) : low_of<BF16>(params[b][i].x);
+                        const float offset = group ? high_of<BF16>(params[b][i].y) : low_of<BF16>(params[b][i].y);
+                        weights[group][i] = transposed(pack2<false>(weight.x * scale, weight.y * scale));
+                        const float middle = fmaf(scale, kCodeMiddle, offset);
                         flat[group].x = fmaf(weight.x, middle, flat[group].x), flat[group].y = fmaf(weight.y, middle, flat[group].y);
                     }
                 }
                 // ---- outputs: a value is offset + 8 scale (its middle) + (code - 8) scale.  With the codes alone the sum would be many times
-                // the result, most of it taken back by the offsets, and its rounding with it.
+                // the result, most of it taken back by the offsets, and its rounding with it: eight times the weights are taken off again
+                // after every chunk.
 #pragma unroll
-                for (int i = 0; i < 8; ++i) mma_16816(acc[i], kMinusMiddleLow, kMinusMiddleHigh, kMinusMiddleLow, kMinusMiddleHigh, weights[i >> 2][0], weights[i >> 2][1]);
+                for (int group = 0; group < 2; ++group) {
+                    if (b == 0)
+                        mma_16816_start(eights[group], kMiddleLow, kMiddleHigh, kMiddleLow, kMiddleHigh, weights[group][0], weights[group][1]);
+                    else
+                        mma_16816(eights[group], kMiddleLow, kMiddleHigh, kMiddleLow, kMiddleHigh, weights[group][0], weights[group][1]);
+                }
                 uint2 rows[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -432,7 +486,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
                     rows[i] = *reinterpret_cast<const uint2*>(values + row * 64 + 8 * (g ^ ((row >> 1 & 1) << 2)));
                 }
 #pragma unroll
-                for (int group = 0; group < 2; ++group) {
+                for (int group = 0; group < 2; ++group)
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {  // bytes 0, 1 and 2, 3 of the words
                         const uint32_t pick = half ? 0x7632u : 0x5410u;
@@ -441,7 +495,12 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
                         mma_16816(acc[group * 4 + half * 2], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, weights[group][0], weights[group][1]);
                         mma_16816(acc[group * 4 + half * 2 + 1], x8 & 0x000F000Fu, x8 & 0x00F000F0u, y8 & 0x000F000Fu, y8 & 0x00F000F0u, weights[group][0], weights[group][1]);
                     }
-                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float2 x = add2(make_float2(acc[i][0], acc[i][1]), make_float2(eights[i >> 2][0], eights[i >> 2][1]));
+                const float2 y = add2(make_float2(acc[i][2], acc[i][3]), make_float2(eights[i >> 2][2], eights[i >> 2][3]));
+                acc[i][0] = x.x, acc[i][1] = x.y, acc[i][2] = y.x, acc[i][3] = y.y;
             }
             __syncwarp();
             if (lane == 0) request(stage);
@@ -455,14 +514,14 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
             return x;
         };
         l = over_tokens(l);
-        m[0] *= q_scale[0], m[1] *= q_scale[1];  // from here on in powers of two
+        const float m[2] = {unit_up - shift[0], unit_up - shift[1]};
         if (g == 0) s_max[warp][2 * t] = m[0], s_max[warp][2 * t + 1] = m[1];
         ctas_sync();
         const int active = min(kPaWarps, end - at.first_chunk());
         float top[2] = {s_max[0][2 * t], s_max[0][2 * t + 1]};
         for (int w = 1; w < active; ++w) top[0] = fmaxf(top[0], s_max[w][2 * t]), top[1] = fmaxf(top[1], s_max[w][2 * t + 1]);
         if (warp < active) {
-            const float unit = power_of_two(-unit_up);
+            const float unit = power_of_two(-static_cast<int>(unit_up));
             const float weight[2] = {m[0] == top[0] ? 1.f : fast_exp2(m[0] - top[0]), m[1] == top[1] ? 1.f : fast_exp2(m[1] - top[1])};
             if (g == 0) s_sum[warp][2 * t] = l.x * unit * weight[0], s_sum[warp][2 * t + 1] = l.y * unit * weight[1];
             float base[2][2];  // [group][head]
@@ -523,28 +582,27 @@ __global__ void __launch_bounds__(1024) paged_merge_kernel(const PagedParams p, 
     __shared__ float4 s_out[32][32];
     __shared__ float s_total[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = warp / split, turn = warp - head * split, unit = blockIdx.x;
-    wait_for_previous_launch();
-    let_next_launch_start();
+    // The lengths may be read at once: this kernel starts when every CTA of the first one has seen the end of what came before
+    // (or the table has no width, and they do not count).
     const int sequence = unit / p.heads, kv_head = unit - sequence * p.heads;
-    const int length = length_of(p, sequence);
     const int64_t row = static_cast<int64_t>(sequence) * p.heads * p.group + kv_head * p.group + head;
-    if (length == 0) {
-        if (turn == 0) *reinterpret_cast<uint2*>(p.out + row * kHeadDim + 4 * lane) = make_uint2(0, 0);
-        if (p.lse && threadIdx.x % (32 * split) == 0) p.lse[row] = -INFINITY;
-        return;
-    }
-    int64_t all = 0, before = 0;
+    int all = 0, before = 0;
     for (int s = lane; s < p.sequences; s += 32) {
         const int n = stretch_of(length_of(p, s));
         all += n, before += s < sequence ? n : 0;
     }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1)
-        all += __shfl_xor_sync(0xffffffffu, all, off), before += __shfl_xor_sync(0xffffffffu, before, off);
-    const Shares shares = shares_of(p, all);
-    const int per = stretch_of(length);
-    const int64_t a = before * p.heads + static_cast<int64_t>(kv_head) * per;
-    const int from = shares.owner(a + kPaCharge), to = shares.owner(a + per - 1);
+    all = __reduce_add_sync(0xffffffffu, all), before = __reduce_add_sync(0xffffffffu, before);
+    const int length = length_of(p, sequence), per = stretch_of(length);
+    const Shares shares(p, all * p.heads);
+    const int a = before * p.heads + kv_head * per;
+    const int from = length ? shares.owner(a + kPaCharge) : 0, to = length ? shares.owner(a + per - 1) : 0;
+    wait_for_previous_launch();
+    let_next_launch_start();
+    if (length == 0) {
+        if (turn == 0) *reinterpret_cast<uint2*>(p.out + row * kHeadDim + 4 * lane) = make_uint2(0, 0);
+        if (p.lse && turn == 0 && lane == 0) p.lse[row] = -INFINITY;
+        return;
+    }
     if (from == to) return;
     const int count = to - from + 1;
     const int skip = shares.begin(from) < a ? 1 : 0;  // the last page of another unit lies in front of it in its first CTA: that CTA's second part
@@ -618,7 +676,7 @@ extern "C" int reskv_paged_attention(const void* q, int bf16, int64_t q_sequence
                     kv_heads, q_heads, page_count);
     if (q_heads / kv_heads > kPagedGroup) return fail(RESKV_ERR_LIMIT, "paged_attention: more than %d query heads per KV head", kPagedGroup);
     if (!(scaling > 0.f) || !(scaling < 3.0e38f)) return fail(RESKV_ERR_INVALID, "paged_attention: scaling must be positive and finite");
-    if (static_cast<int64_t>(sequences) * kv_heads > 0x7fffffff || width > (1 << 24))
+    if (static_cast<int64_t>(sequences) * kv_heads * (static_cast<int64_t>(width) + kPaCharge) > 0x3fffffff || width > (1 << 24))
         return fail(RESKV_ERR_LIMIT, "paged_attention: %d sequences of up to %d pages", sequences, width);
     if (sequences == 0) return RESKV_OK;
     if (!q || !lengths || !out || !status || (width > 0 && (!table || !pages))) return fail(RESKV_ERR_INVALID, "paged_attention: null pointer");
