@@ -450,7 +450,7 @@ int reskv_kmeans_incremental(const void* x, int batch, int kv_heads, int tokens,
  *                16-byte boundaries
  *   cu_seqlens   i32 [sequences + 1] in device memory: sequence s holds tokens [cu[s], cu[s+1]); clamped to
  *                [0, total], lengths may be 0
- *   out          [total, q_heads, 128] of the same type, 16-byte aligned, lse f32 [total, q_heads] or NULL:
+ *   out          [total, q_heads, 128] of the same type, 32-byte aligned, lse f32 [total, q_heads] or NULL:
  *                log of the sum of exponentials.  Rows of no sequence are left as they are.
  * reskv_prompt_attention_status: RESKV_STATUS_* bits of all calls on the device so far (copies four bytes
  * to the host and synchronises `stream`). */

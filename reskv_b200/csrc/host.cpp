@@ -857,8 +857,8 @@ PyObject* py_prompt_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
         if (cu.dim() != 1 || cu.size(0) < 1 || cu.scalar_type() != at::kInt || cu.size(0) > 0x7fffffff)
             value_error("cu_seqlens must be int32 [sequences + 1]");
         if (!(scaling > 0.0) || !(scaling < 3.0e38)) value_error("scaling must be positive and finite");
-        if (out.defined() && (out.sizes() != x[0].sizes() || out.scalar_type() != type || !out.is_contiguous() || !aligned16(out.const_data_ptr())))
-            value_error("out must be contiguous, of the query's shape and type, on a 16-byte boundary");
+        if (out.defined() && (out.sizes() != x[0].sizes() || out.scalar_type() != type || !out.is_contiguous() || (reinterpret_cast<uintptr_t>(out.const_data_ptr()) & 31u)))
+            value_error("out must be contiguous, of the query's shape and type, on a 32-byte boundary");
         refuse_gradients({x[0], x[1], x[2], out}, "prompt_attention");
         {
             const Unlocked free;

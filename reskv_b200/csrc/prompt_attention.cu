@@ -1,7 +1,26 @@
 // Attention over whole prompts that lie one behind the other in packed tensors: for token i of a sequence and every query
 // head, out_i = sum_j softmax_j(q_i . k_j * scaling) v_j over the keys j <= i (causal) or over all keys of the sequence.
-#include <cuda_bf16.h>
-
+//
+// Both products run on tcgen05.mma.  A row tile is 128 rows: the query heads of one KV head for as many tokens as fit, so that
+// grouped heads share the keys and a short sequence still fills rows; an item is two row tiles.  Per tile of 128 keys: scores
+// S = Q K^T into tensor memory, one thread per row forms the weights with a running maximum (it lags by up to 2^8, so that the
+// output is rarely rescaled) and puts them in the scores' place, and the output accumulates P V with P read from tensor memory.
+// While one row tile's threads work the other's products run.  Tiles arrive by TMA through a ring of five.
+//
+// Items are ordered by their place in their sequence, last ones first, which with causal attention are the longest; the grid has
+// a CTA for every item that there may be, and a CTA that has finished takes over one that has not started (cluster launch
+// control), so it keeps its tensor memory and its ring.
+//
+// What is masked counts for nothing: masked scores are replaced, rows of V behind the sequence are cleared in shared memory, and
+// infinities or NaN in rows of V that only part of a row tile sees are cleared there too and added where they are seen.
+//
+// Bound (1 x 8192 tokens, 32 / 8 heads, 550 GFLOP): 463 us = 1.19 PFLOP/s in short runs, 520 us in long ones under the power cap.
+// An iteration of two row tiles takes 3100 cycles where its products need 2048: 1900 of a row tile's chain are its softmax (16
+// exponentials per clock and SM are 1024 of them), the rest the products and four hand-overs.  Exponentials by a polynomial for a
+// quarter to a half of the weights: no faster.  Two threads per row (16 softmax warps): 502 us.  What the MMA warp's descriptors
+// depend on has to be uniform for the compiler: 550 -> 463 us; its loop in one thread: 512 us.  Outputs stored by row, 16 bytes a
+// lane, instead of by lines: seven ragged prompts 106 -> 100 us.
+#include "pairs.cuh"
 #include "tensor_map.cuh"
 #include "tmem.cuh"
 #include "umma.cuh"
@@ -95,24 +114,9 @@ __device__ PromptItem find_item(const PromptParams& p, int index, int lane) {
     return it;
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float r;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    uint32_t r;
-    if (BF16)
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    else
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
 
@@ -121,7 +125,7 @@ __device__ __forceinline__ float unpack(unsigned short bits) {
     return BF16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16) : __half2float(__ushort_as_half(bits));
 }
 
-// Whether one of the two 16-bit numbers is infinite or NaN.
+// Whether a 16-bit number is infinite or NaN.
 template <bool BF16>
 __device__ __forceinline__ bool non_finite(unsigned short bits) {
     constexpr unsigned short mask = BF16 ? 0x7F80 : 0x7C00;
@@ -170,6 +174,21 @@ __device__ __forceinline__ bool wait_once(bool& lost, uint64_t* bar, uint32_t pa
     return !lost;
 }
 
+// Whether the next item has been posted: every warp waits for that whether it has lost a wait before or not, and longer than for all
+// else together, so that the warps leave together.
+__device__ __forceinline__ bool item_posted(uint64_t* bar, uint32_t parity) {
+    for (int i = 0; i < 16; ++i)
+        if (mbar_wait(bar, parity)) return true;
+    return false;
+}
+
+// 32 bytes, on a 32-byte boundary.
+__device__ __forceinline__ void store32(void* to, const uint32_t (&v)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
 template <bool BF16>
 __global__ void __launch_bounds__(kPThreads, 1)
 prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
@@ -186,8 +205,8 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
         mbar_init(&sh.q_full, 1), mbar_init(&sh.q_empty, 1), mbar_init(&sh.cancel, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.s_full[i], 1), mbar_init(&sh.o_done[i], 1);
-            mbar_init(&sh.p_ready[i][0], 128), mbar_init(&sh.p_ready[i][1], 128);
-            mbar_init(&sh.item_full[i], 1), mbar_init(&sh.item_empty[i], 257);  // softmax threads, MMA warp
+            mbar_init(&sh.p_ready[i][0], 4), mbar_init(&sh.p_ready[i][1], 4);  // a warp each
+            mbar_init(&sh.item_full[i], 1), mbar_init(&sh.item_empty[i], 9);  // softmax warps, MMA warp
         }
         mbar_fence_init();
     }
@@ -206,7 +225,7 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
         if (warp == 9) {
             // ---- copies, and the next item: the grid has a CTA for every item that there may be, and a CTA that has finished takes
             // over one that has not started yet -------------------------------------------------------------------------------
-            int index = blockIdx.x, tile = 0;
+            int index = blockIdx.x, tile = 0, queries = 0;  // queries: items whose rows have been asked for
             for (int n = 0;; ++n) {
                 const int slot = n & 1;
                 const PromptItem it = find_item(p, index, lane);
@@ -218,7 +237,6 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                     mbar_arrive(&sh.item_full[slot]);
                 }
                 if (it.tiles0 == 0 || lost) break;
-                if (n > 0) wait_once(lost, &sh.q_empty, (n - 1) & 1);
                 const int kv_tiles = max(it.tiles0, it.tiles1), row_tiles = it.tiles1 ? 2 : 1;
                 if (lane == 0) {
                     mbar_arrive_expect_tx(&sh.cancel, 16);
@@ -226,11 +244,6 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                                      smem_u32(&sh.cancel_reply)),
                                  "r"(smem_u32(&sh.cancel))
                                  : "memory");
-                    mbar_arrive_expect_tx(&sh.q_full, row_tiles * rows * 256);
-                    for (int i = 0; i < row_tiles; ++i)
-                        for (int h = 0; h < 2; ++h)
-                            tma_load_3d(qs + i * kPTile + h * kPHalf, &q_map, 64 * h, it.head * p.group, it.start + it.token0 + i * p.tile_tokens,
-                                        &sh.q_full);
                 }
                 for (int j = 0; j < 2 * kv_tiles; ++j, ++tile) {
                     const int stage = tile % kPStages;
@@ -241,6 +254,22 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                         for (int h = 0; h < 2; ++h)
                             tma_load_3d(ring + stage * kPTile + h * kPHalf, j & 1 ? &v_map : &k_map, 64 * h, it.head,
                                         it.start + (j >> 1) * kPKeys, &sh.kv_full[stage]);
+                    }
+                    __syncwarp();
+                    if (j > 0) continue;
+                    // the first keys are on their way before the query tiles of the item in front are given back
+                    if (n > 0) wait_once(lost, &sh.q_empty, (n - 1) & 1);
+                    if (lost) {
+                        ++tile;
+                        break;
+                    }
+                    ++queries;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&sh.q_full, row_tiles * rows * 256);
+                        for (int i = 0; i < row_tiles; ++i)
+                            for (int h = 0; h < 2; ++h)
+                                tma_load_3d(qs + i * kPTile + h * kPHalf, &q_map, 64 * h, it.head * p.group,
+                                            it.start + it.token0 + i * p.tile_tokens, &sh.q_full);
                     }
                     __syncwarp();
                 }
@@ -261,81 +290,102 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
             }
             if (lost) {  // no copy may land after the block's end
                 for (int t = tile > kPStages ? tile - kPStages : 0; t < tile; ++t) mbar_wait(&sh.kv_full[t % kPStages], (t / kPStages) & 1);
+                if (queries > 0) mbar_wait(&sh.q_full, (queries - 1) & 1);
             }
         } else if (warp == 8) {
             // ---- MMAs: per key tile and row tile scores = Q K^T, output += P V; the scores of the next key tile follow the output
             // in turn, so a row tile's softmax runs beside the other's products -----------------------------------------------
-            const uint32_t score_idesc = umma_idesc(128, false, false, BF16), value_idesc = umma_idesc(128, false, true, BF16);
-            const uint64_t q0 = umma_desc(smem_u32(qs), 16, 1024), k0 = umma_desc(smem_u32(ring), 16, 1024);
-            const uint64_t v0 = umma_desc(smem_u32(ring), kPHalf, 1024);
-            int tile = 0;  // place in the ring
-            uint32_t made[2] = {0, 0};
-            const auto scores = [&](int i, int stage) {
-                if (elect_one()) {
-    #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) {
-                        const uint64_t step = static_cast<uint64_t>(((ks >> 2) * kPHalf + (ks & 3) * 32) >> 4);
-                        umma_f16(tmem + kPColS + i * 128, q0 + static_cast<uint64_t>((i * kPTile) >> 4) + step,
-                                 k0 + static_cast<uint64_t>((stage * kPTile) >> 4) + step, score_idesc, ks > 0);
+            // This warp's instructions are close to what bounds it.  A product takes its descriptors from uniform registers; what they
+            // depend on is therefore kept uniform in the compiler's eyes too (reductions over the warp), or each costs moves that take
+            // longer than the product.
+            constexpr uint32_t kFull = 0xffffffffu;
+            constexpr uint32_t score_idesc = umma_idesc(128, false, false, BF16), value_idesc = umma_idesc(128, false, true, BF16);
+            const UmmaDesc q0 = umma_desc_halves(smem_u32(qs), 16, 1024), k0 = umma_desc_halves(smem_u32(ring), 16, 1024);
+            const UmmaDesc v0 = umma_desc_halves(smem_u32(ring), kPHalf, 1024);
+            const uint32_t columns = __reduce_or_sync(kFull, tmem);
+            const bool issues = elect_one();
+            uint32_t stage = 0, parity = 0, made[2] = {0, 0};  // stage: of the next tile in the ring
+            const auto step = [&] {
+                if (++stage == kPStages) stage = 0, parity ^= 1;
+            };
+            const auto scores = [&](int i, uint32_t at_stage) {
+                const uint32_t d = columns + kPColS + i * 128, q = q0.low + ((i * kPTile) >> 4), k = k0.low + at_stage * (kPTile >> 4);
+                if (issues) {
+                    umma_f16<false>(d, q, k, k0.high, score_idesc);
+#pragma unroll
+                    for (int ks = 1; ks < 8; ++ks) {
+                        const uint32_t at = ((ks >> 2) * kPHalf + (ks & 3) * 32) >> 4;
+                        umma_f16<true>(d, q + at, k + at, k0.high, score_idesc);
                     }
                     umma_commit(&sh.s_full[i]);
                 }
                 __syncwarp();
             };
-            const auto values = [&](int i, int stage, int half, bool first) {
-                if (elect_one()) {
-    #pragma unroll
-                    for (int k4 = 0; k4 < 4; ++k4) {
-                        const int ks = half * 4 + k4;
-                        umma_f16_ta(tmem + kPColO + i * 128, tmem + kPColS + i * 128 + ks * 8,
-                                    v0 + static_cast<uint64_t>((stage * kPTile + ks * 2048) >> 4), value_idesc, !first || ks > 0);
-                    }
+            const auto values = [&](int i, uint32_t at_stage, int half, uint32_t accumulate) {
+                const uint32_t d = columns + kPColO + i * 128, a = columns + kPColS + i * 128 + half * 32;
+                const uint32_t v = v0.low + at_stage * (kPTile >> 4) + half * (4 * 2048 >> 4);
+                if (issues) {
+                    umma_f16_ta(d, a, v, v0.high, value_idesc, accumulate);
+#pragma unroll
+                    for (int ks = 1; ks < 4; ++ks) umma_f16_ta(d, a + ks * 8, v + ks * (2048 >> 4), v0.high, value_idesc, 1);
                 }
                 __syncwarp();
             };
             const auto commit = [&](uint64_t* bar) {
-                if (elect_one()) umma_commit(bar);
+                if (issues) umma_commit(bar);
                 __syncwarp();
             };
-            for (int n = 0;; ++n) {
+            int n = 0;
+            for (;; ++n) {
                 const int slot = n & 1;
-                wait_once(lost, &sh.item_full[slot], (n >> 1) & 1);
-                const PromptItem it = sh.item[slot];
-                __syncwarp();
+                if (!item_posted(&sh.item_full[slot], (n >> 1) & 1)) lost = true;
+                const int tiles0 = __reduce_max_sync(kFull, sh.item[slot].tiles0), tiles1 = __reduce_max_sync(kFull, sh.item[slot].tiles1);
                 if (lane == 0) mbar_arrive(&sh.item_empty[slot]);
-                if (it.tiles0 == 0 || lost) break;
-                const int kv_tiles = max(it.tiles0, it.tiles1);
+                if (tiles0 == 0 || __any_sync(kFull, lost)) break;
+                const int kv_tiles = max(tiles0, tiles1);
                 wait_once(lost, &sh.q_full, n & 1);
-                wait_once(lost, &sh.kv_full[tile % kPStages], (tile / kPStages) & 1);
+                wait_once(lost, &sh.kv_full[stage], parity);
                 tc_fence_after();
-                scores(0, tile % kPStages);
-                if (it.tiles1) scores(1, tile % kPStages);
-                commit(&sh.kv_empty[tile % kPStages]);
+                scores(0, stage);
+                if (tiles1) scores(1, stage);
+                commit(&sh.kv_empty[stage]);
                 if (kv_tiles == 1) commit(&sh.q_empty);
+                step();
                 for (int j = 0; j < kv_tiles; ++j) {
-                    const int vt = tile + 2 * j + 1, kt = vt + 1, v_stage = vt % kPStages, k_stage = kt % kPStages;
+                    const uint32_t v_stage = stage;
                     const bool more = j + 1 < kv_tiles;
-                    wait_once(lost, &sh.kv_full[v_stage], (vt / kPStages) & 1);
-                    if (more) wait_once(lost, &sh.kv_full[k_stage], (kt / kPStages) & 1);
+                    wait_once(lost, &sh.kv_full[v_stage], parity);
+                    step();
+#pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const int tiles = i ? it.tiles1 : it.tiles0;
-                        if (j >= tiles) continue;
-    #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            wait_once(lost, &sh.p_ready[i][half], made[i] & 1);
-                            tc_fence_after();
-                            values(i, v_stage, half, j == 0);
+                        const int tiles = i ? tiles1 : tiles0;
+                        if (j < tiles) {
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                wait_once(lost, &sh.p_ready[i][half], made[i] & 1);
+                                tc_fence_after();
+                                values(i, v_stage, half, half > 0 || j > 0);
+                            }
+                            ++made[i];
                         }
-                        ++made[i];
-                        if (j + 1 < tiles) scores(i, k_stage); else commit(&sh.o_done[i]);
+                        // every stage goes back as soon as its last product has run, and the keys are waited for when they are
+                        // needed: a copy then has more than an iteration's time
+                        if (i == 1) commit(&sh.kv_empty[v_stage]);
+                        if (i == 0 && more) wait_once(lost, &sh.kv_full[stage], parity);
+                        if (j < tiles) {
+                            if (j + 1 < tiles) scores(i, stage); else commit(&sh.o_done[i]);
+                        }
                     }
-                    commit(&sh.kv_empty[v_stage]);
-                    if (more) commit(&sh.kv_empty[k_stage]);
+                    if (more) {
+                        commit(&sh.kv_empty[stage]);
+                        step();
+                    }
                     if (j + 2 == kv_tiles) commit(&sh.q_empty);
                 }
-                tile += 2 * kv_tiles;
             }
-            if (tile > 0) wait_once(lost, &sh.kv_empty[(tile - 1) % kPStages], ((tile - 1) / kPStages) & 1);  // the last commit has arrived
+            // the last commits have arrived before the block ends
+            const uint32_t last = stage ? stage - 1 : kPStages - 1;
+            if (n > 0) wait_once(lost, &sh.kv_empty[last], stage ? parity : parity ^ 1);
         }
     } else {
         // ---- softmax and output: thread = row -----------------------------------------------------------------------------
@@ -349,9 +399,10 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
         int tile = 0;
         for (int n = 0;; ++n) {
             const int slot = n & 1;
-            wait_once(lost, &sh.item_full[slot], (n >> 1) & 1);
+            const bool posted = item_posted(&sh.item_full[slot], (n >> 1) & 1);
             const PromptItem it = sh.item[slot];
-            if (it.tiles0 == 0 || lost) break;
+            lost |= !posted;
+            if (it.tiles0 == 0 || !posted) break;
             const int tiles = i ? it.tiles1 : it.tiles0, other = i ? it.tiles0 : it.tiles1;
             const int first_token = it.token0 + i * p.tile_tokens, token = first_token + row_token;
             const int limit = p.causal ? token : it.len - 1;  // last key that the row sees
@@ -402,34 +453,37 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                 }
                 // an infinite maximum: inf - inf, NaN for the whole row as in the formula
                 const float shift = m == INFINITY ? __int_as_float(0x7fffffff) : -m * scale;
-                float sum[2] = {0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                const float2 scales = make_float2(scale, scale), shifts = make_float2(shift, shift);
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                const auto weights = [&](int c) {  // of 32 keys
                     float packed[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float a = fast_exp2(fmaf(s[c][e], scale, shift)), b = fast_exp2(fmaf(s[c][e + 1], scale, shift));
-                        sum[0] += a, sum[1] += b;
-                        packed[e / 2] = __uint_as_float(pack2<BF16>(a, b));
+                    for (int e = 0; e < 16; ++e) {
+                        const float2 x = fma2(make_float2(s[c][2 * e], s[c][2 * e + 1]), scales, shifts);
+                        const float2 y = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+                        sum[e & 1] = add2(sum[e & 1], y);
+                        packed[e] = __uint_as_float(pack2<BF16>(y.x, y.y));
                     }
                     tmem_st16(s_at + c * 16, packed);
-                    if (c == 1) {
-                        tmem_st_wait();
-                        if (masked && (i == 0 || j >= other)) {
-                            const int vt = tile + 2 * j + 1, stage = vt % kPStages;
-                            wait_once(lost, &sh.kv_full[stage], (vt / kPStages) & 1);
-                            const bool behind = j * kPKeys + row >= it.len;
-                            if ((behind || p.causal) && tame_value_row<BF16>(ring + stage * kPTile + row * 128, behind, lane)) sh.tamed[slot] = 1;
-                            proxy_fence();
-                        }
-                        tc_fence_before();
-                        mbar_arrive(&sh.p_ready[i][0]);
-                    }
+                };
+                const auto hand_over = [&](int half) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.p_ready[i][half]);
+                };
+                weights(0), weights(1);
+                if (masked && (i == 0 || j >= other)) {
+                    const int vt = tile + 2 * j + 1, stage = vt % kPStages;
+                    wait_once(lost, &sh.kv_full[stage], (vt / kPStages) & 1);
+                    const bool behind = j * kPKeys + row >= it.len;
+                    if ((behind || p.causal) && tame_value_row<BF16>(ring + stage * kPTile + row * 128, behind, lane)) sh.tamed[slot] = 1;
+                    proxy_fence();
                 }
-                tmem_st_wait();
-                tc_fence_before();
-                mbar_arrive(&sh.p_ready[i][1]);
-                l += sum[0] + sum[1];
+                hand_over(0);
+                weights(2), weights(3);
+                hand_over(1);
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
             if (tiles) {
                 wait_once(lost, &sh.o_done[i], items & 1);
@@ -439,32 +493,54 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                 const bool tamed = *static_cast<volatile int*>(&sh.tamed[slot]) != 0;
                 const int64_t at = (static_cast<int64_t>(it.start + token) * p.kv_heads + it.head) * p.group + row_head;
                 const float inv = 1.f / l;
+                const uint32_t alive = __ballot_sync(0xffffffffu, live);
+                // 64 columns (128 bytes) at a time.  Four lanes exchange their rows' quarters, so that together they write a row's 128
+                // bytes: a line per four lanes where every lane's own row would be 32 lines an instruction.
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    float o[32];
-                    tmem_ld32(o_at + c * 32, o);
-                    tmem_ld_wait(o);
-                    if (tamed && live) {  // what was cleared reaches the rows that see it
-                        for (int key = it.token0 / kPKeys * kPKeys; key <= limit; ++key) {
-                            const unsigned short* from = p.v + (it.start + key) * p.v_token + it.head * p.v_head + c * 32;
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t v[4][8];
 #pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                if (non_finite<BF16>(from[e])) o[e] += unpack<BF16>(from[e]);
+                    for (int d = 0; d < 2; ++d) {
+                        float o[32];
+                        tmem_ld32(o_at + c * 64 + d * 32, o);
+                        tmem_ld_wait(o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] *= inv;
+                        if (tamed && live) {  // what was cleared reaches the rows that see it
+                            for (int key = it.token0 / kPKeys * kPKeys; key <= limit; ++key) {
+                                const unsigned short* from = p.v + (it.start + key) * p.v_token + it.head * p.v_head + c * 64 + d * 32;
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (non_finite<BF16>(from[e])) o[e] += unpack<BF16>(from[e]);
+                            }
                         }
-                    }
-                    if (live) {
-                        uint4* to = reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.out) + at * 128 + c * 32);
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8)
-                            to[e / 8] = make_uint4(pack2<BF16>(o[e] * inv, o[e + 1] * inv), pack2<BF16>(o[e + 2] * inv, o[e + 3] * inv),
-                                                   pack2<BF16>(o[e + 4] * inv, o[e + 5] * inv), pack2<BF16>(o[e + 6] * inv, o[e + 7] * inv));
+                        for (int e = 0; e < 16; ++e) v[2 * d + (e >> 3)][e & 7] = pack2<BF16>(o[2 * e], o[2 * e + 1]);
+                    }
+#pragma unroll
+                    for (int step = 1; step < 4; step <<= 1)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            if (x & step) continue;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const bool upper = lane & step;
+                                const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? v[x][e] : v[x | step][e], step);
+                                if (upper) v[x][e] = got; else v[x | step][e] = got;
+                            }
+                        }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {  // row x of the four
+                        const int64_t there = __shfl_sync(0xffffffffu, at, (lane & 28) + x);
+                        if (alive >> ((lane & 28) + x) & 1) store32(static_cast<unsigned short*>(p.out) + there * 128 + c * 64 + (lane & 3) * 16, v[x]);
                     }
                 }
                 tc_fence_before();
                 if (live && p.lse) p.lse[at] = m * scale * kLn2 + logf(l);
             }
             tile += 2 * max(it.tiles0, it.tiles1);
-            mbar_arrive(&sh.item_empty[slot]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.item_empty[slot]);
         }
     }
     if (lost) atomicOr(&g_prompt_status, RESKV_STATUS_WAIT_TIMEOUT);
@@ -519,7 +595,7 @@ extern "C" int reskv_prompt_attention(const void* q, const void* k, const void* 
     if (int rc = check_rows("q", q, q_token, q_head)) return rc;
     if (int rc = check_rows("k", k, k_token, k_head)) return rc;
     if (int rc = check_rows("v", v, v_token, v_head)) return rc;
-    if (!aligned16(out)) return fail(RESKV_ERR_INVALID, "prompt_attention: out must start on a 16-byte boundary");
+    if (reinterpret_cast<uintptr_t>(out) & 31u) return fail(RESKV_ERR_INVALID, "prompt_attention: out must start on a 32-byte boundary");
     if (int rc = check_device_pointer(out, "prompt_attention", "out")) return rc;
     if (int rc = check_device_pointer(cu_seqlens, "prompt_attention", "cu_seqlens")) return rc;
     PromptParams p{};

@@ -25,12 +25,29 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a, uint64_t b
         : "memory");
 }
 
-// The same with A in tensor memory: row r in lane r, two 16-bit elements of a row in a column.
-__device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Descriptors in halves, for the compiler to add to the low one only: the address (in units of 16 bytes) is in its low bits.
+struct UmmaDesc {
+    uint32_t low, high;
+};
+__device__ __forceinline__ UmmaDesc umma_desc_halves(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
+    const uint64_t d = umma_desc(saddr, lbo_bytes, sbo_bytes);
+    return {static_cast<uint32_t>(d), static_cast<uint32_t>(d >> 32)};
+}
+template <bool ACCUMULATE>
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t high, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_low), "r"(b_low), "r"(high), "r"(idesc), "n"(ACCUMULATE ? 1 : 0)
+        : "memory");
+}
+
+// The same with A in tensor memory: row r in lane r, two 16-bit elements of a row in a column.
+__device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_low, uint32_t b_high, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_low), "r"(b_high), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 
