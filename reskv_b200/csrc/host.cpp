@@ -1056,6 +1056,53 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
     });
 }
 
+// Page numbers of a sequence.
+std::vector<int32_t> page_numbers(PyObject* o, const char* what) {
+    PyObject* fast = PySequence_Fast(o, what);
+    if (!fast) throw PyError{};
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast);
+    std::vector<int32_t> v;
+    bool whole = n <= 0x7fffffff;
+    try {
+        v.resize(whole ? n : 0);
+    } catch (...) {
+        Py_DECREF(fast);
+        throw;
+    }
+    for (Py_ssize_t i = 0; whole && i < n; ++i) {
+        PyObject* x = PySequence_Fast_GET_ITEM(fast, i);
+        int over = 0;
+        const long long value = PyLong_Check(x) ? PyLong_AsLongLongAndOverflow(x, &over) : -1;
+        whole = PyLong_Check(x) && !over && value >= 0 && value <= 0x7fffffff;
+        v[i] = static_cast<int32_t>(value);
+    }
+    Py_DECREF(fast);
+    if (!whole) value_error(std::string(what) + " must be a sequence of page numbers");
+    return v;
+}
+
+// copy_pages(pages, src, dst): pages [layers, pages, ...] of bytes, in every layer
+PyObject* py_copy_pages(PyObject*, PyObject* const* o, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        expect(n, 3);
+        const at::Tensor pages = tensor(o[0], "pages");
+        if (pages.dim() < 2 || !pages.is_cuda() || !pages.is_contiguous() || pages.size(0) > 0x7fffffff || pages.size(1) > 0x7fffffff)
+            value_error("pages must be dense CUDA [layers, pages, ...]");
+        const std::vector<int32_t> src = page_numbers(o[1], "src"), dst = page_numbers(o[2], "dst");
+        if (src.size() != dst.size()) value_error("as many sources as destinations are needed");
+        if (!src.empty()) {
+            const Unlocked free;
+            const c10::DeviceIndex dev = pages.get_device();
+            const c10::cuda::CUDAGuard guard(dev);
+            check(reskv_copy_pages(pages.data_ptr(), static_cast<int>(pages.size(0)), static_cast<int>(pages.size(1)),
+                                   pages.stride(1) * static_cast<int64_t>(pages.element_size()), src.data(), dst.data(), static_cast<int>(src.size()),
+                                   c10::cuda::getCurrentCUDAStream(dev).stream()));
+            g_launches += static_cast<long long>((src.size() + 479) / 480);
+        }
+        return Py_NewRef(Py_None);
+    });
+}
+
 PyObject* py_launches(PyObject*, PyObject*) { return PyLong_FromLongLong(g_launches); }
 
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f))
@@ -1066,6 +1113,7 @@ PyMethodDef g_methods[] = {
     {"paged_write", FAST(py_paged_write), METH_FASTCALL, "tokens into a 4-bit paged cache"},
     {"paged_read", FAST(py_paged_read), METH_FASTCALL, "values of tokens of a 4-bit paged cache"},
     {"paged_attention", FAST(py_paged_attention), METH_FASTCALL, "one query per sequence against a 4-bit paged cache"},
+    {"copy_pages", FAST(py_copy_pages), METH_FASTCALL, "copy pages of a pool in every layer"},
     {"window_append", FAST(py_window_append), METH_FASTCALL, "append one token to the dense window"},
     {"encode", FAST(py_encode), METH_FASTCALL, "pack one side"},
     {"kmeans_pair", FAST(py_kmeans_pair), METH_FASTCALL, "cluster K and V in the same launch"},

@@ -12,7 +12,9 @@ stay local) and the only collectives are the sum all-reduces after ``o_proj``
 and ``down_proj``.
 
 ``cache="dense"`` keeps an ordinary FP16 KV cache instead (SDPA decode): the
-baseline the compressed path is measured against.
+baseline the compressed path is measured against.  ``cache="int4"`` keeps a
+``PagedInt4Cache``: prompts of different lengths in one batch, attended to by
+``prompt_attention`` and stored in 4 bits, rows that fork and go (``select``).
 
 Dense matrix products use torch (cuBLAS); everything that touches the
 compressed cache goes through ``reskv_b200.compress`` / ``attention``.
@@ -33,6 +35,8 @@ import torch.nn.functional as F
 from .._attention import attention
 from ..cache import ResKVLayerCache
 from ..config import ResKVKernelConfig
+from ..paged import PAGE_TOKENS, PagedInt4Cache
+from ..prompt import prompt_attention
 
 try:  # dense baseline only: library flash-decoding kernel, if the image has it
     from flash_attn import flash_attn_with_kvcache as _flash_kvcache
@@ -132,7 +136,7 @@ class _DenseLayerCache:
 
 
 class ResKVLlama:
-    """Random-weight or loaded Llama decoder with a compressed (or dense) KV cache.
+    """Random-weight or loaded Llama decoder with a compressed (or dense, or 4-bit paged) KV cache.
 
     ``generate(ids, new_tokens)`` = prefill + greedy decode.  With a process
     group the model is tensor-parallel over ``group`` (heads and FFN columns are
@@ -141,9 +145,12 @@ class ResKVLlama:
 
     def __init__(self, shape: LlamaShape = LlamaShape(), kernel_config: ResKVKernelConfig | None = None, *,
                  cache: str = "reskv", device="cuda", seed: int = 0, group=None, prefill_chunk: int = 65536,
-                 sink_tokens: int = 0):
-        if cache not in ("reskv", "dense"):
-            raise ValueError("cache must be 'reskv' or 'dense'")
+                 sink_tokens: int = 0, pages: int | None = None):
+        if cache not in ("reskv", "dense", "int4"):
+            raise ValueError("cache must be 'reskv', 'dense' or 'int4'")
+        if pages is not None and (cache != "int4" or type(pages) is not int or pages < 1):
+            raise ValueError("pages is the size of the 4-bit cache's pool, a positive integer")
+        self.pages = pages  # None: as many as the prompt and its reserve need
         self.shape, self.cache_kind, self.device = shape, cache, torch.device(device)
         self.kernel_config = kernel_config or ResKVKernelConfig()
         if not isinstance(self.kernel_config, ResKVKernelConfig):
@@ -189,6 +196,7 @@ class ResKVLlama:
         self.inv_freq = (shape.rope_theta ** (-torch.arange(64, device=self.device).float() / 64)).contiguous()
         self.scaling = hd**-0.5
         self.caches = None
+        self.paged, self.sequences = None, []  # cache="int4": the cache, and the sequence of each row of the batch
         self.length = 0
         self._lib = None
         # graph decode: the last captured graph (owner of the captures' memory pool), batch sizes whose step has run once
@@ -202,7 +210,10 @@ class ResKVLlama:
         return x
 
     def _trig(self, start, n):
-        ang = torch.arange(start, start + n, device=self.device).float()[:, None] * self.inv_freq[None, :]
+        return self._trig_of(torch.arange(start, start + n, device=self.device))
+
+    def _trig_of(self, positions):
+        ang = positions.float()[:, None] * self.inv_freq[None, :]
         return ang.cos(), ang.sin()
 
     def _native(self):
@@ -266,7 +277,11 @@ class ResKVLlama:
 
         Norms, projections, RoPE and the dense causal attention run over slices of the batch (at most
         ``prefill_chunk`` tokens at a time) so that their FP32 temporaries stay small at long contexts;
-        the cache of a layer receives the whole batch at once."""
+        the cache of a layer receives the whole batch at once.
+
+        With ``cache="int4"`` ``ids`` may also be a sequence of prompts ``[T_i]`` of different lengths."""
+        if self.cache_kind == "int4":
+            return self._prefill_paged(list(ids), reserve)
         b, t = ids.shape
         trig = self._trig(0, t)
         x = self.embed[ids]
@@ -297,12 +312,63 @@ class ResKVLlama:
         self.length = t
         return self._logits(x[:, -1:])
 
+    def _prefill_paged(self, prompts, reserve):
+        lengths = [p.numel() for p in prompts]
+        if not prompts or any(p.ndim != 1 or p.numel() == 0 for p in prompts):
+            raise ValueError("prompts must be one-dimensional and hold a token at least")
+        if type(reserve) is not int or reserve < 0:
+            raise ValueError("reserve must be a non-negative integer")
+        need = sum(-(-(t + reserve) // PAGE_TOKENS) for t in lengths)
+        self.paged = self.caches = self._step = None  # the pool in front goes before the next one comes
+        self.paged = PagedInt4Cache(self.shape.layers, self.h_kv, self.pages or need, dtype=torch.float16, device=self.device)
+        self.sequences = self.paged.add(len(prompts))
+        self.caches, self._graph, self._reserve = [self.paged], None, reserve
+        x = self.embed[torch.cat([p.to(self.device) for p in prompts])].unsqueeze(0)
+        # whole prompts, at most prefill_chunk tokens together: (step, rows of x, sin and cos)
+        parts, at = [], 0
+        while at < len(prompts):
+            end, first = at + 1, sum(lengths[:at])
+            while end < len(prompts) and sum(lengths[at:end + 1]) <= self.prefill_chunk:
+                end += 1
+            step = self.paged.extend(self.sequences[at:end], lengths[at:end])
+            positions = torch.cat([torch.arange(t, device=self.device) for t in lengths[at:end]])
+            parts.append((step, slice(first, first + step.total), self._trig_of(positions)))
+            at = end
+        for index, layer in enumerate(self.layers):
+            for step, rows, trig in parts:
+                k, kr, v = torch.empty((3, 1, self.h_kv, step.total, 128), dtype=torch.float16, device=self.device)
+                _, qr = self._qkv(layer, x[:, rows], trig, k, kr, v)
+                keys, values = kr[0].transpose(0, 1), v[0].transpose(0, 1)
+                self.paged.write(index, step, keys, values)
+                att = prompt_attention(qr[0].transpose(0, 1), keys, values, step.cu_seqlens, scaling=self.scaling)
+                self._add_projection(x[:, rows], att.view(1, step.total, -1), layer["wo"])
+                del k, kr, v, qr, keys, values, att
+            self._add_mlp(layer, x)
+        ends = torch.tensor(lengths, device=self.device).cumsum(0) - 1
+        return self._logits(x[0, ends].unsqueeze(1))
+
+    def select(self, rows) -> None:
+        """``cache="int4"``: the batch becomes these rows of the present one, a row several times where it forks (samples of one
+        prompt, beams), rows that are not named end."""
+        if self.paged is None:
+            raise RuntimeError("select() needs cache='int4' and a prefilled batch")
+        rows = list(rows)
+        if any(type(r) is not int or not 0 <= r < len(self.sequences) for r in rows):
+            raise ValueError(f"rows must be whole numbers below {len(self.sequences)}")
+        again = [i for i, r in enumerate(rows) if r in rows[:i]]
+        forked = dict(zip(again, self.paged.fork([self.sequences[rows[i]] for i in again])))
+        self.paged.free([s for r, s in enumerate(self.sequences) if r not in rows])
+        self.sequences = [forked.get(i, self.sequences[r]) for i, r in enumerate(rows)]
+        self._graph = None
+
     def _logits(self, x):
         return F.linear(self._norm(x, self.final_norm), self.lm_head)[:, 0].float()
 
     @torch.no_grad()
     def decode(self, tokens: torch.Tensor) -> torch.Tensor:
         """One step for ``tokens [B]``; returns logits ``[B, vocab]``."""
+        if self.cache_kind == "int4":
+            return self._decode_paged(tokens)
         b = tokens.shape[0]
         pos = self.length
         trig = self._trig(pos, 1)
@@ -325,9 +391,27 @@ class ResKVLlama:
         self.length += 1
         return self._logits(x)
 
+    def _rows(self, tokens):
+        if tokens.shape != (len(self.sequences),):
+            raise ValueError(f"a step takes one token for each of the {len(self.sequences)} rows")
+
+    def _decode_paged(self, tokens):
+        self._rows(tokens)
+        step = self.paged.extend(self.sequences, 1)
+        trig = self._trig_of(step.starts)
+        x = self.embed[tokens].unsqueeze(0)
+        for index, layer in enumerate(self.layers):
+            k, kr, v = torch.empty((3, 1, self.h_kv, step.total, 128), dtype=torch.float16, device=self.device)
+            _, qr = self._qkv(layer, x, trig, k, kr, v)
+            self.paged.write(index, step, kr[0].transpose(0, 1), v[0].transpose(0, 1))
+            att = self.paged.attend(index, step, qr[0].transpose(0, 1), scaling=self.scaling)
+            self._add_projection(x, att.view(1, step.total, -1), layer["wo"])
+            self._add_mlp(layer, x)
+        return self._logits(x.transpose(0, 1))
+
     @torch.no_grad()
     def generate(self, ids: torch.Tensor, new_tokens: int) -> torch.Tensor:
-        """Greedy continuation ``[B, new_tokens]`` of the prompt ``ids [B, T]``."""
+        """Greedy continuation ``[B, new_tokens]`` of the prompt ``ids [B, T]`` (``cache="int4"``: or of several prompts)."""
         logits = self.prefill(ids, reserve=new_tokens)
         out = [logits.argmax(-1)]
         for _ in range(new_tokens - 1):
@@ -344,6 +428,8 @@ class ResKVLlama:
 
         linear = ctypes.c_uint32(0)
         check(self._native().reskv_skinny_linear_status(ctypes.addressof(linear), _stream(self.device)), launches=0)
+        if self.cache_kind == "int4":
+            self.paged.check()
         decode = self._workspace[:4].view(torch.int32).item() if self.cache_kind == "reskv" else 0
         if linear.value or decode:
             raise RuntimeError(f"decode step: device status 0x{linear.value:x} (linear layers), 0x{decode:x} (attention)")
@@ -360,8 +446,8 @@ class ResKVLlama:
         b = tok.shape[0]
         d = self.shape.hidden
         stream = _stream(self.device)
-        state = self._state.data_ptr()
-        reskv = self.cache_kind == "reskv"
+        reskv, paged = self.cache_kind == "reskv", self.cache_kind == "int4"
+        state = None if paged else self._state.data_ptr()
 
         def half(*shape):
             return torch.empty(shape, dtype=torch.float16, device=self.device)
@@ -406,12 +492,22 @@ class ResKVLlama:
 
         # one step on: the new token's position, and (compressed cache) its place in the window -- it goes to slot
         # count - 1 and the attention of this step already includes it
-        check(lib.reskv_step_advance(state, 1, 1 if reskv else 0, stream))
+        if paged:  # positions, lengths and pages are in the step's tables, which the host fills before a replay
+            cos, sin = self._trig_of(self._step.starts)
+        else:
+            check(lib.reskv_step_advance(state, 1, 1 if reskv else 0, stream))
         x = self.embed[tok]
-        for index, (layer, cache) in enumerate(zip(self.layers, self.caches)):
+        for index, layer in enumerate(self.layers):
+            cache = self.caches[0 if paged else index]
             qkv = linear(x, layer["wqkv"], layer["norm1"])
             q_rot = half(b * self.h_q, 128)
-            if reskv:
+            if paged:
+                q_rot, (k_raw, k_rot, v_new) = half(self.h_q, b, 128), half(3, self.h_kv, b, 128)
+                check(lib.reskv_rope_prompt(qkv.data_ptr(), 1, b, self.h_q, self.h_kv, cos.data_ptr(), sin.data_ptr(), q_rot.data_ptr(),
+                                            k_raw.data_ptr(), k_rot.data_ptr(), v_new.data_ptr(), stream))
+                cache.write(index, self._step, k_rot.transpose(0, 1), v_new.transpose(0, 1))
+                att = cache.attend(index, self._step, q_rot.transpose(0, 1), scaling=self.scaling).view(b, self.h_q * 128)
+            elif reskv:
                 cap = cache.keys.shape[2]
                 q_raw = half(b * self.h_q, 128)
                 check(lib.reskv_rope_split(qkv.data_ptr(), b, self.h_q, self.h_kv, self.inv_freq.data_ptr(), state,
@@ -453,7 +549,7 @@ class ResKVLlama:
                 gate_up = F.linear(norm(x, layer["norm2"]), layer["w_gate_up"])
                 check(lib.reskv_silu_mul(gate_up.data_ptr(), act.data_ptr(), b, self.ffn, stream))
             x = project(x, act, layer["w_down"])
-        if not reskv:
+        if not reskv and not paged:
             self._seqlens += 1
         vocab = self.lm_head.shape[0]
         if streams(x, self.lm_head, vocab, 3, self.final_norm):
@@ -468,7 +564,11 @@ class ResKVLlama:
 
         self._tok_in = torch.zeros(batch, dtype=torch.long, device=self.device)
         self._graph = self._logits_out = None
-        if self.cache_kind == "reskv":
+        if self.cache_kind == "int4":
+            if batch != len(self.sequences):
+                raise ValueError(f"the batch has {len(self.sequences)} rows")
+            self._step = None
+        elif self.cache_kind == "reskv":
             self._state = torch.zeros(4, dtype=torch.int32, device=self.device)
             # centroid tables at their final shape (zero rows beyond the live count), one pair per layer
             rows = self.kernel_config.max_clusters
@@ -517,13 +617,16 @@ class ResKVLlama:
         with torch.cuda.stream(side):
             if self._tok_in.shape[0] not in self._warm:
                 # once per batch size: a step outside capture (library handles, lazy inits), on a state that is restored
-                reskv = self.cache_kind == "reskv"
-                counts = self._state if reskv else self._seqlens
-                saved, saved_state = counts.clone(), self._state.clone()
-                self._step_body(self._tok_in)
-                self._state.copy_(saved_state)
-                if not reskv:
-                    counts.copy_(saved)
+                if self.cache_kind == "int4":  # a step that is run twice stores its tokens twice, in the same place
+                    self._step_body(self._tok_in)
+                else:
+                    reskv = self.cache_kind == "reskv"
+                    counts = self._state if reskv else self._seqlens
+                    saved, saved_state = counts.clone(), self._state.clone()
+                    self._step_body(self._tok_in)
+                    self._state.copy_(saved_state)
+                    if not reskv:
+                        counts.copy_(saved)
                 self._warm.add(self._tok_in.shape[0])
             graph = torch.cuda.CUDAGraph()
             with _collector_held():
@@ -538,6 +641,8 @@ class ResKVLlama:
     @torch.no_grad()
     def decode_graph(self, tokens: torch.Tensor) -> torch.Tensor:
         """Same result as ``decode`` but replaying a captured CUDA graph of the step."""
+        if self.cache_kind == "int4":
+            self._next_paged_step(tokens)
         if self.cache_kind == "reskv" and self.caches[0].live + 1 == self.caches[0].keys.shape[2]:
             # this token fills the window.  The eager step appends it and then compresses the oldest
             # group before attending (as the reference does); the group does not contain the new
@@ -559,10 +664,25 @@ class ResKVLlama:
                 cache.length += 1
         return self._logits_out
 
+    def _next_paged_step(self, tokens):
+        """Room for one more token of every row, in the tables that the captured step reads; a table that has become too narrow, or
+        another batch, invalidates the graph."""
+        self._rows(tokens)
+        wide = max(-(-(self.paged.length(s) + 1) // PAGE_TOKENS) for s in self.sequences)
+        if self._step is not None and len(self._step.sequences) == len(tokens) and wide <= self._step.table.shape[1]:
+            self._step = self.paged.extend(self.sequences, 1, reuse=self._step)
+        else:
+            more = -(-max(self._reserve, PAGE_TOKENS) // PAGE_TOKENS)
+            self._step, self._graph = self.paged.extend(self.sequences, 1, width=wide + more), None
+            if self._tok_in.shape != tokens.shape:
+                self._tok_in = torch.zeros_like(tokens, device=self.device, dtype=torch.long)
+
     def cache_bytes(self) -> int:
         total = 0
         for c in self.caches or []:
-            if isinstance(c, _DenseLayerCache):
+            if isinstance(c, PagedInt4Cache):
+                total += c.nbytes
+            elif isinstance(c, _DenseLayerCache):
                 total += c.k.nbytes + c.v.nbytes
             else:
                 total += (c.compressed.nbytes if c.compressed is not None else 0)

@@ -19,7 +19,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from ._extension import _stream, bound_library, check, device_index_of, host, require_device
+from ._extension import device_index_of, host, require_device
 
 PAGE_TOKENS = 64
 _PAGE_HEAD = (4, 2304)  # blocks of 16 tokens, bytes of a block
@@ -33,7 +33,8 @@ class PagedStep:
     step.  ``cu_seqlens`` (int32, on the device) says which rows of the packed tensors belong to which sequence and serves
     ``prompt_attention`` as it is."""
 
-    __slots__ = ("sequences", "counts", "lengths", "total", "cu_seqlens", "starts", "device_lengths", "table", "_whole", "_epoch", "_current")
+    __slots__ = ("sequences", "counts", "lengths", "total", "cu_seqlens", "starts", "device_lengths", "table", "_numbers", "_whole", "_epoch",
+                 "_current")
 
     def _everything(self):
         """``(cu_seqlens, starts, tokens)`` of all tokens of the sequences, the earlier ones included."""
@@ -45,11 +46,15 @@ class PagedStep:
         return self._whole
 
 
-def _upload(numbers: np.ndarray, device) -> torch.Tensor:
-    """int32 numbers on the device, without waiting for the copy."""
+def _pinned(numbers: np.ndarray) -> torch.Tensor:
     pinned = torch.empty(numbers.size, dtype=torch.int32, pin_memory=True)
     pinned.numpy()[:] = numbers.reshape(-1)
-    return pinned.to(device, non_blocking=True)
+    return pinned
+
+
+def _upload(numbers: np.ndarray, device) -> torch.Tensor:
+    """int32 numbers on the device, without waiting for the copy."""
+    return _pinned(numbers).to(device, non_blocking=True)
 
 
 class PagedInt4Cache:
@@ -74,7 +79,6 @@ class PagedInt4Cache:
         require_device(self.device.index)
         self.pages = torch.empty((layers, pages, kv_heads, *_PAGE_HEAD), dtype=torch.uint8, device=self.device)
         self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
-        self._lib = bound_library(self.device)
         self._book = PageBook(pages)
 
     # -- sequences -------------------------------------------------------------------------------------------------------------
@@ -89,14 +93,28 @@ class PagedInt4Cache:
     def length(self, sequence: int) -> int:
         return self._book.of(sequence).length
 
-    def extend(self, sequences, counts) -> PagedStep:
+    def extend(self, sequences, counts, *, width: int = 0, reuse: PagedStep | None = None) -> PagedStep:
         """Room for ``counts[i]`` (or ``counts`` for each) more tokens of ``sequences[i]``, no sequence twice.  Earlier steps
-        of these sequences may not be used any more.  RuntimeError, and nothing changed, when the pool has too few pages."""
+        of these sequences may not be used any more.  RuntimeError, and nothing changed, when the pool has too few pages.
+
+        For captured graphs: the page table is made at least ``width`` pages wide, and with ``reuse``, an earlier step of as many
+        sequences, the tables are written to that step's tensors, whose addresses a graph holds.  ValueError, and nothing
+        changed, when a sequence has more pages than that table is wide."""
         book = self._book
         sequences, counts = list(sequences), [counts] * len(sequences) if type(counts) is int else list(counts)
+        if type(width) is not int or width < 0:
+            raise ValueError("width must be a non-negative integer")
+        if reuse is not None:
+            if not isinstance(reuse, PagedStep) or reuse.table.device != self.device or reuse.table.shape[0] != len(sequences):
+                raise ValueError("reuse must be a step of this cache with as many sequences")
+            if type(counts) is list and all(type(c) is int for c in counts) and len(counts) == len(sequences):
+                most = max((-(-(book.of(q).length + c) // PAGE_TOKENS) for q, c in zip(sequences, counts)), default=0)
+                if most > reuse.table.shape[1]:
+                    raise ValueError(f"{most} pages of a sequence do not fit a table of {reuse.table.shape[1]}")
+            width = reuse.table.shape[1]
         entries = book.extend(sequences, counts)
         step = PagedStep()
-        n, width = len(entries), max((len(e.pages) for e in entries), default=0)
+        n, width = len(entries), max([width, *(len(e.pages) for e in entries)])
         step.sequences, step.counts, step.lengths = tuple(sequences), tuple(counts), tuple(e.length for e in entries)
         step.total = sum(counts)
         numbers = np.zeros(3 * n + 1 + n * width, np.int32)
@@ -106,7 +124,13 @@ class PagedInt4Cache:
         table = numbers[3 * n + 1:].reshape(n, width)
         for row, e in zip(table, entries):
             row[:len(e.pages)] = e.pages
-        there = _upload(numbers, self.device)
+        if reuse is None:
+            there = _upload(numbers, self.device)
+        else:
+            there = reuse._numbers
+            there.copy_(_pinned(numbers), non_blocking=True)
+            reuse._current = False
+        step._numbers = there
         step.cu_seqlens, step.starts, step.device_lengths = there[:n + 1], there[n + 1:2 * n + 1], there[2 * n + 1:3 * n + 1]
         step.table = there[3 * n + 1:].view(n, width)
         step._whole, step._epoch, step._current = None, book.epoch, True
@@ -165,22 +189,11 @@ class PagedInt4Cache:
     def copy_pages(self, src, dst) -> None:
         """Copies pages ``src[i]`` to ``dst[i]`` in all layers, all at once: no page may be a destination twice, or source and
         destination.  What ``fork`` and ``compact`` use; the caller of this one answers for whose pages they are."""
-        src, dst = list(src), list(dst)
-        if len(src) != len(dst):
-            raise ValueError("as many sources as destinations are needed")
-        for page in (*src, *dst):
-            if type(page) is not int or not 0 <= page < self.capacity:
-                raise ValueError(f"page {page} of {self.capacity}")
-        self._copy(list(zip(src, dst)))
+        host().copy_pages(self.pages, src, dst)
 
     def _copy(self, pairs) -> None:
-        if not pairs:
-            return
-        numbers = np.array(pairs, dtype=np.int32).T.copy()
-        launches = -(-len(pairs) // 480)
-        check(self._lib.reskv_copy_pages(self.pages.data_ptr(), self.layers, self.capacity, self.pages.stride(1),
-                                         numbers[0].ctypes.data, numbers[1].ctypes.data, len(pairs), _stream(self.device)),
-              launches=launches)
+        if pairs:
+            host().copy_pages(self.pages, *zip(*pairs))
 
     def check(self) -> None:
         """Waits for the device and raises if a kernel met a token or page outside its tables, or a wait that ran out."""
