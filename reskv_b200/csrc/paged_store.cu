@@ -6,6 +6,9 @@
 // eight coordinates of either group each, four rows (K and V of two heads) to a warp; extremes of both groups travel together as
 // 16-bit pairs; a code is the low bits of (x - offset) * (1 / scale) + 1.5 * 2^23, and only where that lies within 1e-5 of a half
 // the division itself decides.  A block first looks up where its tokens go, while their rows are on the way.
+//
+// 8 x 4000 tokens, 8 heads: written in 53 us (168 MB, 3.2 TB/s, half of the copy rate; 150 instructions per token and head), read back
+// in 33 us.  With half a warp to a row and the division always: 91 and 51 us.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -15,8 +18,11 @@
 namespace reskv {
 namespace {
 
-constexpr int kStoreWarps = 8, kStoreThreads = kStoreWarps * 32;
-constexpr int kPairsAtOnce = 4;  // pairs of (token, head) rows of a warp, where there are enough of them
+constexpr int kStoreWarps = 4, kStoreThreads = kStoreWarps * 32;
+// Pairs of (token, head) rows of a warp that are in flight together, where there are enough of them.  8 x 4000 tokens, us written and
+// read, pairs at 4 warps a block: 2 / 2 53.1 and 35.5, 4 / 4 54.8 and 32.9; at 8 warps 4 / 4 59.4 and 33.8, 8 / 8 73.4 and 37.0.
+template <bool WRITE>
+constexpr int kPairsAtOnce = WRITE ? 2 : 4;
 
 struct StoreParams {
     PagedPlace at;
@@ -81,7 +87,8 @@ __device__ __forceinline__ uint32_t codes_of(const uint4& x, float low, float sc
     for (int e = 3; e >= 0; --e) {
         above[e] = add2(make_float2(low_of<BF16>(pairs[e]), high_of<BF16>(pairs[e])), minus_low);
         const float2 quotient = mul2(above[e], inverses), rounded = add2(quotient, up), whole = add2(rounded, down);
-        far = max_nan(far, max_nan(fabsf(quotient.x - whole.x), fabsf(quotient.y - whole.y)));
+        const float2 off = fma2(whole, make_float2(-1.f, -1.f), quotient);
+        far = max3_nan(far, fabsf(off.x), fabsf(off.y));
         word = (word * 16u + __float_as_uint(rounded.y)) * 16u + __float_as_uint(rounded.x);  // the constant part goes below
     }
     word -= 0x4B400000u * 0x11111111u;
@@ -261,8 +268,8 @@ int launch_store(const StoreParams& p, cudaStream_t stream) {
 template <bool WRITE>
 int run_store(const StoreParams& p, int bf16, cudaStream_t stream) {
     const bool many = static_cast<int64_t>(p.total) * p.heads > static_cast<int64_t>(sm_count()) * kStoreWarps * 2;
-    return bf16 ? many ? launch_store<true, WRITE, kPairsAtOnce>(p, stream) : launch_store<true, WRITE, 1>(p, stream)
-                : many ? launch_store<false, WRITE, kPairsAtOnce>(p, stream) : launch_store<false, WRITE, 1>(p, stream);
+    return bf16 ? many ? launch_store<true, WRITE, kPairsAtOnce<WRITE>>(p, stream) : launch_store<true, WRITE, 1>(p, stream)
+                : many ? launch_store<false, WRITE, kPairsAtOnce<WRITE>>(p, stream) : launch_store<false, WRITE, 1>(p, stream);
 }
 
 }  // namespace

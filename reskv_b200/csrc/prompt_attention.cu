@@ -114,12 +114,6 @@ __device__ PromptItem find_item(const PromptParams& p, int index, int lane) {
     return it;
 }
 
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-
 template <bool BF16>
 __device__ __forceinline__ float unpack(unsigned short bits) {
     return BF16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16) : __half2float(__ushort_as_half(bits));
