@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(1024) paged_merge_kernel(const PagedParams p, 
     __shared__ float s_total[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = warp / split, turn = warp - head * split, unit = blockIdx.x;
     // The lengths may be read at once: this kernel starts when every CTA of the first one has seen the end of what came before
-    // (or the table has no width, and they do not count).
+    // (without pages there is no first one, and the lengths count as 0).
     const int sequence = unit / p.heads, kv_head = unit - sequence * p.heads;
     const int64_t row = static_cast<int64_t>(sequence) * p.heads * p.group + kv_head * p.group + head;
     int all = 0, before = 0;
@@ -641,6 +641,7 @@ __global__ void __launch_bounds__(1024) paged_merge_kernel(const PagedParams p, 
 
 // CTAs of the first kernel for as many pages as there may be.
 int paged_ctas(int sequences, int width, int heads) {
+    if (width == 0) return 0;
     const int64_t most = (static_cast<int64_t>(sequences) * (width + kPaCharge) * heads + kPaLeast - 1) / kPaLeast, room = kPaPerSm * sm_count();
     return static_cast<int>(most < room ? most : room);
 }

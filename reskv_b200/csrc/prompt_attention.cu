@@ -73,6 +73,7 @@ __device__ __forceinline__ SequenceSpan span_of(const PromptParams& p, int s) {
 __device__ __forceinline__ int pairs_from(const PromptParams& p, int level, int lane) {
     const int pair = 2 * p.tile_tokens;
     int n = 0;
+#pragma unroll 4
     for (int s = lane; s < p.sequences; s += 32) {
         const int tiles = (span_of(p, s).len + pair - 1) / pair;
         n += tiles > level ? tiles - level : 0;
@@ -80,39 +81,49 @@ __device__ __forceinline__ int pairs_from(const PromptParams& p, int level, int 
     return __reduce_add_sync(0xffffffffu, n);
 }
 
-// Item `index`, items ordered by their place in their sequence, last ones first: with causal attention the longest ones.
-// tiles0 = 0 in the result: there is none.  Whole warp.
-__device__ PromptItem find_item(const PromptParams& p, int index, int lane) {
-    PromptItem it{};
-    const int pos = index / p.kv_heads, pair = 2 * p.tile_tokens;
-    int low = 0, high = (p.total + pair - 1) / pair;
-    if (pairs_from(p, 0, lane) <= pos) return it;
-    while (high - low > 1) {
-        const int mid = (low + high) >> 1;
-        if (pairs_from(p, mid, lane) > pos) low = mid; else high = mid;
-    }
-    int rest = pos - pairs_from(p, low + 1, lane);
-    for (int s0 = 0; s0 < p.sequences; s0 += 32) {
-        const SequenceSpan sp = s0 + lane < p.sequences ? span_of(p, s0 + lane) : SequenceSpan{0, 0};
-        const bool has = sp.len > low * pair;
-        const uint32_t mask = __ballot_sync(0xffffffffu, has);
-        const int count = __popc(mask);
-        if (rest >= count) {
-            rest -= count;
-            continue;
+// Items are ordered by their place in their sequence, last ones first: with causal attention the longest ones.  The items that a CTA
+// takes come as a rule in this order, so the search for one begins at the level of the one before.
+struct ItemSearch {
+    int all, level, before, upto;  // all pairs; the level's are those from `before` to `upto`
+    __device__ __forceinline__ ItemSearch(const PromptParams& p, int lane) : all(pairs_from(p, 0, lane)), level(highest(p)), before(0), upto(0) {}
+    static __device__ __forceinline__ int highest(const PromptParams& p) { return (p.total + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens); }
+    // Item `index`.  tiles0 = 0 in the result: there is none.  Whole warp.
+    __device__ PromptItem find(const PromptParams& p, int index, int lane) {
+        PromptItem it{};
+        const int pos = index / p.kv_heads, pair = 2 * p.tile_tokens;
+        if (pos >= all) return it;
+        if (pos < before) level = highest(p), before = upto = 0;
+        if (pos >= upto) {
+            int low = 0, high = level, from_high = upto, from_low = all;
+            while (high - low > 1) {
+                const int mid = (low + high) >> 1, n = pairs_from(p, mid, lane);
+                if (n > pos) low = mid, from_low = n; else high = mid, from_high = n;
+            }
+            level = low, before = from_high, upto = from_low;
         }
-        const int owner = __ffs(__ballot_sync(0xffffffffu, has && __popc(mask & ((1u << lane) - 1u)) == rest)) - 1;
-        it.start = __shfl_sync(0xffffffffu, sp.start, owner);
-        it.len = __shfl_sync(0xffffffffu, sp.len, owner);
-        it.head = index % p.kv_heads;
-        it.token0 = low * pair;
-        const int end0 = min(it.token0 + p.tile_tokens, it.len), end1 = min(it.token0 + pair, it.len);
-        it.tiles0 = ((p.causal ? end0 : it.len) + kPKeys - 1) / kPKeys;
-        it.tiles1 = end1 <= it.token0 + p.tile_tokens ? 0 : ((p.causal ? end1 : it.len) + kPKeys - 1) / kPKeys;
+        int rest = pos - before;
+        for (int s0 = 0; s0 < p.sequences; s0 += 32) {
+            const SequenceSpan sp = s0 + lane < p.sequences ? span_of(p, s0 + lane) : SequenceSpan{0, 0};
+            const bool has = sp.len > level * pair;
+            const uint32_t mask = __ballot_sync(0xffffffffu, has);
+            const int count = __popc(mask);
+            if (rest >= count) {
+                rest -= count;
+                continue;
+            }
+            const int owner = __ffs(__ballot_sync(0xffffffffu, has && __popc(mask & ((1u << lane) - 1u)) == rest)) - 1;
+            it.start = __shfl_sync(0xffffffffu, sp.start, owner);
+            it.len = __shfl_sync(0xffffffffu, sp.len, owner);
+            it.head = index % p.kv_heads;
+            it.token0 = level * pair;
+            const int end0 = min(it.token0 + p.tile_tokens, it.len), end1 = min(it.token0 + pair, it.len);
+            it.tiles0 = ((p.causal ? end0 : it.len) + kPKeys - 1) / kPKeys;
+            it.tiles1 = end1 <= it.token0 + p.tile_tokens ? 0 : ((p.causal ? end1 : it.len) + kPKeys - 1) / kPKeys;
+            return it;
+        }
         return it;
     }
-    return it;
-}
+};
 
 template <bool BF16>
 __device__ __forceinline__ float unpack(unsigned short bits) {
@@ -220,9 +231,10 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
             // ---- copies, and the next item: the grid has a CTA for every item that there may be, and a CTA that has finished takes
             // over one that has not started yet -------------------------------------------------------------------------------
             int index = blockIdx.x, tile = 0, queries = 0;  // queries: items whose rows have been asked for
+            ItemSearch search(p, lane);
             for (int n = 0;; ++n) {
                 const int slot = n & 1;
-                const PromptItem it = find_item(p, index, lane);
+                const PromptItem it = search.find(p, index, lane);
                 if (n >= 2) wait_once(lost, &sh.item_empty[slot], ((n >> 1) - 1) & 1);
                 if (lane == 0) {
                     sh.item[slot] = it;

@@ -446,3 +446,58 @@ def test_refusals():
     cache.fork([seqs[0]])
     with pytest.raises(ValueError):
         cache.write(0, step, x[:2], x[:2])
+
+
+@pytest.mark.gpu
+def test_attention_on_two_streams_at_once():
+    """Every call has scratch of its own: calls that overlap give the bits of calls in turn."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    cache = PagedInt4Cache(1, 2, 200)
+    seqs, _, _ = fill(cache, [3000, 20, 1500, 64], seed=31)
+    steps = [cache.extend(seqs[:2], 0), cache.extend(seqs[2:], 0)]
+    queries = [torch.randn(2, 8, 128, device=DEV).half() for _ in range(2)]
+    want = [cache.attend(0, s, q) for s, q in zip(steps, queries)]
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [cache.attend(0, steps[i], queries[i]) for _ in range(50)]
+        torch.cuda.synchronize()
+        return all(torch.equal(g, want[i]) for g in got)
+
+    with ThreadPoolExecutor(2) as pool:
+        assert list(pool.map(work, (0, 1))) == [True, True]
+
+
+@pytest.mark.gpu
+def test_steps_without_sequences_or_tokens():
+    cache = PagedInt4Cache(1, 2, 2)
+    none = cache.extend([], [])
+    empty = torch.zeros(0, 2, 128, dtype=torch.float16, device=DEV)
+    cache.write(0, none, empty, empty)
+    assert cache.attend(0, none, torch.zeros(0, 4, 128, dtype=torch.float16, device=DEV)).shape == (0, 4, 128)
+    assert cache.read(0, none, everything=True)[0].shape == (0, 2, 128)
+    step = cache.extend(cache.add(2), 0)  # sequences that have no tokens: no pages
+    out, lse = cache.attend(0, step, torch.ones(2, 4, 128, dtype=torch.float16, device=DEV), return_lse=True)
+    assert not out.any() and (lse == -torch.inf).all()
+    assert cache.fork([]) == [] and cache.compact() == 0
+    cache.free([])
+
+
+@pytest.mark.gpu
+def test_long_sequences_and_a_pool_beyond_four_gigabytes():
+    """Byte offsets that pass 32 bits."""
+    cache = PagedInt4Cache(1, 8, 62000)  # 4.57 GB
+    filler, target = cache.add(2)
+    cache.extend([filler], 61000 * 64)
+    seqs = [target]
+    k, v = vectors(40000, 8, torch.float16, 41), vectors(40000, 8, torch.float16, 42)
+    step = cache.extend(seqs, 40000)
+    assert min(cache._book.of(target).pages) * 8 * 9216 > 2**32
+    cache.write(0, step, k, v)
+    got = cache.read(0, step)
+    assert torch.equal(got[0], values_of(k)) and torch.equal(got[1], values_of(v))
+    assert_attends(cache, seqs, [k], [v], 2)
+    cache.copy_pages([cache._book.of(target).pages[0]], [0])
+    assert torch.equal(cache.pages[0, 0], cache.pages[0, cache._book.of(target).pages[0]])

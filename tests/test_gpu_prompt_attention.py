@@ -240,3 +240,31 @@ def test_the_library_refuses_bad_arguments_before_any_launch():
     assert call(step=129) == ERR_INVALID and call(q=x.ctypes.data + 2) == ERR_INVALID
     assert call() == ERR_INVALID and b"prompt_attention: q" in lib.reskv_last_error()  # host memory
     assert call(total=0) == 0 and call(sequences=0) == 0
+
+
+@pytest.mark.gpu
+def test_a_thousand_sequences():
+    """More sequences than a warp looks at at once, of very different lengths."""
+    lengths = [(i * 7919) % 61 for i in range(1000)] + [700, 1, 333]
+    q, k, v, ends, cu = inputs(lengths, 1, 2, torch.bfloat16, seed=11)
+    assert_within(prompt_attention(q, k, v, cu), *formula(q, k, v, ends)[::2])
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once():
+    """Calls of two threads on two streams give the bits of calls in turn."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    cases = [inputs(lengths, 2, 4, torch.float16, seed=i) for i, lengths in enumerate(([500, 40], [1, 2, 1200]))]
+    want = [prompt_attention(q, k, v, cu) for q, k, v, _, cu in cases]
+    torch.cuda.synchronize()
+
+    def work(i):
+        q, k, v, _, cu = cases[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [prompt_attention(q, k, v, cu) for _ in range(20)]
+        torch.cuda.synchronize()
+        return all(torch.equal(g, want[i]) for g in got)
+
+    with ThreadPoolExecutor(2) as pool:
+        assert list(pool.map(work, (0, 1))) == [True, True]
