@@ -28,17 +28,22 @@
 namespace reskv {
 namespace {
 
-constexpr int kPKeys = 128;                     // keys of a tile
-constexpr int kPHalf = 128 * 128;               // bytes of 128 rows x 64 coordinates
-constexpr int kPTile = 2 * kPHalf;              // 128 rows of 128 coordinates
-constexpr int kPStages = 5;                     // ring of K and V tiles
-constexpr int kPThreads = 384;                  // two softmax warpgroups; MMA warp, copying warp and two that idle
+constexpr int kPKeys = 80;                      // keys of a tile
+constexpr int kPChunks = kPKeys / 16;           // of a row of scores
+constexpr int kPQHalf = 128 * 128, kPQTile = 2 * kPQHalf;        // bytes of 128 rows x 64 coordinates, and of all coordinates
+constexpr int kPKHalf = kPKeys * 128, kPKTile = 2 * kPKHalf;     // the same of a tile of keys or values
+constexpr int kPStages = 8;                     // ring of K and V tiles
+constexpr int kPThreads = 384;                  // two softmax warpgroups; a warp each for scores, outputs and copies, one idle
 // A row of scores is 128 registers of its thread.  The launch gives 168 a thread (the most for 384); the last warpgroup hands
 // back what the softmax warpgroups take: 2 x 208 + 88 = 3 x 168.
 constexpr int kPLaunchRegs = 168, kPSoftmaxRegs = 208, kPOtherRegs = 88;
 static_assert(2 * kPSoftmaxRegs + kPOtherRegs <= 3 * kPLaunchRegs, "the shares come out of the launch's registers");
-constexpr int kPSmem = 2 * kPTile + kPStages * kPTile + 1024;  // + room to start on a 1024-byte boundary
-constexpr uint32_t kPColS = 0, kPColO = 256;    // tensor memory: scores 2 x 128 columns, outputs 2 x 128
+constexpr int kPSmem = 2 * kPQTile + kPStages * kPKTile + 1024;  // + room to start on a 1024-byte boundary
+// Tensor memory, columns of the two row tiles: scores (80), weights (40, two to a column), outputs (128).
+__host__ __device__ constexpr uint32_t score_column(int i) { return i * 128; }
+__host__ __device__ constexpr uint32_t weight_column(int i) { return i * 128 + kPKeys; }
+__host__ __device__ constexpr uint32_t output_column(int i) { return 256 + i * 128; }
+static_assert(kPKeys + kPKeys / 2 <= 128 && kPKeys % 16 == 0, "scores and weights of a row tile share 128 columns");
 constexpr float kPSlack = 8.f;                  // the running maximum lags by at most this (in powers of two)
 
 __device__ uint32_t g_prompt_status;  // RESKV_STATUS_* bits
@@ -147,7 +152,7 @@ __device__ __forceinline__ bool tame_value_row(unsigned char* row, bool drop, in
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            uint4* at = reinterpret_cast<uint4*>(row + h * kPHalf + (((i + lane) & 7) << 4));
+            uint4* at = reinterpret_cast<uint4*>(row + h * kPKHalf + (((i + lane) & 7) << 4));
             if (drop) {
                 *at = make_uint4(0, 0, 0, 0);
             } else {
@@ -159,7 +164,7 @@ __device__ __forceinline__ bool tame_value_row(unsigned char* row, bool drop, in
     if (drop || !(seen & 0x80008000u)) return false;
     for (int h = 0; h < 2; ++h)
         for (int i = 0; i < 64; ++i) {
-            unsigned short* at = reinterpret_cast<unsigned short*>(row + h * kPHalf) + i;
+            unsigned short* at = reinterpret_cast<unsigned short*>(row + h * kPKHalf) + i;
             if (non_finite<BF16>(*at)) *at = 0;
         }
     return true;
@@ -167,7 +172,7 @@ __device__ __forceinline__ bool tame_value_row(unsigned char* row, bool drop, in
 
 struct __align__(16) PromptShared {
     uint64_t kv_full[kPStages], kv_empty[kPStages];
-    uint64_t q_full, q_empty, s_full[2], p_ready[2][2], o_done[2], item_full[2], item_empty[2], cancel;
+    uint64_t q_full, q_empty, s_full[2], s_empty[2], p_full[2], p_empty[2], item_full[2], item_empty[2], cancel;
     uint4 cancel_reply;
     PromptItem item[2];
     int tamed[2];   // of an item: infinities or NaN were cleared in a tile of values
@@ -194,6 +199,45 @@ __device__ __forceinline__ void store32(void* to, const uint32_t (&v)[8]) {
                  : "memory");
 }
 
+// A product takes its descriptors from uniform registers; what they depend on is kept uniform in the compiler's eyes too, or each
+// costs moves that take longer than the product.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_or_sync(0xffffffffu, x); }
+
+// The loop of a warp that issues products: items, key tiles, row tiles.  `first`: place of the first tile of keys (0) or of values
+// (1) in the ring.  begin(n) before item n, product(i, j, stage, issues) for row tile i and key tile j, end(issues) behind an item;
+// the commands themselves are for the one lane for which `issues` holds.
+template <class Begin, class Product, class End>
+__device__ __forceinline__ void for_key_tiles(PromptShared& sh, bool& lost, int lane, uint32_t first, Begin begin, Product product, End end) {
+    const bool issues = elect_one();
+    uint32_t stage = first, parity = 0, last_stage = 0, last_parity = 0;
+    int n = 0;
+    for (;; ++n) {
+        const int slot = n & 1;
+        if (!item_posted(&sh.item_full[slot], (n >> 1) & 1)) lost = true;
+        const int tiles0 = static_cast<int>(uniform(sh.item[slot].tiles0)), tiles1 = static_cast<int>(uniform(sh.item[slot].tiles1));
+        if (lane == 0) mbar_arrive(&sh.item_empty[slot]);
+        if (tiles0 == 0 || __any_sync(0xffffffffu, lost)) break;
+        const int kv_tiles = max(tiles0, tiles1);
+        begin(n);
+        for (int j = 0; j < kv_tiles; ++j) {
+            wait_once(lost, &sh.kv_full[stage], parity);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (j < (i ? tiles1 : tiles0)) product(i, j, stage, issues);
+                __syncwarp();
+            }
+            if (issues) umma_commit(&sh.kv_empty[stage]);
+            __syncwarp();
+            last_stage = stage, last_parity = parity;
+            stage += 2;
+            if (stage >= kPStages) stage -= kPStages, parity ^= 1;
+        }
+        end(issues);
+        __syncwarp();
+    }
+    if (n > 0) wait_once(lost, &sh.kv_empty[last_stage], last_parity);  // the last commits have arrived before the block ends
+}
+
 template <bool BF16>
 __global__ void __launch_bounds__(kPThreads, 1)
 prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
@@ -202,16 +246,16 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
     __shared__ PromptShared sh;
     unsigned char* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     unsigned char* qs = smem;                 // two row tiles
-    unsigned char* ring = smem + 2 * kPTile;  // K0 V0 K1 V1 ...
+    unsigned char* ring = smem + 2 * kPQTile;  // K0 V0 K1 V1 ...
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rows = p.tile_tokens * p.group;
     if (tid == 0) {
         for (int s = 0; s < kPStages; ++s) mbar_init(&sh.kv_full[s], 1), mbar_init(&sh.kv_empty[s], 1);
         mbar_init(&sh.q_full, 1), mbar_init(&sh.q_empty, 1), mbar_init(&sh.cancel, 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.s_full[i], 1), mbar_init(&sh.o_done[i], 1);
-            mbar_init(&sh.p_ready[i][0], 4), mbar_init(&sh.p_ready[i][1], 4);  // a warp each
-            mbar_init(&sh.item_full[i], 1), mbar_init(&sh.item_empty[i], 9);  // softmax warps, MMA warp
+            mbar_init(&sh.s_full[i], 1), mbar_init(&sh.p_empty[i], 1);    // products
+            mbar_init(&sh.s_empty[i], 4), mbar_init(&sh.p_full[i], 4);    // softmax warps of a row tile
+            mbar_init(&sh.item_full[i], 1), mbar_init(&sh.item_empty[i], 10);  // softmax warps, the warps of the products
         }
         mbar_fence_init();
     }
@@ -256,9 +300,9 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                     if (tile >= kPStages) wait_once(lost, &sh.kv_empty[stage], (tile / kPStages - 1) & 1);
                     if (lost) break;
                     if (lane == 0) {
-                        mbar_arrive_expect_tx(&sh.kv_full[stage], kPTile);
+                        mbar_arrive_expect_tx(&sh.kv_full[stage], kPKTile);
                         for (int h = 0; h < 2; ++h)
-                            tma_load_3d(ring + stage * kPTile + h * kPHalf, j & 1 ? &v_map : &k_map, 64 * h, it.head,
+                            tma_load_3d(ring + stage * kPKTile + h * kPKHalf, j & 1 ? &v_map : &k_map, 64 * h, it.head,
                                         it.start + (j >> 1) * kPKeys, &sh.kv_full[stage]);
                     }
                     __syncwarp();
@@ -274,7 +318,7 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                         mbar_arrive_expect_tx(&sh.q_full, row_tiles * rows * 256);
                         for (int i = 0; i < row_tiles; ++i)
                             for (int h = 0; h < 2; ++h)
-                                tma_load_3d(qs + i * kPTile + h * kPHalf, &q_map, 64 * h, it.head * p.group,
+                                tma_load_3d(qs + i * kPQTile + h * kPQHalf, &q_map, 64 * h, it.head * p.group,
                                             it.start + it.token0 + i * p.tile_tokens, &sh.q_full);
                     }
                     __syncwarp();
@@ -299,109 +343,66 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                 if (queries > 0) mbar_wait(&sh.q_full, (queries - 1) & 1);
             }
         } else if (warp == 8) {
-            // ---- MMAs: per key tile and row tile scores = Q K^T, output += P V; the scores of the next key tile follow the output
-            // in turn, so a row tile's softmax runs beside the other's products -----------------------------------------------
-            // This warp's instructions are close to what bounds it.  A product takes its descriptors from uniform registers; what they
-            // depend on is therefore kept uniform in the compiler's eyes too (reductions over the warp), or each costs moves that take
-            // longer than the product.
-            constexpr uint32_t kFull = 0xffffffffu;
-            constexpr uint32_t score_idesc = umma_idesc(128, false, false, BF16), value_idesc = umma_idesc(128, false, true, BF16);
+            // ---- scores, for both row tiles, as soon as those in front have been read -------------------------------------------
+            constexpr uint32_t idesc = umma_idesc(kPKeys, false, false, BF16);
             const UmmaDesc q0 = umma_desc_halves(smem_u32(qs), 16, 1024), k0 = umma_desc_halves(smem_u32(ring), 16, 1024);
-            const UmmaDesc v0 = umma_desc_halves(smem_u32(ring), kPHalf, 1024);
-            const uint32_t columns = __reduce_or_sync(kFull, tmem);
-            const bool issues = elect_one();
-            uint32_t stage = 0, parity = 0, made[2] = {0, 0};  // stage: of the next tile in the ring
-            const auto step = [&] {
-                if (++stage == kPStages) stage = 0, parity ^= 1;
-            };
-            const auto scores = [&](int i, uint32_t at_stage) {
-                const uint32_t d = columns + kPColS + i * 128, q = q0.low + ((i * kPTile) >> 4), k = k0.low + at_stage * (kPTile >> 4);
-                if (issues) {
-                    umma_f16<false>(d, q, k, k0.high, score_idesc);
+            const uint32_t columns = uniform(tmem);
+            uint32_t made[2] = {0, 0};
+            for_key_tiles(
+                sh, lost, lane, 0,
+                [&](int n) { wait_once(lost, &sh.q_full, n & 1); },
+                [&](int i, int, uint32_t stage, bool issues) {
+                    if (made[i] > 0) wait_once(lost, &sh.s_empty[i], (made[i] - 1) & 1);
+                    ++made[i];
+                    tc_fence_after();
+                    const uint32_t d = columns + score_column(i), q = q0.low + ((i * kPQTile) >> 4), k = k0.low + stage * (kPKTile >> 4);
+                    if (issues) {
+                        umma_f16<false>(d, q, k, k0.high, idesc);
 #pragma unroll
-                    for (int ks = 1; ks < 8; ++ks) {
-                        const uint32_t at = ((ks >> 2) * kPHalf + (ks & 3) * 32) >> 4;
-                        umma_f16<true>(d, q + at, k + at, k0.high, score_idesc);
+                        for (int ks = 1; ks < 8; ++ks)
+                            umma_f16<true>(d, q + (((ks >> 2) * kPQHalf + (ks & 3) * 32) >> 4), k + (((ks >> 2) * kPKHalf + (ks & 3) * 32) >> 4), k0.high, idesc);
+                        umma_commit(&sh.s_full[i]);
                     }
-                    umma_commit(&sh.s_full[i]);
-                }
-                __syncwarp();
-            };
-            const auto values = [&](int i, uint32_t at_stage, int half, uint32_t accumulate) {
-                const uint32_t d = columns + kPColO + i * 128, a = columns + kPColS + i * 128 + half * 32;
-                const uint32_t v = v0.low + at_stage * (kPTile >> 4) + half * (4 * 2048 >> 4);
-                if (issues) {
-                    umma_f16_ta(d, a, v, v0.high, value_idesc, accumulate);
+                },
+                [&](bool issues) {
+                    if (issues) umma_commit(&sh.q_empty);
+                });
+        } else if (warp == 10) {
+            // ---- outputs, as soon as weights are there ----------------------------------------------------------------------------
+            constexpr uint32_t idesc = umma_idesc(128, false, true, BF16);
+            const UmmaDesc v0 = umma_desc_halves(smem_u32(ring), kPKHalf, 1024);
+            const uint32_t columns = uniform(tmem);
+            uint32_t made[2] = {0, 0};
+            for_key_tiles(
+                sh, lost, lane, 1, [](int) {},
+                [&](int i, int j, uint32_t stage, bool issues) {
+                    wait_once(lost, &sh.p_full[i], made[i] & 1);
+                    ++made[i];
+                    tc_fence_after();
+                    const uint32_t d = columns + output_column(i), a = columns + weight_column(i), v = v0.low + stage * (kPKTile >> 4);
+                    if (issues) {
+                        umma_f16_ta(d, a, v, v0.high, idesc, j > 0);
 #pragma unroll
-                    for (int ks = 1; ks < 4; ++ks) umma_f16_ta(d, a + ks * 8, v + ks * (2048 >> 4), v0.high, value_idesc, 1);
-                }
-                __syncwarp();
-            };
-            const auto commit = [&](uint64_t* bar) {
-                if (issues) umma_commit(bar);
-                __syncwarp();
-            };
-            int n = 0;
-            for (;; ++n) {
-                const int slot = n & 1;
-                if (!item_posted(&sh.item_full[slot], (n >> 1) & 1)) lost = true;
-                const int tiles0 = __reduce_max_sync(kFull, sh.item[slot].tiles0), tiles1 = __reduce_max_sync(kFull, sh.item[slot].tiles1);
-                if (lane == 0) mbar_arrive(&sh.item_empty[slot]);
-                if (tiles0 == 0 || __any_sync(kFull, lost)) break;
-                const int kv_tiles = max(tiles0, tiles1);
-                wait_once(lost, &sh.q_full, n & 1);
-                wait_once(lost, &sh.kv_full[stage], parity);
-                tc_fence_after();
-                scores(0, stage);
-                if (tiles1) scores(1, stage);
-                commit(&sh.kv_empty[stage]);
-                if (kv_tiles == 1) commit(&sh.q_empty);
-                step();
-                for (int j = 0; j < kv_tiles; ++j) {
-                    const uint32_t v_stage = stage;
-                    const bool more = j + 1 < kv_tiles;
-                    wait_once(lost, &sh.kv_full[v_stage], parity);
-                    step();
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int tiles = i ? tiles1 : tiles0;
-                        if (j < tiles) {
-#pragma unroll
-                            for (int half = 0; half < 2; ++half) {
-                                wait_once(lost, &sh.p_ready[i][half], made[i] & 1);
-                                tc_fence_after();
-                                values(i, v_stage, half, half > 0 || j > 0);
-                            }
-                            ++made[i];
-                        }
-                        // every stage goes back as soon as its last product has run, and the keys are waited for when they are
-                        // needed: a copy then has more than an iteration's time
-                        if (i == 1) commit(&sh.kv_empty[v_stage]);
-                        if (i == 0 && more) wait_once(lost, &sh.kv_full[stage], parity);
-                        if (j < tiles) {
-                            if (j + 1 < tiles) scores(i, stage); else commit(&sh.o_done[i]);
-                        }
+                        for (int ks = 1; ks < kPChunks; ++ks) umma_f16_ta(d, a + ks * 8, v + ks * (2048 >> 4), v0.high, idesc, 1);
+                        umma_commit(&sh.p_empty[i]);
                     }
-                    if (more) {
-                        commit(&sh.kv_empty[stage]);
-                        step();
-                    }
-                    if (j + 2 == kv_tiles) commit(&sh.q_empty);
-                }
-            }
-            // the last commits have arrived before the block ends
-            const uint32_t last = stage ? stage - 1 : kPStages - 1;
-            if (n > 0) wait_once(lost, &sh.kv_empty[last], stage ? parity : parity ^ 1);
+                },
+                [](bool) {});
         }
     } else {
         // ---- softmax and output: thread = row -----------------------------------------------------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPSoftmaxRegs));
         const int i = warp >> 2, row = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + lanes + kPColS + i * 128, o_at = tmem + lanes + kPColO + i * 128;
+        const uint32_t s_at = tmem + lanes + score_column(i), p_at = tmem + lanes + weight_column(i), o_at = tmem + lanes + output_column(i);
         const int row_token = row / p.group, row_head = row - row_token * p.group;
         const float scale = p.scale_log2, slack = kPSlack / scale;
-        uint32_t seen = 0, items = 0;
+        const auto arrive = [&](uint64_t* bar) {  // of the warp, behind its reads and writes of tensor memory
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        uint32_t seen = 0;
         int tile = 0;
         for (int n = 0;; ++n) {
             const int slot = n & 1;
@@ -415,33 +416,37 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
             float m = 0.f, l = 0.f;
             for (int j = 0; j < tiles; ++j) {
                 wait_once(lost, &sh.s_full[i], seen & 1);
-                ++seen;
                 tc_fence_after();
-                float s[4][32];
+                float s[kPChunks][16];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(s_at + c * 32, s[c]);
+                for (int c = 0; c < kPChunks; ++c) tmem_ld16(s_at + c * 16, s[c]);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld_wait(s[c]);
+                for (int c = 0; c < kPChunks; ++c) tmem_ld_wait(s[c]);
+                arrive(&sh.s_empty[i]);  // the next scores may come
                 const bool masked = j * kPKeys + kPKeys > it.len || (p.causal && j * kPKeys + kPKeys - 1 > first_token);
                 if (masked) {
                     const int last = limit - j * kPKeys;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < kPChunks; ++c)
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) s[c][e] = c * 32 + e <= last ? s[c][e] : -INFINITY;
+                        for (int e = 0; e < 16; ++e) s[c][e] = c * 16 + e <= last ? s[c][e] : -INFINITY;
                 }
-                float top[4];
+                float top[kPChunks];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < kPChunks; ++c) {
                     top[c] = max_nan(s[c][0], s[c][1]);
 #pragma unroll
-                    for (int e = 2; e < 32; e += 2) top[c] = max3_nan(top[c], s[c][e], s[c][e + 1]);
+                    for (int e = 2; e < 16; e += 2) top[c] = max3_nan(top[c], s[c][e], s[c][e + 1]);
                 }
-                const float most = max3_nan(max_nan(top[0], top[1]), top[2], top[3]);
+                const float most = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[4]);
+                if (j > 0) {  // the product in front has read its weights, and the output is at rest
+                    wait_once(lost, &sh.p_empty[i], (seen - 1) & 1);
+                    tc_fence_after();
+                }
+                ++seen;
                 if (j == 0) {
                     m = most;
                 } else {
-                    // the output so far is at rest: the scores at hand were committed behind the last product
                     const bool grows = !(most <= m + slack);
                     if (__any_sync(0xffffffffu, grows)) {
                         const float next = grows ? max_nan(m, most) : m, factor = grows ? fast_exp2((m - next) * scale) : 1.f;
@@ -461,39 +466,32 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                 const float shift = m == INFINITY ? __int_as_float(0x7fffffff) : -m * scale;
                 const float2 scales = make_float2(scale, scale), shifts = make_float2(shift, shift);
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                const auto weights = [&](int c) {  // of 32 keys
-                    float packed[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
+                for (int c = 0; c < kPChunks; ++c) {
+                    float packed[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
                         const float2 x = fma2(make_float2(s[c][2 * e], s[c][2 * e + 1]), scales, shifts);
                         const float2 y = make_float2(fast_exp2(x.x), fast_exp2(x.y));
                         sum[e & 1] = add2(sum[e & 1], y);
                         packed[e] = __uint_as_float(pack2<BF16>(y.x, y.y));
                     }
-                    tmem_st16(s_at + c * 16, packed);
-                };
-                const auto hand_over = [&](int half) {
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.p_ready[i][half]);
-                };
-                weights(0), weights(1);
-                if (masked && (i == 0 || j >= other)) {
+                    tmem_st8(p_at + c * 8, packed);
+                }
+                if (masked && (i == 0 || j >= other) && row < kPKeys) {
                     const int vt = tile + 2 * j + 1, stage = vt % kPStages;
                     wait_once(lost, &sh.kv_full[stage], (vt / kPStages) & 1);
                     const bool behind = j * kPKeys + row >= it.len;
-                    if ((behind || p.causal) && tame_value_row<BF16>(ring + stage * kPTile + row * 128, behind, lane)) sh.tamed[slot] = 1;
+                    if ((behind || p.causal) && tame_value_row<BF16>(ring + stage * kPKTile + row * 128, behind, lane)) sh.tamed[slot] = 1;
                     proxy_fence();
                 }
-                hand_over(0);
-                weights(2), weights(3);
-                hand_over(1);
+                __syncwarp();
+                tmem_st_wait();
+                arrive(&sh.p_full[i]);
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
             if (tiles) {
-                wait_once(lost, &sh.o_done[i], items & 1);
-                ++items;
+                wait_once(lost, &sh.p_empty[i], (seen - 1) & 1);
                 tc_fence_after();
                 const bool live = row < rows && token < it.len && !lost;
                 const bool tamed = *static_cast<volatile int*>(&sh.tamed[slot]) != 0;
