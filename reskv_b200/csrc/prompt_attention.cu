@@ -2,10 +2,12 @@
 // head, out_i = sum_j softmax_j(q_i . k_j * scaling) v_j over the keys j <= i (causal) or over all keys of the sequence.
 //
 // Both products run on tcgen05.mma.  A row tile is 128 rows: the query heads of one KV head for as many tokens as fit, so that
-// grouped heads share the keys and a short sequence still fills rows; an item is two row tiles.  Per tile of 128 keys: scores
-// S = Q K^T into tensor memory, one thread per row forms the weights with a running maximum (it lags by up to 2^8, so that the
-// output is rarely rescaled) and puts them in the scores' place, and the output accumulates P V with P read from tensor memory.
-// While one row tile's threads work the other's products run.  Tiles arrive by TMA through a ring of five.
+// grouped heads share the keys and a short sequence still fills rows; an item is two row tiles.  Per tile of 80 keys: scores
+// S = Q K^T into tensor memory, one thread per row forms the weights P with a running maximum (it lags by up to 2^8, so that the
+// output is rarely rescaled), and the output accumulates P V with P read from tensor memory.  A row tile's scores (80 columns)
+// and weights (40) lie side by side in 128 columns, which is why a tile has 80 keys: the next scores do not wait for the product
+// with the weights in front.  A warp issues the scores' products, another one the outputs', so neither waits for the other's
+// operands.  Tiles arrive by TMA through a ring of eight.
 //
 // Items are ordered by their place in their sequence, last ones first, which with causal attention are the longest; the grid has
 // a CTA for every item that there may be, and a CTA that has finished takes over one that has not started (cluster launch
@@ -14,12 +16,17 @@
 // What is masked counts for nothing: masked scores are replaced, rows of V behind the sequence are cleared in shared memory, and
 // infinities or NaN in rows of V that only part of a row tile sees are cleared there too and added where they are seen.
 //
-// Bound (1 x 8192 tokens, 32 / 8 heads, 550 GFLOP): 463 us = 1.19 PFLOP/s in short runs, 520 us in long ones under the power cap.
-// An iteration of two row tiles takes 3100 cycles where its products need 2048: 1900 of a row tile's chain are its softmax (16
-// exponentials per clock and SM are 1024 of them), the rest the products and four hand-overs.  Exponentials by a polynomial for a
-// quarter to a half of the weights: no faster.  Two threads per row (16 softmax warps): 502 us.  What the MMA warp's descriptors
-// depend on has to be uniform for the compiler: 550 -> 463 us; its loop in one thread: 512 us.  Outputs stored by row, 16 bytes a
-// lane, instead of by lines: seven ragged prompts 106 -> 100 us.
+// Bound (1 x 8192 tokens, 32 / 8 heads, 550 GFLOP): 449 us = 1.22 PFLOP/s in short runs, 507 us = 1.08 PFLOP/s in long ones under
+// the power cap; seven ragged prompts of 84 GFLOP 93 us, five short ones of 0.9 GFLOP 14.5 us.  A row tile's softmax is what
+// takes longest: 2070 cycles per tile of 80 keys, of them 1230 forming weights (16 exponentials per clock and SM, two row tiles: 1280
+// for both), 180 and 280 waiting for scores and for the product in front, 150 the maximum; per item another 1300 waiting for the
+// last product, 2300 storing, 1000 until the first scores.  What was measured besides, on 1 x 8192 in short runs:
+//   128 keys a tile, weights in the scores' place, one warp for both products, ring of five: 463 us (seven ragged: 100 us)
+//   a quarter of the exponentials by a polynomial: 447 us, not worth its code; a half: no faster
+//   two threads per row (16 softmax warps): 502 us
+//   the wait for the product in front behind all exponentials: 490 us; one lane polling for its warp: 490 us
+//   descriptors that the compiler does not see as uniform: 550 us for 463; the products issued from a loop in one thread: 512 us
+//   outputs stored by row, 16 bytes a lane, instead of by lines: seven ragged prompts 106 us for 100
 #include "pairs.cuh"
 #include "tensor_map.cuh"
 #include "tmem.cuh"
