@@ -2,13 +2,14 @@
 //
 // Storing: of a token's vector of one head, every group of 64 coordinates becomes offset = min, scale = (max - min) / 15
 // rounded to the model's type, code = round((x - offset) / scale) to the nearest, ties to even, at most 15 (0 where the scale
-// is 0).  512 bytes of K and V become 144.  Bound by bytes, and close to that by instructions.  Eight lanes hold a row of one side,
-// eight coordinates of either group each, four rows (K and V of two heads) to a warp; extremes of both groups travel together as
-// 16-bit pairs; a code is the low bits of (x - offset) * (1 / scale) + 1.5 * 2^23, and only where that lies within 1e-5 of a half
-// the division itself decides.  A block first looks up where its tokens go, while their rows are on the way.
+// is 0).  512 bytes of K and V become 144.  Bound by bytes, and close to that by instructions.  Four lanes hold a row of one side,
+// sixteen coordinates of either group each, eight rows (K and V of four heads) to a warp; a lane's words of a key row are then 16
+// bytes in a row of their own.  Extremes of both groups travel together as 16-bit pairs.  A warp looks up by itself where its tokens
+// go, while their rows are on the way.
 //
-// 8 x 4000 tokens, 8 heads: written in 53 us (168 MB, 3.2 TB/s, half of the copy rate; 150 instructions per token and head), read back
-// in 33 us.  With half a warp to a row and the division always: 91 and 51 us.
+// 8 x 4000 tokens, 8 heads: written in 36 us (168 MB, 4.6 TB/s, 0.72 of the copy rate), read back in 30 us (5.6 TB/s, 0.87).
+// Eight lanes to a row: 46 and 32 us, sixteen: 91 and 51 us.  Ties and what is near them left to the division: 2 us more, with six BF16
+// prompts of 4546 tokens 11 us for 7.9.  Places looked up by a few threads for the block: 0.2 to 0.9 us more on small calls.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -19,10 +20,10 @@ namespace reskv {
 namespace {
 
 constexpr int kStoreWarps = 4, kStoreThreads = kStoreWarps * 32;
-// Pairs of (token, head) rows of a warp that are in flight together, where there are enough of them.  8 x 4000 tokens, us written and
-// read, pairs at 4 warps a block: 2 / 2 53.1 and 35.5, 4 / 4 54.8 and 32.9; at 8 warps 4 / 4 59.4 and 33.8, 8 / 8 73.4 and 37.0.
-template <bool WRITE>
-constexpr int kPairsAtOnce = WRITE ? 2 : 4;
+constexpr int kPassRows = 4;  // (token, head) rows that a warp takes at once
+// Passes of a warp that are in flight together, where there are enough rows.  8 x 4000 tokens, us written and read, by passes: 1 37.5 and
+// 32.9, 2 36.4 and 30.2, 4 42.6 and 32.0; 8 warps a block at 2 passes 39.7 and 30.2, 2 warps 35.9 and 29.9 (small calls slower).
+constexpr int kPasses = 2;
 
 struct StoreParams {
     PagedPlace at;
@@ -72,36 +73,50 @@ __device__ __forceinline__ uint32_t min_pair(uint32_t a, uint32_t b) {
 }
 
 // Codes of eight numbers; `scale` as stored, `low` the offset.
+//
+// The quotient by the reciprocal, corrected by its remainder, is the one that IEEE division gives: the correction leaves a relative
+// error below 2^-40, while a quotient of a 24-bit number and an 11-bit scale is never nearer than 2^-37 to the middle of two FP32
+// numbers.  That holds as long as the remainder does not underflow, hence kLeast.  Ties are common (one in
+// seven groups of 64 normal BF16 numbers has one), so they are not left to the division.
+struct Codes {
+    uint32_t a, b;
+};
 template <bool BF16>
-__device__ __forceinline__ uint32_t codes_of(const uint4& x, float low, float scale) {
+__device__ __forceinline__ Codes codes_of(const uint4& x, const uint4& y, float low, float scale) {
     constexpr float kRound = 12582912.f;  // 1.5 * 2^23: a sum with it is rounded to a whole number
-    constexpr float kNormal = BF16 ? 0x1p-126f : 0x1p-14f;
-    const uint32_t pairs[4] = {x.x, x.y, x.z, x.w};
-    float inverse, far = 0.f;
+    constexpr float kLeast = BF16 ? 0x1p-90f : 0x1p-14f, kMost = BF16 ? 0x1p125f : 65504.f;
+    const uint32_t pairs[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    float inverse;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(scale));
-    const float2 minus_low = make_float2(-low, -low), inverses = make_float2(inverse, inverse), up = make_float2(kRound, kRound),
-                 down = make_float2(-kRound, -kRound);
-    float2 above[4];
-    uint32_t word = 0;
+    const float2 minus_low = make_float2(-low, -low), inverses = make_float2(inverse, inverse), minus_scale = make_float2(-scale, -scale),
+                 up = make_float2(kRound, kRound);
+    const bool usual = scale >= kLeast && scale <= kMost;
+    uint32_t words[2];
 #pragma unroll
-    for (int e = 3; e >= 0; --e) {
-        above[e] = add2(make_float2(low_of<BF16>(pairs[e]), high_of<BF16>(pairs[e])), minus_low);
-        const float2 quotient = mul2(above[e], inverses), rounded = add2(quotient, up), whole = add2(rounded, down);
-        const float2 off = fma2(whole, make_float2(-1.f, -1.f), quotient);
-        far = max3_nan(far, fabsf(off.x), fabsf(off.y));
-        word = (word * 16u + __float_as_uint(rounded.y)) * 16u + __float_as_uint(rounded.x);  // the constant part goes below
-    }
-    word -= 0x4B400000u * 0x11111111u;
-    // By the reciprocal a quotient is off by less than 1e-5.  A quotient that near to a half, a scale that rounding has made much
-    // smaller than it should be (below the normal numbers, 0) and what is not finite: by the division.
-    if (far <= 0.49999f && scale >= kNormal) return word;
-    word = 0;
+    for (int w = 0; w < 2; ++w) {
+        uint32_t word = 0;
 #pragma unroll
-    for (int e = 7; e >= 0; --e) {
-        const float code = fminf(fmaxf(rintf((e & 1 ? above[e >> 1].y : above[e >> 1].x) / scale), 0.f), 15.f);  // a NaN becomes 0:
-        word = word * 16u + (scale > 0.f ? static_cast<uint32_t>(code) : 0u);                                   // the scale says it
+        for (int e = 4 * w + 3; e >= 4 * w; --e) {
+            const float2 above = add2(make_float2(low_of<BF16>(pairs[e]), high_of<BF16>(pairs[e])), minus_low), first = mul2(above, inverses);
+            const float2 rounded = add2(fma2(fma2(minus_scale, first, above), inverses, first), up);
+            word = (word * 16u + __float_as_uint(rounded.y)) * 16u + __float_as_uint(rounded.x);  // the constant part goes below
+        }
+        words[w] = word - 0x4B400000u * 0x11111111u;
     }
-    return word;
+    if (!usual) {  // scales that rounding may have made much too small (below the normal numbers, 0), and what is not finite
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            words[w] = 0;
+#pragma unroll
+            for (int e = 4 * w + 3; e >= 4 * w; --e)
+#pragma unroll
+                for (int half = 1; half >= 0; --half) {  // a NaN becomes 0: the scale says it
+                    const float quotient = ((half ? high_of<BF16>(pairs[e]) : low_of<BF16>(pairs[e])) - low) / scale;
+                    words[w] = words[w] * 16u + (scale > 0.f ? static_cast<uint32_t>(fminf(fmaxf(rintf(quotient), 0.f), 15.f)) : 0u);
+                }
+        }
+    }
+    return {words[0], words[1]};
 }
 
 // x / 15 as IEEE division rounds it (x finite): the quotient by the reciprocal, corrected by its remainder.
@@ -111,96 +126,98 @@ __device__ __forceinline__ float fifteenth(float x) {
     return fmaf(fmaf(-15.f, q, x), kInverse, q);
 }
 
-template <bool BF16, bool WRITE, int PAIRS>
+template <bool BF16, bool WRITE, int PASSES>
 __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const StoreParams p) {
-    constexpr int kRows = kStoreWarps * 2 * PAIRS;  // of a block
-    __shared__ TokenPlace places[kRows];
     wait_for_previous_launch();
     let_next_launch_start();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side = lane >> 3 & 1, c = lane & 7;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kRows;
-    const int token0 = static_cast<int>(first / p.heads), head0 = static_cast<int>(first - static_cast<int64_t>(token0) * p.heads);
-    // a warp's pairs of rows lie next to each other
-    int token[PAIRS], head[PAIRS];
-    uint4 x[PAIRS][2];
+    const int lane = threadIdx.x & 31, side = lane >> 2 & 1, c = lane & 3;
+    // a warp's rows lie next to each other
+    const int64_t first = (static_cast<int64_t>(blockIdx.x) * kStoreWarps + (threadIdx.x >> 5)) * (PASSES * kPassRows);
+    int token[PASSES], head[PASSES];
+    uint4 x[PASSES][4];
     {
-        const int row = warp * PAIRS * 2 + (lane >> 4);
-        int t = token0 + (head0 + row) / p.heads, h = (head0 + row) % p.heads;
+        const int before = static_cast<int>(first / p.heads), row = static_cast<int>(first - static_cast<int64_t>(before) * p.heads) + (lane >> 3);
+        int t = before + row / p.heads, h = row % p.heads;
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) {
+        for (int i = 0; i < PASSES; ++i) {
             token[i] = t < p.total ? t : -1, head[i] = h;
             if (WRITE && token[i] >= 0) {
                 const uint4* from = reinterpret_cast<const uint4*>(side ? p.v + t * p.v_token + h * p.v_head : p.k + t * p.k_token + h * p.k_head);
-                x[i][0] = from[c], x[i][1] = from[8 + c];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[i][j] = from[c + 4 * j];
             }
-            for (h += 2; h >= p.heads; h -= p.heads) ++t;
+            for (h += kPassRows; h >= p.heads; h -= p.heads) ++t;
         }
     }
-    for (int i = threadIdx.x; i < kRows && token0 + i < p.total && i <= (head0 + kRows - 1) / p.heads; i += kStoreThreads)
-        places[i] = place_of(p, token0 + i);
-    __syncthreads();
-    unsigned char* block[PAIRS];  // of the row's side, or null
-    int row[PAIRS];
+    unsigned char* block[PASSES];  // of the row's side, or null
+    int row[PASSES];
+    TokenPlace to{-1, 0};
 #pragma unroll
-    for (int i = 0; i < PAIRS; ++i) {
+    for (int i = 0; i < PASSES; ++i) {
         block[i] = nullptr, row[i] = 0;
         if (token[i] < 0) continue;
-        const TokenPlace to = places[token[i] - token0];
+        if (i == 0 || token[i] != token[i - 1]) to = place_of(p, token[i]);
         if (to.block >= 0) block[i] = p.pages + to.block + static_cast<int64_t>(head[i]) * kPageHeadBytes + side * kBlockSide;
         row[i] = to.row;
     }
     if (WRITE) {
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) {
+        for (int i = 0; i < PASSES; ++i) {
             // (group 0, group 1) extremes; rows without a place take part in the exchange with whatever they hold
-            if (token[i] < 0) x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);
+            if (token[i] < 0) x[i][0] = x[i][1] = x[i][2] = x[i][3] = make_uint4(0, 0, 0, 0);
             uint32_t top[2], bottom[2];
 #pragma unroll
             for (int group = 0; group < 2; ++group) {
-                const uint4& v = x[i][group];
-                top[group] = max_pair<BF16>(max_pair<BF16>(v.x, v.y), max_pair<BF16>(v.z, v.w));
-                bottom[group] = min_pair<BF16>(min_pair<BF16>(v.x, v.y), min_pair<BF16>(v.z, v.w));
+                const uint4 &v = x[i][2 * group], &w = x[i][2 * group + 1];
+                top[group] = max_pair<BF16>(max_pair<BF16>(max_pair<BF16>(v.x, v.y), max_pair<BF16>(v.z, v.w)),
+                                            max_pair<BF16>(max_pair<BF16>(w.x, w.y), max_pair<BF16>(w.z, w.w)));
+                bottom[group] = min_pair<BF16>(min_pair<BF16>(min_pair<BF16>(v.x, v.y), min_pair<BF16>(v.z, v.w)),
+                                               min_pair<BF16>(min_pair<BF16>(w.x, w.y), min_pair<BF16>(w.z, w.w)));
             }
             uint32_t high = max_pair<BF16>(__byte_perm(top[0], top[1], 0x5410), __byte_perm(top[0], top[1], 0x7632));
             uint32_t low = min_pair<BF16>(__byte_perm(bottom[0], bottom[1], 0x5410), __byte_perm(bottom[0], bottom[1], 0x7632));
 #pragma unroll
-            for (int off = 1; off < 8; off <<= 1) {
+            for (int off = 1; off < 4; off <<= 1) {
                 high = max_pair<BF16>(high, __shfl_xor_sync(0xffffffffu, high, off));
                 low = min_pair<BF16>(low, __shfl_xor_sync(0xffffffffu, low, off));
             }
             if (!block[i]) continue;
             const float low0 = low_of<BF16>(low), low1 = high_of<BF16>(low);
             const uint32_t scales = pack2<BF16>(fifteenth(low_of<BF16>(high) - low0), fifteenth(high_of<BF16>(high) - low1));
-            const uint32_t w0 = codes_of<BF16>(x[i][0], low0, low_of<BF16>(scales)), w1 = codes_of<BF16>(x[i][1], low1, high_of<BF16>(scales));
+            const Codes first_group = codes_of<BF16>(x[i][0], x[i][1], low0, low_of<BF16>(scales)),
+                        second_group = codes_of<BF16>(x[i][2], x[i][3], low1, high_of<BF16>(scales));
             if (side) {
-                *reinterpret_cast<uint2*>(block[i] + value_word(row[i], c)) = make_uint2(w0, w1);
+                *reinterpret_cast<uint2*>(block[i] + value_word(row[i], c)) = make_uint2(first_group.a, second_group.a);
+                *reinterpret_cast<uint2*>(block[i] + value_word(row[i], c + 4)) = make_uint2(first_group.b, second_group.b);
             } else {
-                *reinterpret_cast<uint32_t*>(block[i] + key_word(row[i], c)) = w0;
-                *reinterpret_cast<uint32_t*>(block[i] + key_word(row[i], c + 8)) = w1;
+                *reinterpret_cast<uint4*>(block[i] + key_word(row[i], c)) = make_uint4(first_group.a, first_group.b, second_group.a, second_group.b);
             }
             if (c == 0) *reinterpret_cast<uint2*>(block[i] + kBlockCodes + row[i] * 8) = make_uint2(scales, low);
         }
     } else {
-        uint2 words[PAIRS], params[PAIRS];
+        uint4 words[PASSES];  // c, c + 4, c + 8, c + 12
+        uint2 params[PASSES];
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) {
+        for (int i = 0; i < PASSES; ++i) {
             if (!block[i]) continue;
-            if (side)
-                words[i] = *reinterpret_cast<const uint2*>(block[i] + value_word(row[i], c));
-            else
-                words[i] = make_uint2(*reinterpret_cast<const uint32_t*>(block[i] + key_word(row[i], c)),
-                                      *reinterpret_cast<const uint32_t*>(block[i] + key_word(row[i], c + 8)));
+            if (side) {
+                const uint2 a = *reinterpret_cast<const uint2*>(block[i] + value_word(row[i], c)),
+                            b = *reinterpret_cast<const uint2*>(block[i] + value_word(row[i], c + 4));
+                words[i] = make_uint4(a.x, b.x, a.y, b.y);
+            } else {
+                words[i] = *reinterpret_cast<const uint4*>(block[i] + key_word(row[i], c));
+            }
             params[i] = *reinterpret_cast<const uint2*>(block[i] + kBlockCodes + row[i] * 8);
         }
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) {
+        for (int i = 0; i < PASSES; ++i) {
             if (!block[i]) continue;
             uint4* to = reinterpret_cast<uint4*>((side ? p.v_out : p.k_out) + (static_cast<int64_t>(token[i]) * p.heads + head[i]) * 128);
 #pragma unroll
-            for (int group = 0; group < 2; ++group) {
-                const float scale = group ? high_of<BF16>(params[i].x) : low_of<BF16>(params[i].x);
-                const float low = group ? high_of<BF16>(params[i].y) : low_of<BF16>(params[i].y);
-                const uint32_t word = group ? words[i].y : words[i].x;
+            for (int j = 0; j < 4; ++j) {
+                const float scale = j >> 1 ? high_of<BF16>(params[i].x) : low_of<BF16>(params[i].x);
+                const float low = j >> 1 ? high_of<BF16>(params[i].y) : low_of<BF16>(params[i].y);
+                const uint32_t word = j == 0 ? words[i].x : j == 1 ? words[i].y : j == 2 ? words[i].z : words[i].w;
                 const float2 scales = make_float2(scale, scale), lows = make_float2(low, low), down = make_float2(-8388608.f, -8388608.f);
                 uint4 y;
                 uint32_t* pairs = reinterpret_cast<uint32_t*>(&y);
@@ -211,7 +228,7 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const StoreP
                     const float2 v = fma2(scales, code, lows);
                     pairs[e] = pack2<BF16>(v.x, v.y);
                 }
-                to[8 * group + c] = y;
+                to[4 * j + c] = y;
             }
         }
     }
@@ -256,20 +273,20 @@ int check_place(const char* who, const int32_t* cu, const int32_t* starts, const
     return width > 0 ? check_device_pointer(table, who, "table") : RESKV_OK;
 }
 
-template <bool BF16, bool WRITE, int PAIRS>
+template <bool BF16, bool WRITE, int PASSES>
 int launch_store(const StoreParams& p, cudaStream_t stream) {
-    constexpr int per = kStoreWarps * 2 * PAIRS;
+    constexpr int per = kStoreWarps * kPassRows * PASSES;
     const int64_t blocks = (static_cast<int64_t>(p.total) * p.heads + per - 1) / per;
     if (blocks > 0x7fffffff) return fail(RESKV_ERR_LIMIT, "paged cache: too many tokens for one call");
-    return check_cuda(launch_overlapped(paged_store_kernel<BF16, WRITE, PAIRS>, dim3(static_cast<unsigned>(blocks)), kStoreThreads, 0, stream, true, p),
+    return check_cuda(launch_overlapped(paged_store_kernel<BF16, WRITE, PASSES>, dim3(static_cast<unsigned>(blocks)), kStoreThreads, 0, stream, true, p),
                       WRITE ? "paged_write launch" : "paged_read launch");
 }
-// One pair of rows per warp as long as that leaves SMs without a block.
+// One pass per warp as long as that leaves SMs without a block.
 template <bool WRITE>
 int run_store(const StoreParams& p, int bf16, cudaStream_t stream) {
-    const bool many = static_cast<int64_t>(p.total) * p.heads > static_cast<int64_t>(sm_count()) * kStoreWarps * 2;
-    return bf16 ? many ? launch_store<true, WRITE, kPairsAtOnce<WRITE>>(p, stream) : launch_store<true, WRITE, 1>(p, stream)
-                : many ? launch_store<false, WRITE, kPairsAtOnce<WRITE>>(p, stream) : launch_store<false, WRITE, 1>(p, stream);
+    const bool many = static_cast<int64_t>(p.total) * p.heads > static_cast<int64_t>(sm_count()) * kStoreWarps * kPassRows;
+    return bf16 ? many ? launch_store<true, WRITE, kPasses>(p, stream) : launch_store<true, WRITE, 1>(p, stream)
+                : many ? launch_store<false, WRITE, kPasses>(p, stream) : launch_store<false, WRITE, 1>(p, stream);
 }
 
 }  // namespace

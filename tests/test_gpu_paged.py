@@ -153,6 +153,33 @@ def test_rows_at_the_edges(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_codes_at_ties_and_at_every_magnitude(dtype):
+    """Quotients that are halves, or next to one, and scales from the subnormal numbers to the largest: the codes of the division."""
+    info = torch.finfo(dtype)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    halves = torch.arange(31, device=DEV) / 2  # 0, 0.5, .. 15: with 15 and 0 among them the scale is 1
+    rows = []
+    for i in range(400):
+        x = halves[torch.randint(31, (128,), generator=g, device=DEV)]
+        x[[0, 64]], x[[1, 65]] = 0.0, 15.0
+        if i % 4 == 1:  # a step of the type beside them
+            x = x * (1 + info.eps * (torch.randint(3, (128,), generator=g, device=DEV) - 1))
+        elif i % 4 == 2:
+            x = torch.rand(128, generator=g, device=DEV) * 15
+        elif i % 4 == 3:
+            x = x - 7.5
+        least, most = (-132, 123) if dtype == torch.bfloat16 else (-24, 11)
+        rows.append((x.double() * 2.0 ** (least + i * (most - least) // 399)).to(dtype))
+    x = torch.stack(rows)[:, None]
+    cache = PagedInt4Cache(1, 1, 8, dtype=dtype)
+    step = cache.extend(cache.add(1), [400])
+    cache.write(0, step, x, x.flip(0))
+    k, v = cache.read(0, step)
+    assert torch.equal(k, values_of(x)) and torch.equal(v, values_of(x.flip(0)))
+
+
+@pytest.mark.gpu
 def test_layouts_in_memory():
     """Views of a fused projection, head-major and misaligned tensors are stored alike."""
     cache = PagedInt4Cache(1, 2, 4)
