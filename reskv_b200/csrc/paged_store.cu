@@ -7,7 +7,8 @@
 // bytes in a row of their own.  Extremes of both groups travel together as 16-bit pairs.  A warp looks up by itself where its tokens
 // go, while their rows are on the way.
 //
-// 8 x 4000 tokens, 8 heads: written in 36 us (168 MB, 4.6 TB/s, 0.72 of the copy rate), read back in 30 us (5.6 TB/s, 0.87).
+// 8 x 4000 tokens, 8 heads: written in 36 us (168 MB, 4.7 TB/s, 0.72 of the copy rate), read back in 30 us (5.6 TB/s, 0.87); 65 % of the
+// issue slots are taken.  Loads that ask to leave L2 first: 34.6 us, but attention over the prompt reads the same rows.
 // Eight lanes to a row: 46 and 32 us, sixteen: 91 and 51 us.  Ties and what is near them left to the division: 2 us more, with six BF16
 // prompts of 4546 tokens 11 us for 7.9.  Places looked up by a few threads for the block: 0.2 to 0.9 us more on small calls.
 #include <algorithm>
@@ -24,6 +25,10 @@ constexpr int kPassRows = 4;  // (token, head) rows that a warp takes at once
 // Passes of a warp that are in flight together, where there are enough rows.  8 x 4000 tokens, us written and read, by passes: 1 37.5 and
 // 32.9, 2 36.4 and 30.2, 4 42.6 and 32.0; 8 warps a block at 2 passes 39.7 and 30.2, 2 warps 35.9 and 29.9 (small calls slower).
 constexpr int kPasses = 2;
+// Blocks that an SM is to hold: registers against rows in flight.  6 prompts of 4546 BF16 tokens, us written: left to the compiler (71
+// registers) 7.2, 8 blocks 6.4, 10 (spills) 8.1; read: left to the compiler 6.4, 10 blocks 6.1, 14 blocks 5.6, 16 blocks 5.6.
+template <bool WRITE>
+constexpr int kBlocksPerSm = WRITE ? 8 : 14;
 
 struct StoreParams {
     PagedPlace at;
@@ -127,7 +132,7 @@ __device__ __forceinline__ float fifteenth(float x) {
 }
 
 template <bool BF16, bool WRITE, int PASSES>
-__global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const StoreParams p) {
+__global__ void __launch_bounds__(kStoreThreads, kBlocksPerSm<WRITE>) paged_store_kernel(const StoreParams p) {
     wait_for_previous_launch();
     let_next_launch_start();
     const int lane = threadIdx.x & 31, side = lane >> 2 & 1, c = lane & 3;
