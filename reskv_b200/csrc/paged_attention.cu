@@ -5,8 +5,12 @@
 // nibble, code * 2^-20 in the next one, exactly; scales and offsets enter outside of the product,
 //     q . k_j   = sum_groups scale_j,g * (q_g . code_j,g) + offset_j,g * sum(q_g)
 //     sum p v   = sum_j (p_j scale_j,g) (code_j,g - 8) + sum_j p_j (offset_j,g + 8 scale_j,g)
-// with p * scale rounded to FP16 once as the product's operand.  Bound by the cache's bytes as long as a token costs less than
-// its 144 bytes take to arrive.
+// with p * scale rounded to FP16 once as the product's operand.
+//
+// 32 x 8128 tokens, 32 / 8 heads: 68 us for 300 MB, 4.4 TB/s (0.69 of the copy rate).  Bound by instructions, 21 of a warp per token and
+// KV head (issue slots 58 %, integer pipe 50 %: masks and shifts that bring the codes into operands).  Small calls are bound by
+// latency: one sequence of 300 tokens 6.9 us, of 8128 10.5 us, nine ragged ones with eight query heads 16 us (28 MB), of which two
+// dependent launches, look-ups of lengths and pages, a copy, a chunk, two meetings of the warps and the merge follow one another.
 //
 // Work: the pages of all (sequence, KV head) units lie end to end and every CTA takes an equal share; a unit that lies in one
 // CTA is finished there, the parts of the others are added by a second kernel.  Eight warps take a segment's chunks of 32 tokens
@@ -25,8 +29,14 @@ constexpr int kPaStages = 2;
 constexpr int kChunkBlocks = 2, kChunkTokens = kChunkBlocks * kBlockTokens, kChunkBytes = kChunkBlocks * kBlockBytes;  // a warp's turn
 constexpr int kPaPerSm = 2;                       // CTAs of an SM
 constexpr int kPageChunks = kPageTokens / kChunkTokens;
-constexpr int kPaCharge = 8;                      // a segment costs as much as that many pages besides its own
-constexpr int kPaLeast = 4;                       // a share is at least that long (a unit of one page: two CTAs' worth)
+// A segment costs as much as kPaCharge pages besides its own.  us at charges of 2, 5, 8, 12: nine ragged sequences 21.5, 18.0, 16.8,
+// 17.5; 64 ragged ones 33.0, 26.1, 25.7, 26.6; 32 x 2000 tokens 26.4, 26.1, 25.7, 25.2.
+constexpr int kPaCharge = 8;
+// A share is at least two pages long, four or eight (one or two turns of the eight warps) where the average stretch of a unit is
+// longer: parts cost time when they are added.  us at 2, 4, 8: 1 x 1000 tokens 7.0, 7.6, 8.7; 1 x 3000 9.1, 8.2, 9.1; 1 x 8128 11.3,
+// 10.9, 10.2.
+__host__ __device__ constexpr int least_share(int average) { return average > 90 ? 8 : average > 40 ? 4 : 2; }
+constexpr int kPaMergeWarps = 16;                 // of a query head at most
 constexpr int kPaSumBytes = kPaWarps * kPagedGroup * kHeadDim * 4;
 constexpr int kPaSmem = kPaWarps * kPaStages * kChunkBytes + kPaSumBytes;
 constexpr float kCodeMiddle = 8.f;
@@ -62,7 +72,8 @@ __device__ __forceinline__ int stretch_of(int length) { return length > 0 ? page
 struct Shares {
     int ctas, each, extra;
     __device__ __forceinline__ Shares(const PagedParams& p, int all) {
-        ctas = min(p.ctas, (all + kPaLeast - 1) / kPaLeast);
+        const int least = least_share(all / (p.heads * p.sequences));
+        ctas = min(p.ctas, (all + least - 1) / least);
         each = ctas ? all / ctas : 0, extra = all - each * ctas;
     }
     __device__ __forceinline__ int begin(int cta) const { return cta * each + min(cta, extra); }
@@ -576,12 +587,13 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
 }
 
 // Adds the parts of a unit that lies in several CTAs; a unit without tokens gets zeros.  Bound by latency: `split` warps per query
-// head take the parts in turn, and meet in shared memory.
+// head take the parts in turn, each with a running maximum of its own, and meet in shared memory.
 template <bool BF16>
 __global__ void __launch_bounds__(1024) paged_merge_kernel(const PagedParams p, int split) {
     __shared__ float4 s_out[32][32];
-    __shared__ float s_total[32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = warp / split, turn = warp - head * split, unit = blockIdx.x;
+    __shared__ float2 s_stats[32];  // maximum, sum
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, turn = warp % split, unit = blockIdx.x;
+    const int head = blockIdx.y * (blockDim.x / 32 / split) + warp / split;
     // The lengths may be read at once: this kernel starts when every CTA of the first one has seen the end of what came before
     // (without pages there is no first one, and the lengths count as 0).
     const int sequence = unit / p.heads, kv_head = unit - sequence * p.heads;
@@ -607,31 +619,25 @@ __global__ void __launch_bounds__(1024) paged_merge_kernel(const PagedParams p, 
     const int count = to - from + 1;
     const int skip = shares.begin(from) < a ? 1 : 0;  // the last page of another unit lies in front of it in its first CTA: that CTA's second part
     const float* parts = p.parts + 2 * static_cast<int64_t>(from) * kPartialFloats;
-    const auto part = [&](int i) { return parts + (2 * i + (i == 0 ? skip : 0)) * kPartialFloats; };
-    float top = -INFINITY;
-    for (int i = lane; i < count; i += 32) top = fmaxf(top, part(i)[kPagedGroup * kHeadDim + head]);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    float top = -INFINITY, total = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    float total = 0.f;
+    const auto add = [&](float m, float l, const float4& x) {
+        const float next = fmaxf(top, m), old = top == next ? 1.f : fast_exp2(top - next), now = m == next ? 1.f : fast_exp2(m - next);
+        top = next;
+        sum.x = fmaf(x.x, now, sum.x * old), sum.y = fmaf(x.y, now, sum.y * old), sum.z = fmaf(x.z, now, sum.z * old), sum.w = fmaf(x.w, now, sum.w * old);
+        total = fmaf(l, now, total * old);
+    };
 #pragma unroll 4
     for (int i = turn; i < count; i += split) {
-        const float* from_part = part(i);
-        const float m = from_part[kPagedGroup * kHeadDim + head], l = from_part[kPagedGroup * (kHeadDim + 1) + head];
-        const float4 x = *reinterpret_cast<const float4*>(from_part + head * kHeadDim + 4 * lane);
-        const float weight = m == top ? 1.f : fast_exp2(m - top);
-        sum.x = fmaf(x.x, weight, sum.x), sum.y = fmaf(x.y, weight, sum.y), sum.z = fmaf(x.z, weight, sum.z), sum.w = fmaf(x.w, weight, sum.w);
-        total = fmaf(l, weight, total);
+        const float* part = parts + (2 * i + (i == 0 ? skip : 0)) * kPartialFloats;
+        add(part[kPagedGroup * kHeadDim + head], part[kPagedGroup * (kHeadDim + 1) + head], *reinterpret_cast<const float4*>(part + head * kHeadDim + 4 * lane));
     }
     if (split > 1) {
         s_out[warp][lane] = sum;
-        if (lane == 0) s_total[warp] = total;
+        if (lane == 0) s_stats[warp] = make_float2(top, total);
         __syncthreads();
         if (turn > 0) return;
-        for (int w = 1; w < split; ++w) {
-            const float4 x = s_out[warp + w][lane];
-            sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w, total += s_total[warp + w];
-        }
+        for (int w = 1; w < min(split, count); ++w) add(s_stats[warp + w].x, s_stats[warp + w].y, s_out[warp + w][lane]);
     }
     const float inv = 1.f / total;
     *reinterpret_cast<uint2*>(p.out + row * kHeadDim + 4 * lane) =
@@ -639,11 +645,12 @@ __global__ void __launch_bounds__(1024) paged_merge_kernel(const PagedParams p, 
     if (p.lse && lane == 0) p.lse[row] = top * kLn2 + logf(total);
 }
 
-// CTAs of the first kernel for as many pages as there may be.
+// CTAs of the first kernel for as many pages as there may be.  No more than will have a share: those without one displace others
+// (1 x 8128 tokens: 12.6 us with 296 CTAs for 135 shares, 10.2 with 135).
 int paged_ctas(int sequences, int width, int heads) {
     if (width == 0) return 0;
-    const int64_t most = (static_cast<int64_t>(sequences) * (width + kPaCharge) * heads + kPaLeast - 1) / kPaLeast, room = kPaPerSm * sm_count();
-    return static_cast<int>(most < room ? most : room);
+    const int64_t least = least_share(width + kPaCharge), most = (static_cast<int64_t>(sequences) * (width + kPaCharge) * heads + least - 1) / least;
+    return static_cast<int>(std::min<int64_t>(most, kPaPerSm * sm_count()));
 }
 
 template <bool BF16>
@@ -654,8 +661,14 @@ int launch(const PagedParams& p, cudaStream_t stream) {
         if (int rc = check_cuda(launch_overlapped(paged_attention_kernel<BF16>, dim3(static_cast<unsigned>(p.ctas)), kPaThreads, kPaSmem, stream, true, p),
                                 "paged_attention launch"))
             return rc;
-    const int units = p.sequences * p.heads, split = units <= sm_count() && 32 / p.group > 1 ? std::min(8, 32 / p.group) : 1;
-    return check_cuda(launch_overlapped(paged_merge_kernel<BF16>, dim3(static_cast<unsigned>(units)), p.group * split * 32, 0, stream, true, p, split),
+    const int units = p.sequences * p.heads;
+    // As many warps per query head as the SMs hold at once; one, and all heads in a block, where that would be two: 16, 8 and 1
+    // for nine sequences of eight heads with eight query heads each 16.7, 15.7 and 19 us, for 64 with four each 22 (8) and 18.4 (1) us.
+    int split = kPaMergeWarps;
+    while (split > 1 && static_cast<int64_t>(units) * p.group * split > 32 * sm_count()) split /= 2;
+    const bool few = split >= 4;
+    const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(few ? p.group : 1));
+    return check_cuda(launch_overlapped(paged_merge_kernel<BF16>, grid, (few ? split : p.group) * 32, 0, stream, true, p, few ? split : 1),
                       "paged_attention merge launch");
 }
 
