@@ -5,11 +5,11 @@
 // nibble, code * 2^-20 in the next one, exactly; scales and offsets enter outside of the product,
 //     q . k_j   = sum_groups scale_j,g * (q_g . code_j,g) + offset_j,g * sum(q_g)
 //     sum p v   = sum_j (p_j scale_j,g) (code_j,g - 8) + sum_j p_j (offset_j,g + 8 scale_j,g)
-// with p * scale rounded to FP16 once as the product's operand.
+// with p * scale in FP16 as the product's operand, for FP16 models in two parts.
 //
-// 32 x 8128 tokens, 32 / 8 heads: 68 us for 300 MB, 4.4 TB/s (0.69 of the copy rate).  Bound by instructions, 21 of a warp per token and
+// 32 x 8128 tokens, 32 / 8 heads: 71 us for 300 MB, 4.2 TB/s (0.65 of the copy rate).  Bound by instructions, 22 of a warp per token and
 // KV head (issue slots 58 %, integer pipe 50 %: masks and shifts that bring the codes into operands).  Small calls are bound by
-// latency: one sequence of 300 tokens 6.9 us, of 8128 10.5 us, nine ragged ones with eight query heads 16 us (28 MB), of which two
+// latency: one sequence of 300 tokens 7.0 us, of 8128 10.6 us, nine ragged BF16 ones with eight query heads 16 us (28 MB), of which two
 // dependent launches, look-ups of lengths and pages, a copy, a chunk, two meetings of the warps and the merge follow one another.
 //
 // Work: the pages of all (sequence, KV head) units lie end to end and every CTA takes an equal share; a unit that lies in one
@@ -218,8 +218,15 @@ __device__ __forceinline__ bool next_segment(const PagedParams& p, Segments& at,
     return __shfl_sync(0xffffffffu, any, 0);
 }
 
-template <bool BF16>
+// How p * scale goes into the product with the codes.  Rounded to FP16 once it is off by as much as an FP16 result, so FP16 models add
+// what the rounding took: in columns 4 to 7, which hold the heads once more, as long as there are four heads at most, otherwise by a
+// second product.  Error of the result over that of its own rounding, 32 x 8128 tokens: 1.45 rounded once, 1.00 with the rest.  That
+// costs 67.8 to 71.2 us there, 27.0 to 30.1 us with 32 x 2000 tokens of eight heads.  BF16 results are rounded eight times as far: 1.01.
+enum class Weights { kOnce, kBeside, kTwice };
+
+template <bool BF16, Weights WEIGHTS>
 __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(const PagedParams p) {
+    constexpr bool kBeside = WEIGHTS == Weights::kBeside, kTwice = WEIGHTS == Weights::kTwice;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint64_t bar_full[kPaWarps][kPaStages];
     __shared__ float s_max[kPaWarps][kPagedGroup], s_sum[kPaWarps][kPagedGroup], s_top[kPagedGroup];
@@ -298,6 +305,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
     // Row n of a tile of eight tokens is row n / 2 (n even) or 4 + (n / 2 ^ 1) (n odd) of the block's eight: the rows that the lanes
     // of a quad read together (tokens 2t, 2t + 1 of the contraction with the values) lie on different banks.
     const int row_even = t, row_odd = 4 + (t ^ 1), own_row = (g >> 1) ^ (g & 1 ? 5 : 0);
+    const float takes = kTwice || t >= 2 ? -1.f : 0.f;  // whether the lane's columns hold what the rounding took
     int stage = 0, phase = 0;
     bool first_segment = true;
     for (bool any = true; any; any = next_segment(p, at, lane)) {
@@ -310,8 +318,9 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint4 raw = make_uint4(0, 0, 0, 0);
-                if (g < p.group)
-                    raw = *reinterpret_cast<const uint4*>(p.q + at.sequence * p.q_sequence + (at.head * p.group + g) * p.q_head + 32 * j + 8 * t);
+                const int head = kBeside ? g & 3 : g;
+                if (head < p.group)
+                    raw = *reinterpret_cast<const uint4*>(p.q + at.sequence * p.q_sequence + (at.head * p.group + head) * p.q_head + 32 * j + 8 * t);
                 const uint32_t* pairs = reinterpret_cast<const uint32_t*>(&raw);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -466,7 +475,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
             for (int b = 0; b < kChunkBlocks; ++b) {
                 const unsigned char* values = chunk + b * kBlockBytes + kBlockSide;
                 // ---- weights: rows = tokens, turned round for the contraction over them --------------------------------------------
-                uint32_t weights[2][2];  // [group][half of the block's tokens]
+                uint32_t weights[2][2], rest[2][2];  // [group][half of the block's tokens]
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float2 weight = make_float2(fast_exp2(power[b][2 * i]), fast_exp2(power[b][2 * i + 1]));
@@ -475,7 +484,14 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
                     for (int group = 0; group < 2; ++group) {
                         const float scale = group ? high_of<BF16>(params[b][i].x) : low_of<BF16>(params[b][i].x);
                         const float offset = group ? high_of<BF16>(params[b][i].y) : low_of<BF16>(params[b][i].y);
-                        weights[group][i] = transposed(pack2<false>(weight.x * scale, weight.y * scale));
+                        const float2 exact = make_float2(weight.x * scale, weight.y * scale);
+                        uint32_t pair = pack2<false>(exact.x, exact.y);
+                        if (kBeside || kTwice) {
+                            const float2 left = fma2(make_float2(low_of<false>(pair), high_of<false>(pair)), make_float2(takes, takes), exact);
+                            const uint32_t other = pack2<false>(left.x, left.y);
+                            if (kBeside) pair = other; else rest[group][i] = transposed(other);
+                        }
+                        weights[group][i] = transposed(pair);
                         const float middle = fmaf(scale, kCodeMiddle, offset);
                         flat[group].x = fmaf(weight.x, middle, flat[group].x), flat[group].y = fmaf(weight.y, middle, flat[group].y);
                     }
@@ -489,6 +505,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
                         mma_16816_start(eights[group], kMiddleLow, kMiddleHigh, kMiddleLow, kMiddleHigh, weights[group][0], weights[group][1]);
                     else
                         mma_16816(eights[group], kMiddleLow, kMiddleHigh, kMiddleLow, kMiddleHigh, weights[group][0], weights[group][1]);
+                    if (kTwice) mma_16816(eights[group], kMiddleLow, kMiddleHigh, kMiddleLow, kMiddleHigh, rest[group][0], rest[group][1]);
                 }
                 uint2 rows[4];
 #pragma unroll
@@ -503,8 +520,12 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
                         const uint32_t pick = half ? 0x7632u : 0x5410u;
                         const uint32_t x = __byte_perm(group ? rows[0].y : rows[0].x, group ? rows[1].y : rows[1].x, pick), x8 = x >> 8;
                         const uint32_t y = __byte_perm(group ? rows[2].y : rows[2].x, group ? rows[3].y : rows[3].x, pick), y8 = y >> 8;
-                        mma_16816(acc[group * 4 + half * 2], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, weights[group][0], weights[group][1]);
-                        mma_16816(acc[group * 4 + half * 2 + 1], x8 & 0x000F000Fu, x8 & 0x00F000F0u, y8 & 0x000F000Fu, y8 & 0x00F000F0u, weights[group][0], weights[group][1]);
+                        const auto add = [&](const uint32_t(&w)[2]) {
+                            mma_16816(acc[group * 4 + half * 2], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, w[0], w[1]);
+                            mma_16816(acc[group * 4 + half * 2 + 1], x8 & 0x000F000Fu, x8 & 0x00F000F0u, y8 & 0x000F000Fu, y8 & 0x00F000F0u, w[0], w[1]);
+                        };
+                        add(weights[group]);
+                        if (kTwice) add(rest[group]);
                     }
             }
 #pragma unroll
@@ -540,6 +561,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
             for (int i = 0; i < 2; ++i) {
                 const float2 f = over_tokens(flat[i]);
                 base[i][0] = f.x * unit, base[i][1] = f.y * unit;
+                if (kBeside && t >= 2) base[i][0] = base[i][1] = 0.f;
             }
             float* mine = sums + warp * kPagedGroup * kHeadDim + 2 * t * kHeadDim;
 #pragma unroll
@@ -548,7 +570,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
                 const int d = (i >> 2) * 64 + 8 * g + (i & 3) * 2;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    if (2 * t + h < p.group)
+                    if ((kBeside ? (2 * t + h) & 3 : 2 * t + h) < p.group)
                         *reinterpret_cast<float2*>(mine + h * kHeadDim + d) = make_float2(fmaf(acc[i][h] * low, unit, base[i >> 2][h]) * weight[h],
                                                                                        fmaf(acc[i][2 + h] * high, unit, base[i >> 2][h]) * weight[h]);
             }
@@ -564,6 +586,10 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
             for (int w = 0; w < active; ++w) {
                 const float4 x = *reinterpret_cast<const float4*>(sums + w * kPagedGroup * kHeadDim + i);
                 sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+                if (kBeside) {
+                    const float4 y = *reinterpret_cast<const float4*>(sums + (w * kPagedGroup + 4) * kHeadDim + i);
+                    sum.x += y.x, sum.y += y.y, sum.z += y.z, sum.w += y.w;
+                }
                 total += s_sum[w][head];
             }
             if (whole) {
@@ -653,12 +679,12 @@ int paged_ctas(int sequences, int width, int heads) {
     return static_cast<int>(std::min<int64_t>(most, kPaPerSm * sm_count()));
 }
 
-template <bool BF16>
+template <bool BF16, Weights WEIGHTS>
 int launch(const PagedParams& p, cudaStream_t stream) {
     static std::atomic<unsigned long long> done{0};
-    if (int rc = allow_smem(paged_attention_kernel<BF16>, kPaSmem, done, "cudaFuncSetAttribute(paged_attention)")) return rc;
+    if (int rc = allow_smem(paged_attention_kernel<BF16, WEIGHTS>, kPaSmem, done, "cudaFuncSetAttribute(paged_attention)")) return rc;
     if (p.ctas > 0)
-        if (int rc = check_cuda(launch_overlapped(paged_attention_kernel<BF16>, dim3(static_cast<unsigned>(p.ctas)), kPaThreads, kPaSmem, stream, true, p),
+        if (int rc = check_cuda(launch_overlapped(paged_attention_kernel<BF16, WEIGHTS>, dim3(static_cast<unsigned>(p.ctas)), kPaThreads, kPaSmem, stream, true, p),
                                 "paged_attention launch"))
             return rc;
     const int units = p.sequences * p.heads;
@@ -714,5 +740,7 @@ extern "C" int reskv_paged_attention(const void* q, int bf16, int64_t q_sequence
     p.q = static_cast<const unsigned short*>(q), p.q_sequence = q_sequence, p.q_head = q_head, p.scale_log2 = scaling * kLog2e;
     p.out = static_cast<unsigned short*>(out), p.lse = lse, p.parts = static_cast<float*>(workspace);
     p.ctas = paged_ctas(sequences, width, kv_heads), p.status = status;
-    return bf16 ? launch<true>(p, static_cast<cudaStream_t>(stream)) : launch<false>(p, static_cast<cudaStream_t>(stream));
+    const cudaStream_t on = static_cast<cudaStream_t>(stream);
+    if (bf16) return launch<true, Weights::kOnce>(p, on);
+    return p.group <= kPagedGroup / 2 ? launch<false, Weights::kBeside>(p, on) : launch<false, Weights::kTwice>(p, on);
 }
