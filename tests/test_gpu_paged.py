@@ -262,6 +262,21 @@ def test_magnitudes(dtype, key_size, value_size, scaling):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kv_heads,ratio", [(4, 1), (2, 3), (2, 4), (1, 5), (2, 8)])
+def test_an_fp16_result_is_as_good_as_its_rounding(kv_heads, ratio):
+    """Besides the result's rounding (2^-11 at most, about 2e-4 in the mean square) there are FP32 errors of scores, exponentials and
+    sums: below 2e-5 of a result that is a fiftieth of its terms, a tenth of the rounding, sqrt(1 + 0.1^2) = 1.005 together."""
+    cache = PagedInt4Cache(1, kv_heads, 40)
+    seqs, k, v = fill(cache, [2000, 300], seed=11)
+    got = assert_attends(cache, seqs, k, v, ratio, seed=4)
+    q = torch.randn(2, kv_heads * ratio, 128, generator=torch.Generator(device=DEV).manual_seed(4), device=DEV).half()
+    for i in range(2):
+        want = formula(q[i], k[i], v[i])[0]
+        off, rounding = (got[i].double() - want).norm(), (want.half().double() - want).norm()
+        assert off < 1.05 * rounding, f"sequence {i}: {off / rounding:.3f}"
+
+
+@pytest.mark.gpu
 def test_a_maximum_that_grows_along_the_sequence():
     cache = PagedInt4Cache(1, 1, 40)
     seqs = cache.add(1)
