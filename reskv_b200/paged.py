@@ -33,7 +33,7 @@ class PagedStep:
     step.  ``cu_seqlens`` (int32, on the device) says which rows of the packed tensors belong to which sequence and serves
     ``prompt_attention`` as it is."""
 
-    __slots__ = ("sequences", "counts", "lengths", "total", "cu_seqlens", "starts", "device_lengths", "table", "_numbers", "_whole", "_epoch",
+    __slots__ = ("sequences", "counts", "lengths", "total", "cu_seqlens", "starts", "device_lengths", "table", "_tables", "_use", "_whole", "_epoch",
                  "_current")
 
     def _everything(self):
@@ -44,6 +44,15 @@ class PagedStep:
                 raise ValueError("too many tokens for one call")
             self._whole = (_upload(ends.astype(np.int32), self.table.device), torch.zeros_like(self.starts), int(ends[-1]))
         return self._whole
+
+
+class _Tables:
+    """Tables on the device, and how many steps have had them: they are the last one's."""
+
+    __slots__ = ("numbers", "book", "uses")
+
+    def __init__(self, numbers, book):
+        self.numbers, self.book, self.uses = numbers, book, 0
 
 
 def _pinned(numbers: np.ndarray) -> torch.Tensor:
@@ -98,14 +107,15 @@ class PagedInt4Cache:
         of these sequences may not be used any more.  RuntimeError, and nothing changed, when the pool has too few pages.
 
         For captured graphs: the page table is made at least ``width`` pages wide, and with ``reuse``, an earlier step of as many
-        sequences, the tables are written to that step's tensors, whose addresses a graph holds.  ValueError, and nothing
+        sequences, the tables are written to that step's tensors, whose addresses a graph holds; the step that had them last may
+        not be used any more either.  ValueError, and nothing
         changed, when a sequence has more pages than that table is wide."""
         book = self._book
         sequences, counts = list(sequences), [counts] * len(sequences) if type(counts) is int else list(counts)
         if type(width) is not int or width < 0:
             raise ValueError("width must be a non-negative integer")
         if reuse is not None:
-            if not isinstance(reuse, PagedStep) or reuse.table.device != self.device or reuse.table.shape[0] != len(sequences):
+            if not isinstance(reuse, PagedStep) or reuse._tables.book is not book or reuse.table.shape[0] != len(sequences):
                 raise ValueError("reuse must be a step of this cache with as many sequences")
             if type(counts) is list and all(type(c) is int for c in counts) and len(counts) == len(sequences):
                 most = max((-(-(book.of(q).length + c) // PAGE_TOKENS) for q, c in zip(sequences, counts)), default=0)
@@ -125,12 +135,12 @@ class PagedInt4Cache:
         for row, e in zip(table, entries):
             row[:len(e.pages)] = e.pages
         if reuse is None:
-            there = _upload(numbers, self.device)
+            step._tables = _Tables(_upload(numbers, self.device), book)
         else:
-            there = reuse._numbers
-            there.copy_(_pinned(numbers), non_blocking=True)
-            reuse._current = False
-        step._numbers = there
+            step._tables = reuse._tables
+            step._tables.numbers.copy_(_pinned(numbers), non_blocking=True)
+        step._tables.uses += 1
+        step._use, there = step._tables.uses, step._tables.numbers
         step.cu_seqlens, step.starts, step.device_lengths = there[:n + 1], there[n + 1:2 * n + 1], there[2 * n + 1:3 * n + 1]
         step.table = there[3 * n + 1:].view(n, width)
         step._whole, step._epoch, step._current = None, book.epoch, True
@@ -159,7 +169,7 @@ class PagedInt4Cache:
     def _check(self, step: PagedStep) -> None:
         if not isinstance(step, PagedStep):
             raise TypeError(f"expected a PagedStep, got {type(step).__name__}")
-        if not step._current or step._epoch is not self._book.epoch:
+        if not step._current or step._use != step._tables.uses or step._epoch is not self._book.epoch:
             raise ValueError("the step belongs to another cache, or its sequences have been extended, forked, freed or moved since")
 
     def write(self, layer: int, step: PagedStep, key: torch.Tensor, value: torch.Tensor) -> None:

@@ -190,3 +190,28 @@ def test_constructor_checks():
             ResKVLlama(LlamaShape(**TINY), device="cpu", **kw)
     with pytest.raises(RuntimeError, match="select"):
         ResKVLlama(LlamaShape(**TINY), cache="dense", device="cpu").select([0])
+
+
+@pytest.mark.gpu
+def test_reused_tables_belong_to_the_last_step_of_this_cache():
+    from reskv_b200 import PagedInt4Cache
+
+    cache, other = (PagedInt4Cache(1, 1, 16) for _ in range(2))
+    a, b = cache.add(2), cache.add(2)
+    first = cache.extend(a, [3, 4])
+    second = cache.extend(a, [1, 1], reuse=first)
+    third = cache.extend(b, [2, 2], reuse=first)  # other sequences, over the same tensors
+    x = torch.ones(2, 1, 128, dtype=torch.float16, device="cuda")
+    for stale in (first, second):
+        with pytest.raises(ValueError, match="the step belongs"):
+            cache.write(0, stale, x, x)
+        with pytest.raises(ValueError, match="the step belongs"):
+            cache.attend(0, stale, x)
+    assert third.table.data_ptr() == first.table.data_ptr()
+    k = torch.ones(4, 1, 128, dtype=torch.float16, device="cuda")
+    cache.write(0, third, k, k)
+    assert torch.equal(cache.attend(0, third, x), x)
+    with pytest.raises(ValueError, match="reuse must be a step of this cache"):
+        other.extend(other.add(2), 1, reuse=third)
+    cache.attend(0, third, x)  # and nothing changed
+    cache.check()
