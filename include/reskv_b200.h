@@ -448,8 +448,8 @@ int reskv_kmeans_incremental(const void* x, int batch, int kv_heads, int tokens,
  *   q            f16 (bf16 != 0: bf16) [total, q_heads, 128], k and v [total, kv_heads, 128]; rows of 128
  *                dense, *_token / *_head elements between tokens / heads (positive multiples of 8), on
  *                16-byte boundaries
- *   cu_seqlens   i32 [sequences + 1] in device memory: sequence s holds tokens [cu[s], cu[s+1]); clamped to
- *                [0, total], lengths may be 0
+ *   cu_seqlens   i32 [sequences + 1] in device memory, non-decreasing: sequence s holds tokens
+ *                [cu[s], cu[s+1]); clamped to [0, total], lengths may be 0
  *   out          [total, q_heads, 128] of the same type, 32-byte aligned, lse f32 [total, q_heads] or NULL:
  *                log of the sum of exponentials.  Rows of no sequence are left as they are.
  * reskv_prompt_attention_status: RESKV_STATUS_* bits of all calls on the device so far (copies four bytes

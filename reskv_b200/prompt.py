@@ -27,8 +27,8 @@ def prompt_attention(
 
     ``query`` is FP16 or BF16 ``[T,H,128]``, ``key`` and ``value`` ``[T,KH,128]`` of the same type, ``H`` a multiple of
     ``KH`` (query head ``h`` reads KV head ``h // (H / KH)``; at most 128 per KV head); views of a fused projection are read
-    where they lie.  ``cu_seqlens`` is int32 ``[n+1]`` on the same device: sequence ``i`` holds the tokens
-    ``[cu_seqlens[i], cu_seqlens[i+1])``; lengths may be 0, bounds are clamped to ``[0, T]``.  ``scaling`` (positive) defaults
+    where they lie.  ``cu_seqlens`` is int32 ``[n+1]`` on the same device, non-decreasing: sequence ``i`` holds
+    the tokens ``[cu_seqlens[i], cu_seqlens[i+1])``; lengths may be 0, bounds are clamped to ``[0, T]``.  ``scaling`` (positive) defaults
     to ``128**-0.5``.
 
     Returns ``[T,H,128]`` of the query's type, written to ``out`` if that is given (contiguous, not overlapping the inputs);
