@@ -26,6 +26,8 @@
 //   two threads per row (16 softmax warps): 502 us
 //   the wait for the product in front behind all exponentials: 490 us; one lane polling for its warp: 490 us
 //   descriptors that the compiler does not see as uniform: 550 us for 463; the products issued from a loop in one thread: 512 us
+//   a fourth warpgroup that stores the outputs while the others go on: 458 us, seven ragged prompts 95 us for 96; the row tiles' warps of
+//   an SM quarter taking turns at the exponentials: 472 us
 //   outputs stored by row, 16 bytes a lane, instead of by lines: seven ragged prompts 106 us for 100
 #include "pairs.cuh"
 #include "tensor_map.cuh"
@@ -41,8 +43,8 @@ constexpr int kPQHalf = 128 * 128, kPQTile = 2 * kPQHalf;        // bytes of 128
 constexpr int kPKHalf = kPKeys * 128, kPKTile = 2 * kPKHalf;     // the same of a tile of keys or values
 constexpr int kPStages = 8;                     // ring of K and V tiles
 constexpr int kPThreads = 384;                  // two softmax warpgroups; a warp each for scores, outputs and copies, one idle
-// A row of scores is 128 registers of its thread.  The launch gives 168 a thread (the most for 384); the last warpgroup hands
-// back what the softmax warpgroups take: 2 x 208 + 88 = 3 x 168.
+// A row of scores and what becomes of it take more than the 168 registers that the launch gives a thread (the most for 384); the last
+// warpgroup hands back what the softmax warpgroups take: 2 x 208 + 88 = 3 x 168.
 constexpr int kPLaunchRegs = 168, kPSoftmaxRegs = 208, kPOtherRegs = 88;
 static_assert(2 * kPSoftmaxRegs + kPOtherRegs <= 3 * kPLaunchRegs, "the shares come out of the launch's registers");
 constexpr int kPSmem = 2 * kPQTile + kPStages * kPKTile + 1024;  // + room to start on a 1024-byte boundary
