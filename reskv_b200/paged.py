@@ -39,6 +39,7 @@ class PagedStep:
     def _everything(self):
         """``(cu_seqlens, starts, tokens)`` of all tokens of the sequences, the earlier ones included."""
         if self._whole is None:
+            _refuse_capture()
             ends = np.concatenate(([0], np.cumsum(self.lengths)))
             if ends[-1] > 2**31 - 1:
                 raise ValueError("too many tokens for one call")
@@ -53,6 +54,11 @@ class _Tables:
 
     def __init__(self, numbers, book):
         self.numbers, self.book, self.uses = numbers, book, 0
+
+
+def _refuse_capture() -> None:
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a step's tables come from the host: make them outside of the capture (extend(reuse=) fills those of a captured step)")
 
 
 def _pinned(numbers: np.ndarray) -> torch.Tensor:
@@ -110,6 +116,7 @@ class PagedInt4Cache:
         sequences, the tables are written to that step's tensors, whose addresses a graph holds; the step that had them last may
         not be used any more either.  ValueError, and nothing
         changed, when a sequence has more pages than that table is wide."""
+        _refuse_capture()
         book = self._book
         sequences, counts = list(sequences), [counts] * len(sequences) if type(counts) is int else list(counts)
         if type(width) is not int or width < 0:
@@ -175,7 +182,7 @@ class PagedInt4Cache:
     def write(self, layer: int, step: PagedStep, key: torch.Tensor, value: torch.Tensor) -> None:
         """Stores the step's new tokens: ``key`` (after RoPE) and ``value`` ``[step.total, KV heads, 128]`` of the cache's type."""
         self._check(step)
-        if key.dtype != self.dtype or key.shape[0] != step.total:
+        if isinstance(key, torch.Tensor) and (key.dtype != self.dtype or key.shape[:1] != (step.total,)):
             raise ValueError(f"key and value must hold the step's {step.total} tokens in {self.dtype}")
         host().paged_write(self.pages, layer, self._status, key, value, step.cu_seqlens, step.starts, step.table)
 
@@ -192,7 +199,7 @@ class PagedInt4Cache:
         ``return_lse`` also FP32 ``[sequences, H]``, the logarithm of the sum of exponentials.  A sequence without tokens gets
         zeros (and minus infinity)."""
         self._check(step)
-        if query.dtype != self.dtype:
+        if isinstance(query, torch.Tensor) and query.dtype != self.dtype:
             raise ValueError(f"query must be {self.dtype}")
         return host().paged_attention(self.pages, layer, self._status, query, step.device_lengths, step.table, scaling, bool(return_lse))
 

@@ -543,3 +543,41 @@ def test_long_sequences_and_a_pool_beyond_four_gigabytes():
     assert_attends(cache, seqs, [k], [v], 2)
     cache.copy_pages([cache._book.of(target).pages[0]], [0])
     assert torch.equal(cache.pages[0, 0], cache.pages[0, cache._book.of(target).pages[0]])
+
+
+@pytest.mark.gpu
+def test_tables_are_not_made_in_a_capture():
+    """A captured copy would read host memory that belongs to somebody else by the time of a replay."""
+    cache = PagedInt4Cache(1, 1, 4)
+    seqs, _, _ = fill(cache, [5, 70])
+    step = cache.extend(seqs, 1)
+    x = torch.zeros(2, 1, 128, dtype=torch.float16, device=DEV)
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    cache.write(0, step, x, x)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        graph.capture_begin()
+        try:
+            with pytest.raises(RuntimeError, match="outside of the capture"):
+                cache.extend(seqs, 1)
+            with pytest.raises(RuntimeError, match="outside of the capture"):
+                cache.read(0, step, everything=True)
+            out = cache.attend(0, step, x)
+        finally:
+            graph.capture_end()
+    assert cache.length(seqs[0]) == 6
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, cache.attend(0, step, x))
+
+
+@pytest.mark.gpu
+def test_what_is_no_tensor_is_refused():
+    cache = PagedInt4Cache(1, 1, 4)
+    step = cache.extend(cache.add(1), 1)
+    x = torch.zeros(1, 1, 128, dtype=torch.float16, device=DEV)
+    for call in (lambda: cache.write(0, step, None, x), lambda: cache.write(0, step, x, 1.0), lambda: cache.attend(0, step, [1])):
+        with pytest.raises(TypeError):
+            call()
+    with pytest.raises(ValueError):
+        cache.write(0, step, x[0, 0, 0], x)
