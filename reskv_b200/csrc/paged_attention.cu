@@ -40,7 +40,7 @@ constexpr int kPaMergeWarps = 16;                 // of a query head at most
 constexpr int kPaSumBytes = kPaWarps * kPagedGroup * kHeadDim * 4;
 constexpr int kPaSmem = kPaWarps * kPaStages * kChunkBytes + kPaSumBytes;
 constexpr float kCodeMiddle = 8.f;
-constexpr uint32_t kMiddleLow = 0x80088008u, kMiddleHigh = 0x80808080u;  // pairs of -8 * 2^-24 and -8 * 2^-20
+constexpr uint32_t kMiddleLow = 0x80088008u, kMiddleByte = 0x80888088u;  // pairs of -8 * 2^-24 and -(8 + 16 * 8) * 2^-24
 constexpr int kPaSlack = 5;
 constexpr int kPartialFloats = kPagedGroup * (kHeadDim + 2);  // of a part: outputs [8][128], maxima [8], sums [8]
 
@@ -502,10 +502,10 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
 #pragma unroll
                 for (int group = 0; group < 2; ++group) {
                     if (b == 0)
-                        mma_16816_start(eights[group], kMiddleLow, kMiddleHigh, kMiddleLow, kMiddleHigh, weights[group][0], weights[group][1]);
+                        mma_16816_start(eights[group], kMiddleLow, kMiddleByte, kMiddleLow, kMiddleByte, weights[group][0], weights[group][1]);
                     else
-                        mma_16816(eights[group], kMiddleLow, kMiddleHigh, kMiddleLow, kMiddleHigh, weights[group][0], weights[group][1]);
-                    if (kTwice) mma_16816(eights[group], kMiddleLow, kMiddleHigh, kMiddleLow, kMiddleHigh, rest[group][0], rest[group][1]);
+                        mma_16816(eights[group], kMiddleLow, kMiddleByte, kMiddleLow, kMiddleByte, weights[group][0], weights[group][1]);
+                    if (kTwice) mma_16816(eights[group], kMiddleLow, kMiddleByte, kMiddleLow, kMiddleByte, rest[group][0], rest[group][1]);
                 }
                 uint2 rows[4];
 #pragma unroll
@@ -518,11 +518,11 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {  // bytes 0, 1 and 2, 3 of the words
                         const uint32_t pick = half ? 0x7632u : 0x5410u;
-                        const uint32_t x = __byte_perm(group ? rows[0].y : rows[0].x, group ? rows[1].y : rows[1].x, pick), x8 = x >> 8;
-                        const uint32_t y = __byte_perm(group ? rows[2].y : rows[2].x, group ? rows[3].y : rows[3].x, pick), y8 = y >> 8;
+                        const uint32_t x = __byte_perm(group ? rows[0].y : rows[0].x, group ? rows[1].y : rows[1].x, pick), x8 = __byte_perm(x, 0, 0x4341);
+                        const uint32_t y = __byte_perm(group ? rows[2].y : rows[2].x, group ? rows[3].y : rows[3].x, pick), y8 = __byte_perm(y, 0, 0x4341);
                         const auto add = [&](const uint32_t(&w)[2]) {
-                            mma_16816(acc[group * 4 + half * 2], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, w[0], w[1]);
-                            mma_16816(acc[group * 4 + half * 2 + 1], x8 & 0x000F000Fu, x8 & 0x00F000F0u, y8 & 0x000F000Fu, y8 & 0x00F000F0u, w[0], w[1]);
+                            mma_16816(acc[group * 4 + half * 2], x & 0x000F000Fu, x & 0x00FF00FFu, y & 0x000F000Fu, y & 0x00FF00FFu, w[0], w[1]);
+                            mma_16816(acc[group * 4 + half * 2 + 1], x8 & 0x000F000Fu, x8, y8 & 0x000F000Fu, y8, w[0], w[1]);
                         };
                         add(weights[group]);
                         if (kTwice) add(rest[group]);
@@ -566,13 +566,13 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
             float* mine = sums + warp * kPagedGroup * kHeadDim + 2 * t * kHeadDim;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                constexpr float low = 1 << 24, high = 1 << 20;  // of codes in the low and in the next nibbles
+                constexpr float low = 1 << 24, high = 1 << 20;  // of codes alone, and of what they leave of their bytes
                 const int d = (i >> 2) * 64 + 8 * g + (i & 3) * 2;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
                     if ((kBeside ? (2 * t + h) & 3 : 2 * t + h) < p.group)
                         *reinterpret_cast<float2*>(mine + h * kHeadDim + d) = make_float2(fmaf(acc[i][h] * low, unit, base[i >> 2][h]) * weight[h],
-                                                                                       fmaf(acc[i][2 + h] * high, unit, base[i >> 2][h]) * weight[h]);
+                                                                                       fmaf((acc[i][2 + h] - acc[i][h]) * high, unit, base[i >> 2][h]) * weight[h]);
             }
         }
         if (warp == 0 && g == 0) s_top[2 * t] = top[0], s_top[2 * t + 1] = top[1];
