@@ -248,6 +248,7 @@ struct PagePairs {
     int src[kPairsPerLaunch], dst[kPairsPerLaunch];
 };
 
+// Bound by bytes: 192 pages in 32 layers of 8 heads, 906 MB, 138 us = 6.6 TB/s, 1.02 of the copy rate.
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(unsigned char* pages, int64_t layer_bytes, int64_t page_bytes, const PagePairs pairs) {
     wait_for_previous_launch();
     let_next_launch_start();
@@ -286,10 +287,11 @@ int launch_store(const StoreParams& p, cudaStream_t stream) {
     return check_cuda(launch_overlapped(paged_store_kernel<BF16, WRITE, PASSES>, dim3(static_cast<unsigned>(blocks)), kStoreThreads, 0, stream, true, p),
                       WRITE ? "paged_write launch" : "paged_read launch");
 }
-// One pass per warp as long as that leaves SMs without a block.
+// One pass per warp up to eight blocks per SM.  us written and read with one pass and with two, 8 heads: 64 tokens 2.0 and 2.0, 2.7 and
+// 2.5; 800 tokens 2.7 and 2.7, 3.2 and 3.0; 1600 tokens 3.8 and 3.2, 3.6 and 3.4; 4546 tokens 6.4 and 5.5, 5.9 and 5.4.
 template <bool WRITE>
 int run_store(const StoreParams& p, int bf16, cudaStream_t stream) {
-    const bool many = static_cast<int64_t>(p.total) * p.heads > static_cast<int64_t>(sm_count()) * kStoreWarps * kPassRows;
+    const bool many = static_cast<int64_t>(p.total) * p.heads > 8 * static_cast<int64_t>(sm_count()) * kStoreWarps * kPassRows;
     return bf16 ? many ? launch_store<true, WRITE, kPasses>(p, stream) : launch_store<true, WRITE, 1>(p, stream)
                 : many ? launch_store<false, WRITE, kPasses>(p, stream) : launch_store<false, WRITE, 1>(p, stream);
 }
