@@ -672,12 +672,15 @@ __global__ void __launch_bounds__(1024) paged_merge_kernel(const PagedParams p, 
     if (p.lse && lane == 0) p.lse[row] = top * kLn2 + logf(total);
 }
 
+int most_shares(int sequences, int width, int heads, int least) {
+    const int64_t most = (static_cast<int64_t>(sequences) * (width + kPaCharge) * heads + least - 1) / least;
+    return static_cast<int>(std::min<int64_t>(most, kPaPerSm * sm_count()));
+}
+
 // CTAs of the first kernel for as many pages as there may be.  No more than will have a share: those without one displace others
 // (1 x 8128 tokens: 12.6 us with 296 CTAs for 135 shares, 10.2 with 135).
 int paged_ctas(int sequences, int width, int heads) {
-    if (width == 0) return 0;
-    const int64_t least = least_share(width + kPaCharge), most = (static_cast<int64_t>(sequences) * (width + kPaCharge) * heads + least - 1) / least;
-    return static_cast<int>(std::min<int64_t>(most, kPaPerSm * sm_count()));
+    return width == 0 ? 0 : most_shares(sequences, width, heads, least_share(width + kPaCharge));
 }
 
 template <bool BF16, Weights WEIGHTS>
@@ -706,7 +709,8 @@ using namespace reskv;
 
 extern "C" size_t reskv_paged_attention_workspace_bytes(int sequences, int width, int kv_heads) {
     if (sequences < 0 || width < 0 || kv_heads < 1) return 0;
-    return static_cast<size_t>(paged_ctas(sequences, width, kv_heads)) * 2 * kPartialFloats * sizeof(float) + 256;
+    // for the shortest shares, so that what is enough for a wide table is enough for a narrow one
+    return static_cast<size_t>(width == 0 ? 0 : most_shares(sequences, width, kv_heads, least_share(0))) * 2 * kPartialFloats * sizeof(float) + 256;
 }
 
 extern "C" int reskv_paged_attention(const void* q, int bf16, int64_t q_sequence, int64_t q_head, const int32_t* lengths, const int32_t* table,

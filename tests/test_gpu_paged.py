@@ -581,3 +581,14 @@ def test_what_is_no_tensor_is_refused():
             call()
     with pytest.raises(ValueError):
         cache.write(0, step, x[0, 0, 0], x)
+
+
+@pytest.mark.gpu
+def test_a_workspace_for_more_is_enough_for_less():
+    from reskv_b200._extension import library
+
+    need = library().reskv_paged_attention_workspace_bytes
+    for sequences in (1, 2, 7, 40):
+        for heads in (1, 2, 8):
+            sizes = [need(sequences, width, heads) for width in range(0, 300)]
+            assert sizes == sorted(sizes) and sizes[-1] <= need(sequences + 1, 299, heads) <= need(sequences + 1, 299, heads + 1)
