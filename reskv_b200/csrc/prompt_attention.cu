@@ -60,6 +60,7 @@ __device__ uint32_t g_prompt_status;  // RESKV_STATUS_* bits
 struct PromptParams {
     const int* cu;      // [sequences + 1]
     int sequences, total, kv_heads, group, tile_tokens;  // tile_tokens: tokens of 128 rows
+    int64_t most_single;  // items have one row tile each if there are no more than that many of them
     const unsigned short* v;      // the values once more, for the outputs that infinities and NaN reach
     int64_t v_token, v_head;      // elements between its tokens and heads
     void* out;          // [total, query heads, 128]
@@ -68,7 +69,7 @@ struct PromptParams {
     int causal;
 };
 
-// A work item: two row tiles of one sequence and KV head.
+// A work item: one or two row tiles of one sequence and KV head.
 struct PromptItem {
     int start, len, token0, head, tiles0, tiles1;  // tiles0 / tiles1: key tiles that the first / second row tile needs
 };
@@ -83,13 +84,12 @@ __device__ __forceinline__ SequenceSpan span_of(const PromptParams& p, int s) {
     return {a, b - a};
 }
 
-// Number of (sequence, pair of row tiles) whose place in the sequence is `level` or behind it; whole warp.
-__device__ __forceinline__ int pairs_from(const PromptParams& p, int level, int lane) {
-    const int pair = 2 * p.tile_tokens;
+// Number of pieces of `per` tokens of all sequences whose place in the sequence is `level` or behind it; whole warp.
+__device__ __forceinline__ int items_from(const PromptParams& p, int per, int level, int lane) {
     int n = 0;
 #pragma unroll 4
     for (int s = lane; s < p.sequences; s += 32) {
-        const int tiles = (span_of(p, s).len + pair - 1) / pair;
+        const int tiles = (span_of(p, s).len + per - 1) / per;
         n += tiles > level ? tiles - level : 0;
     }
     return __reduce_add_sync(0xffffffffu, n);
@@ -98,19 +98,23 @@ __device__ __forceinline__ int pairs_from(const PromptParams& p, int level, int 
 // Items are ordered by their place in their sequence, last ones first: with causal attention the longest ones.  The items that a CTA
 // takes come as a rule in this order, so the search for one begins at the level of the one before.
 struct ItemSearch {
-    int all, level, before, upto;  // all pairs; the level's are those from `before` to `upto`
-    __device__ __forceinline__ ItemSearch(const PromptParams& p, int lane) : all(pairs_from(p, 0, lane)), level(highest(p)), before(0), upto(0) {}
-    static __device__ __forceinline__ int highest(const PromptParams& p) { return (p.total + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens); }
+    int per, all, level, before, upto;  // tokens of an item; all pieces; the level's are those from `before` to `upto`
+    __device__ __forceinline__ ItemSearch(const PromptParams& p, int lane) : per(p.tile_tokens), all(0), before(0), upto(0) {
+        if (p.most_single) all = items_from(p, per, 0, lane);
+        if (!p.most_single || static_cast<int64_t>(all) * p.kv_heads > p.most_single) per *= 2, all = items_from(p, per, 0, lane);
+        level = highest(p);
+    }
+    __device__ __forceinline__ int highest(const PromptParams& p) const { return (p.total + per - 1) / per; }
     // Item `index`.  tiles0 = 0 in the result: there is none.  Whole warp.
     __device__ PromptItem find(const PromptParams& p, int index, int lane) {
         PromptItem it{};
-        const int pos = index / p.kv_heads, pair = 2 * p.tile_tokens;
+        const int pos = index / p.kv_heads;
         if (pos >= all) return it;
         if (pos < before) level = highest(p), before = upto = 0;
         if (pos >= upto) {
             int low = 0, high = level, from_high = upto, from_low = all;
             while (high - low > 1) {
-                const int mid = (low + high) >> 1, n = pairs_from(p, mid, lane);
+                const int mid = (low + high) >> 1, n = items_from(p, per, mid, lane);
                 if (n > pos) low = mid, from_low = n; else high = mid, from_high = n;
             }
             level = low, before = from_high, upto = from_low;
@@ -118,7 +122,7 @@ struct ItemSearch {
         int rest = pos - before;
         for (int s0 = 0; s0 < p.sequences; s0 += 32) {
             const SequenceSpan sp = s0 + lane < p.sequences ? span_of(p, s0 + lane) : SequenceSpan{0, 0};
-            const bool has = sp.len > level * pair;
+            const bool has = sp.len > level * per;
             const uint32_t mask = __ballot_sync(0xffffffffu, has);
             const int count = __popc(mask);
             if (rest >= count) {
@@ -129,8 +133,8 @@ struct ItemSearch {
             it.start = __shfl_sync(0xffffffffu, sp.start, owner);
             it.len = __shfl_sync(0xffffffffu, sp.len, owner);
             it.head = index % p.kv_heads;
-            it.token0 = level * pair;
-            const int end0 = min(it.token0 + p.tile_tokens, it.len), end1 = min(it.token0 + pair, it.len);
+            it.token0 = level * per;
+            const int end0 = min(it.token0 + p.tile_tokens, it.len), end1 = min(it.token0 + per, it.len);
             it.tiles0 = ((p.causal ? end0 : it.len) + kPKeys - 1) / kPKeys;
             it.tiles1 = end1 <= it.token0 + p.tile_tokens ? 0 : ((p.causal ? end1 : it.len) + kPKeys - 1) / kPKeys;
             return it;
@@ -620,8 +624,13 @@ extern "C" int reskv_prompt_attention(const void* q, const void* k, const void* 
     if (int rc = rows_map(&qm, q, q_heads, total, q_token, q_head, p.group, p.tile_tokens)) return rc;
     if (int rc = rows_map(&km, k, kv_heads, total, k_token, k_head, 1, kPKeys)) return rc;
     if (int rc = rows_map(&vm, v, kv_heads, total, v_token, v_head, 1, kPKeys)) return rc;
-    // every sequence has at most one pair of row tiles that is not full
-    const int64_t items = (total / (2 * p.tile_tokens) + static_cast<int64_t>(sequences < total ? sequences : total)) * kv_heads;
+    // One row tile per item where all of them find an SM of their own, which the device counts unless the tokens alone say no.  us with
+    // one and with two: 1 x 300 tokens, 32 / 8 heads 12.0 and 13.3, 1 x 512 14.5 and 16.8, five short ones 12.9 and 13.7; five of 100
+    // (160 items of one row tile, 12 of them behind others) 13.4 and 12.1.
+    const int64_t parts = sequences < total ? sequences : total;
+    p.most_single = total / p.tile_tokens * kv_heads <= sm_count() ? sm_count() : 0;
+    // every sequence has at most one item that is not full
+    const int64_t items = (total / (p.most_single ? p.tile_tokens : 2 * p.tile_tokens) + parts) * kv_heads;
     if (items > 0x7ffffffe) return fail(RESKV_ERR_LIMIT, "prompt_attention: too many tokens for one call");
     const auto st = static_cast<cudaStream_t>(stream);
     return bf16 ? launch<true>(p, qm, km, vm, static_cast<unsigned>(items), st) : launch<false>(p, qm, km, vm, static_cast<unsigned>(items), st);

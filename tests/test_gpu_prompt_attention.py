@@ -268,3 +268,54 @@ def test_two_calls_at_once():
 
     with ThreadPoolExecutor(2) as pool:
         assert list(pool.map(work, (0, 1))) == [True, True]
+
+
+# Short calls give every row tile an item of its own; with 150 further sequences there are too many for that, and items hold two.
+CROWD = [1] * 150
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lengths", [*LENGTHS, [500, 123]], ids=str)
+def test_one_and_two_row_tiles_per_item(lengths, dtype, causal):
+    q, k, v, ends, cu = inputs(lengths + CROWD, 2, 4, dtype, seed=12)
+    got, lse = prompt_attention(q, k, v, cu, causal=causal, return_lse=True)
+    want, want_lse, bound = formula(q, k, v, ends, causal=causal)
+    assert_within(got, want, bound)
+    assert (lse.double() - want_lse).abs().max().item() < 2e-3
+    few = slice(0, ends[len(lengths)])  # a row's arithmetic does not depend on what shares its item
+    alone, alone_lse = prompt_attention(q[few], k[few], v[few], cu[:len(lengths) + 1], causal=causal, return_lse=True)
+    assert torch.equal(alone, got[few]) and torch.equal(alone_lse, lse[few])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_heads,ratio", [(3, 1), (1, 3), (2, 5), (1, 12), (1, 40), (1, 128)])
+def test_head_layouts_with_two_row_tiles_per_item(kv_heads, ratio):
+    q, k, v, ends, cu = inputs([45, 200, 1] + CROWD, kv_heads, ratio, torch.float16, seed=13)
+    assert_within(prompt_attention(q, k, v, cu), *formula(q, k, v, ends)[::2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ratio", [1, 4])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_value_that_is_not_finite_with_two_row_tiles_per_item(ratio, bad):
+    q, k, v, ends, cu = inputs([200, 150] + CROWD, 2, ratio, torch.float16, seed=14)
+    clean = prompt_attention(q, k, v, cu)
+    at = 131
+    v[at, 1, 5:9] = bad
+    got = prompt_attention(q, k, v, cu)
+    own = slice(ratio, 2 * ratio)
+    seen = torch.zeros_like(got, dtype=torch.bool)
+    seen[at:200, own, 5:9] = True
+    assert torch.equal(got[~seen], clean[~seen])
+    assert (got[seen].isnan() if bad != bad else got[seen] == bad).all()
+
+
+@pytest.mark.gpu
+def test_the_number_of_items_decides_at_its_limit():
+    """As many items of one row tile as there are SMs, one less and one more: 32 tokens each."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    for n in (sms - 1, sms, sms + 1):
+        q, k, v, ends, cu = inputs([32 * 4] * (n // 4) + [32] * (n % 4), 1, 4, torch.float16, seed=n)
+        assert_within(prompt_attention(q, k, v, cu), *formula(q, k, v, ends)[::2])
