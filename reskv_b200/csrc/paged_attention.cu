@@ -7,7 +7,7 @@
 //     sum p v   = sum_j (p_j scale_j,g) (code_j,g - 8) + sum_j p_j (offset_j,g + 8 scale_j,g)
 // with p * scale in FP16 as the product's operand, for FP16 models in two parts.
 //
-// 32 x 8128 tokens, 32 / 8 heads: 71 us for 300 MB, 4.2 TB/s (0.65 of the copy rate); 77 us where none of it is in L2.  Bound by
+// 32 x 8128 tokens, 32 / 8 heads: 71 us for 300 MB, 4.2 TB/s (0.65 of the copy rate).  Bound by
 // instructions, 20 of a warp per token and KV head (issue slots 57 %, integer pipe 48 %: masks and shifts that bring the codes into
 // operands).  Small calls are bound by latency: one sequence of 300 tokens 7.0 us, of 8128 10.6 us, nine ragged BF16 ones with eight
 // query heads 16 us (28 MB), of which two dependent launches, look-ups of lengths and pages, a copy, a chunk, two meetings of the

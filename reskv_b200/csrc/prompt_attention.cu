@@ -3,10 +3,10 @@
 //
 // Both products run on tcgen05.mma.  A row tile is 128 rows: the query heads of one KV head for as many tokens as fit, so that
 // grouped heads share the keys and a short sequence still fills rows; an item is two row tiles, in short calls one.  Per tile of 80
-// keys: scores S = Q K^T into tensor memory, one thread per row forms the weights P with a running maximum (it lags by up to 2^8, so that the
-// output is rarely rescaled), and the output accumulates P V with P read from tensor memory.  A row tile's scores (80 columns)
-// and weights (40) lie side by side in 128 columns, which is why a tile has 80 keys: the next scores do not wait for the product
-// with the weights in front.  A warp issues the scores' products, another one the outputs', so neither waits for the other's
+// keys: scores S = Q K^T into tensor memory, one thread per row forms the weights P with a running maximum (it lags by up to 2^8, so
+// that the output is rarely rescaled), and the output accumulates P V with P read from tensor memory.  A row tile's scores (80
+// columns) and weights (40) lie side by side in 128 columns, which is why a tile has 80 keys: the next scores do not wait for the
+// product with the weights in front.  A warp issues the scores' products, another one the outputs', so neither waits for the other's
 // operands.  Tiles arrive by TMA through a ring of eight.
 //
 // Items are ordered by their place in their sequence, last ones first, which with causal attention are the longest; the grid has
@@ -17,11 +17,10 @@
 // infinities or NaN in rows of V that only part of a row tile sees are cleared there too and added where they are seen.
 //
 // Bound (1 x 8192 tokens, 32 / 8 heads, 550 GFLOP): 449 us = 1.22 PFLOP/s in short runs, 507 us = 1.08 PFLOP/s in long ones under
-// the power cap; seven ragged prompts of 84 GFLOP 93 us, five short ones of 0.9 GFLOP 13 us in a
-// captured row of calls.  A row tile's softmax is what
-// takes longest: 2070 cycles per tile of 80 keys, of them 1230 forming weights (16 exponentials per clock and SM, two row tiles: 1280
-// for both), 180 and 280 waiting for scores and for the product in front, 150 the maximum; per item another 1300 waiting for the
-// last product, 2300 storing, 1000 until the first scores.  What was measured besides, on 1 x 8192 in short runs:
+// the power cap; seven ragged prompts of 84 GFLOP 93 us, five short ones of 0.9 GFLOP 13 us.  A row tile's softmax is what takes
+// longest: 2070 cycles per tile of 80 keys, of them 1230 forming weights (16 exponentials per clock and SM, two row tiles: 1280 for
+// both), 180 and 280 waiting for scores and for the product in front, 150 the maximum; per item another 1300 waiting for the last
+// product, 2300 storing, 1000 until the first scores.  What was measured besides, on 1 x 8192 in short runs:
 //   128 keys a tile, weights in the scores' place, one warp for both products, ring of five: 463 us (seven ragged: 100 us)
 //   a quarter of the exponentials by a polynomial: 447 us, not worth its code; a half: no faster
 //   two threads per row (16 softmax warps): 502 us
