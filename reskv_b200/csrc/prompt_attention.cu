@@ -28,6 +28,7 @@
 //   descriptors that the compiler does not see as uniform: 550 us for 463; the products issued from a loop in one thread: 512 us
 //   a fourth warpgroup that stores the outputs while the others go on: 458 us, seven ragged prompts 95 us for 96; the row tiles' warps of
 //   an SM quarter taking turns at the exponentials: 472 us
+//   the product begun with the weights of the first 16, 32 or 48 keys of a tile: no faster, seven ragged prompts 96 us for 94
 //   outputs stored by row, 16 bytes a lane, instead of by lines: seven ragged prompts 106 us for 100
 #include "pairs.cuh"
 #include "tensor_map.cuh"
