@@ -211,11 +211,13 @@ struct Requests {
     const unsigned char* at[kPaStages];
 };
 
-// The warp's next segment, in shared memory; whole warp.
+// The warp's next segment, in shared memory; whole warp.  The first barrier keeps the record until every lane has read it, the second
+// puts lane 0's stores before the other lanes' loads: an exchange between lanes alone orders no memory.
 __device__ __forceinline__ bool next_segment(const PagedParams& p, Segments& at, int lane) {
     bool any = false;
     __syncwarp();
     if (lane == 0) any = at.next(p);
+    __syncwarp();
     return __shfl_sync(0xffffffffu, any, 0);
 }
 

@@ -592,3 +592,18 @@ def test_a_workspace_for_more_is_enough_for_less():
         for heads in (1, 2, 8):
             sizes = [need(sequences, width, heads) for width in range(0, 300)]
             assert sizes == sorted(sizes) and sizes[-1] <= need(sequences + 1, 299, heads) <= need(sequences + 1, 299, heads + 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_shares_of_several_segments_have_the_same_bits_every_time(dtype):
+    """Shares that hold several units, each one or two pages long: every lane of a warp has to see the segment that the
+    warp has gone on to.  Against the formula, and the same bits in every call."""
+    lengths = [1 + (53 * i) % 128 for i in range(250)]
+    cache = PagedInt4Cache(1, 3, sum(-(-t // 64) for t in lengths), dtype=dtype)
+    seqs, k, v = fill(cache, lengths, seed=43)
+    first = assert_attends(cache, seqs, k, v, 3, seed=44)
+    step = cache.extend(seqs, 0)
+    q = torch.randn(250, 9, 128, generator=torch.Generator(device=DEV).manual_seed(44), device=DEV).to(dtype)
+    for _ in range(30):
+        assert torch.equal(cache.attend(0, step, q), first)
