@@ -55,6 +55,7 @@ __host__ __device__ constexpr uint32_t weight_column(int i) { return i * 128 + k
 __host__ __device__ constexpr uint32_t output_column(int i) { return 256 + i * 128; }
 static_assert(kPKeys + kPKeys / 2 <= 128 && kPKeys % 16 == 0, "scores and weights of a row tile share 128 columns");
 constexpr float kPSlack = 8.f;                  // the running maximum lags by at most this (in powers of two)
+constexpr float kPLowest = -0x1.ffffp127f;      // the running maximum of a row whose scores have all been -infinity
 
 __device__ uint32_t g_prompt_status;  // RESKV_STATUS_* bits
 
@@ -411,6 +412,8 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
         const uint32_t s_at = tmem + lanes + score_column(i), p_at = tmem + lanes + weight_column(i), o_at = tmem + lanes + output_column(i);
         const int row_token = row / p.group, row_head = row - row_token * p.group;
         const float scale = p.scale_log2, slack = kPSlack / scale;
+        // Finite, and finite times `scale`: scores of -infinity less it have weights of 0, and what comes later finds a sum of 0, no NaN.
+        const float lowest = scale > 1.f ? kPLowest / scale : kPLowest;
         const auto arrive = [&](uint64_t* bar) {  // of the warp, behind its reads and writes of tensor memory
             tc_fence_before();
             __syncwarp();
@@ -459,7 +462,7 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                 }
                 ++seen;
                 if (j == 0) {
-                    m = most;
+                    m = max_nan(most, lowest);
                 } else {
                     const bool grows = !(most <= m + slack);
                     if (__any_sync(0xffffffffu, grows)) {

@@ -319,3 +319,31 @@ def test_the_number_of_items_decides_at_its_limit():
     for n in (sms - 1, sms, sms + 1):
         q, k, v, ends, cu = inputs([32 * 4] * (n // 4) + [32] * (n % 4), 1, 4, torch.float16, seed=n)
         assert_within(prompt_attention(q, k, v, cu), *formula(q, k, v, ends)[::2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,bad", [(torch.float16, "infinite"), (torch.bfloat16, "infinite"), (torch.bfloat16, "overflow")])
+@pytest.mark.parametrize("crowd", [[], CROWD], ids=["few", "many"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("scaling", [128**-0.5, 4.0])
+@pytest.mark.parametrize("at", [79, 80, 160, 230])
+def test_leading_keys_whose_scores_are_minus_infinity(at, scaling, dtype, causal, crowd, bad):
+    """The first ``at`` keys of a sequence have scores of -inf for all of its queries: their weights are 0, and every row that sees a
+    later key has what the sequence without them has.  A row that sees nothing else: no weights, NaN and a sum of 0."""
+    q, k, v, ends, cu = inputs([33, 2 * at] + crowd, 2, 4, dtype, seed=15)
+    clean = prompt_attention(q, k, v, cu, scaling=scaling, causal=causal)
+    a, b = ends[1], ends[2]
+    q[a:b, 4:, 7] = 2 + q[a:b, 4:, 7].abs()
+    k[a:a + at, 1, 7] = -torch.inf if bad == "infinite" else -torch.finfo(dtype).max
+    got, lse = prompt_attention(q, k, v, cu, scaling=scaling, causal=causal, return_lse=True)
+    assert torch.equal(got[:, :4], clean[:, :4]) and torch.equal(got[:a], clean[:a]) and torch.equal(got[b:], clean[b:])
+    for first in (a, a + at):  # two halves of as many rows
+        rows = slice(first, first + at)
+        if first == a and causal:
+            if bad == "infinite":
+                assert got[rows, 4:].isnan().all() and (lse[rows, 4:] == -torch.inf).all()
+            continue
+        want, want_lse, bound = formula(q[rows, 4:], k[a + at:b, 1:], v[a + at:b, 1:], [0, at], scaling=scaling, causal=causal)
+        assert_within(got[rows, 4:], want, bound)
+        # a score is off by less than 128 * 2^-23 * sum|q k| * scaling (sum|q k| < 600), the sum of exponentials by 2^-13
+        assert (lse[rows, 4:].double() - want_lse).abs().max().item() < 2e-3 + 0.01 * scaling
