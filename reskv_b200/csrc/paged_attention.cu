@@ -364,7 +364,10 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
         // Of heads 2t and 2t + 1, over the lane's tokens: sums of p and per group of p * middle.  They and the outputs are in units of
         // 2^-unit_up, which keeps p * scale where FP16 is exact to half a step.
         // m may lag behind the maximum by kPaSlack powers of two: fewer rescalings.
-        float shift[2] = {INFINITY, INFINITY};  // unit_up - m * q_scale
+        // It starts at the lowest finite number: scores of -infinity (BF16 offsets so large that their products leave FP32) have weights
+        // of 0 then, where a maximum of -infinity would make them NaN.
+        constexpr float kNone = 3.402823466e38f;
+        float shift[2] = {kNone, kNone};  // unit_up - m * q_scale
         float unit_up = 0.f, unit_limit = -1.f;
         float2 l = make_float2(0.f, 0.f), flat[2] = {l, l};
         float acc[8][4];  // rows = coordinates, columns = heads 2t, 2t + 1

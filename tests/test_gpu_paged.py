@@ -607,3 +607,25 @@ def test_shares_of_several_segments_have_the_same_bits_every_time(dtype):
     q = torch.randn(250, 9, 128, generator=torch.Generator(device=DEV).manual_seed(44), device=DEV).to(dtype)
     for _ in range(30):
         assert torch.equal(cache.attend(0, step, q), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths", [[40, 90], [600, 33], [5000]], ids=str)
+def test_keys_whose_scores_overflow_to_minus_infinity(lengths):
+    """BF16 keys so large that their products leave FP32: where these are the first ones of a warp or of a share, the later ones have
+    the weights that they have alone."""
+    cache = PagedInt4Cache(1, 2, 100, dtype=torch.bfloat16)
+    seqs = cache.add(len(lengths))
+    k = [vectors(t, 2, torch.bfloat16, 80 + i) for i, t in enumerate(lengths)]
+    v = [vectors(t, 2, torch.bfloat16, 90 + i) for i, t in enumerate(lengths)]
+    for x in k:
+        x[:len(x) - 7, 1] = -1e38
+    cache.write(0, cache.extend(seqs, lengths), torch.cat(k), torch.cat(v))
+    q = vectors(len(lengths), 8, torch.bfloat16, 99).abs() + 1
+    got, lse = cache.attend(0, cache.extend(seqs, 0), q, return_lse=True)
+    for i in range(len(lengths)):
+        for heads, keys in ((slice(0, 4), slice(None)), (slice(4, 8), slice(-7, None))):
+            g = slice(heads.start // 4, heads.start // 4 + 1)
+            want, want_lse, bound = formula(q[i, heads], k[i][keys, g], v[i][keys, g])
+            assert ((got[i, heads].double() - want).abs() <= bound).all()
+            assert (lse[i, heads].double() - want_lse).abs().max() < 1e-3
