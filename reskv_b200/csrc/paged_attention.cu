@@ -357,7 +357,9 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
                 if (t == part) q_sums = pair;
                 sum[0] -= low_of<BF16>(pair), sum[1] -= high_of<BF16>(pair);
             }
-            const float mine = 4.f * p.scale_log2 / by;
+            // not below the normal numbers, which leave scores as good as 0: a factor of 0 (a query of zeros, a tiny scaling) would make
+            // masked scores NaN
+            const float mine = fmaxf(4.f * p.scale_log2 / by, 0x1p-126f);
             q_scale[0] = __shfl_sync(0xffffffffu, mine, 8 * t), q_scale[1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
         }
 

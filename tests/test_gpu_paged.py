@@ -629,3 +629,19 @@ def test_keys_whose_scores_overflow_to_minus_infinity(lengths):
             want, want_lse, bound = formula(q[i, heads], k[i][keys, g], v[i][keys, g])
             assert ((got[i, heads].double() - want).abs() <= bound).all()
             assert (lse[i, heads].double() - want_lse).abs().max() < 1e-3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scaling", [1e-12, 1e-20, 1e-37])
+def test_queries_of_zeros_with_a_tiny_scaling(dtype, scaling):
+    """All scores are 0: the mean of the values, whatever factor the scores are brought to."""
+    cache = PagedInt4Cache(1, 2, 20, dtype=dtype)
+    seqs, k, v = fill(cache, [40, 300], seed=47)
+    q = torch.zeros(2, 8, 128, dtype=dtype, device=DEV)
+    q[:, 4:] = vectors(2, 4, dtype, 48)  # scores that are as good as 0
+    got, lse = cache.attend(0, cache.extend(seqs, 0), q, scaling=scaling, return_lse=True)
+    for i in range(2):
+        want, want_lse, bound = formula(q[i], k[i], v[i], scaling)
+        assert ((got[i].double() - want).abs() <= bound).all()
+        assert (lse[i].double() - want_lse).abs().max() < 1e-3
