@@ -209,6 +209,7 @@ struct Requests {
     int chunks;                 // left to look up of the segment (-1: none at all)
     int page[kPaStages];        // looked up: pages, and `base` (null: there is no further chunk)
     const unsigned char* at[kPaStages];
+    int stage, phase;           // of the wait that ran out
 };
 
 // The warp's next segment, in shared memory; whole warp.  The first barrier keeps the record until every lane has read it, the second
@@ -378,7 +379,14 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
         const int end = at.last_chunk(), start = at.first_chunk() + warp;
         int tokens = at.length - start * kChunkTokens;  // from this chunk on
         for (int chunks = end - start; chunks > 0; chunks -= kPaWarps, tokens -= kPaWarps * kChunkTokens) {
-            if (!lost) lost = !mbar_wait(&bar_full[warp][stage], phase);
+            if (!lost && !mbar_wait(&bar_full[warp][stage], phase)) {
+                lost = true;
+                if (lane == 0) {  // nothing more is asked for: a stage whose copy has not arrived must not be armed again
+#pragma unroll
+                    for (int s = 0; s < kPaStages; ++s) ahead.at[s] = nullptr;
+                    ahead.stage = stage, ahead.phase = phase;
+                }
+            }
             unsigned char* const chunk = ring + stage * kChunkBytes;
             // ---- scores: rows = tokens g, g + 8 of a block, columns = heads: (scale . (q . code) 2^22 + offset . sum(q) / 4) * q_scale ----
             float s[kChunkBlocks][4];
@@ -614,9 +622,11 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
         // the next segment's sums and s_top are written behind its first barrier
         first_segment = false;
     }
-    if (lost) {  // no copy may land after the block's end
-        for (int s = 0; s < kPaStages; ++s) mbar_wait(&bar_full[warp][s], s < stage ? phase ^ 1 : phase);
-        if (lane == 0) atomicOr(p.status, RESKV_STATUS_WAIT_TIMEOUT);
+    if (lost && lane == 0) {  // no copy may land after the block's end: those from the lost one on, once round the ring
+#pragma unroll 1
+        for (int s = 0; s < kPaStages; ++s) mbar_wait(&bar_full[warp][s], s < ahead.stage ? ahead.phase ^ 1 : ahead.phase);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        atomicOr(p.status, RESKV_STATUS_WAIT_TIMEOUT);
     }
 }
 
