@@ -199,6 +199,12 @@ __device__ __forceinline__ bool wait_once(bool& lost, uint64_t* bar, uint32_t pa
     return !lost;
 }
 
+// The same for a warp whose lanes have to agree on it, because they go on by what it says.
+__device__ __forceinline__ void wait_together(bool& lost, uint64_t* bar, uint32_t parity) {
+    wait_once(lost, bar, parity);
+    lost = __any_sync(0xffffffffu, lost);
+}
+
 // Whether the next item has been posted: every warp waits for that whether it has lost a wait before or not, and longer than for all
 // else together, so that the warps leave together.
 __device__ __forceinline__ bool item_posted(uint64_t* bar, uint32_t parity) {
@@ -220,9 +226,9 @@ __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_or_syn
 
 // The loop of a warp that issues products: items, key tiles, row tiles.  `first`: place of the first tile of keys (0) or of values
 // (1) in the ring.  begin(n) before item n, product(i, j, stage, issues) for row tile i and key tile j, end(issues) behind an item;
-// the commands themselves are for the one lane for which `issues` holds.
+// the commands themselves are for the one lane for which `issues` holds.  Returns the number of items.
 template <class Begin, class Product, class End>
-__device__ __forceinline__ void for_key_tiles(PromptShared& sh, bool& lost, int lane, uint32_t first, Begin begin, Product product, End end) {
+__device__ __forceinline__ int for_key_tiles(PromptShared& sh, bool& lost, int lane, uint32_t first, Begin begin, Product product, End end) {
     const bool issues = elect_one();
     uint32_t stage = first, parity = 0, last_stage = 0, last_parity = 0;
     int n = 0;
@@ -250,7 +256,9 @@ __device__ __forceinline__ void for_key_tiles(PromptShared& sh, bool& lost, int 
         end(issues);
         __syncwarp();
     }
-    if (n > 0) wait_once(lost, &sh.kv_empty[last_stage], last_parity);  // the last commits have arrived before the block ends
+    // the last commits have arrived before the block ends, whether a wait has run out before or not
+    if (n > 0) lost |= !mbar_wait(&sh.kv_empty[last_stage], last_parity);
+    return n;
 }
 
 template <bool BF16>
@@ -294,7 +302,7 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
             for (int n = 0;; ++n) {
                 const int slot = n & 1;
                 const PromptItem it = search.find(p, index, lane);
-                if (n >= 2) wait_once(lost, &sh.item_empty[slot], ((n >> 1) - 1) & 1);
+                if (n >= 2) wait_together(lost, &sh.item_empty[slot], ((n >> 1) - 1) & 1);
                 if (lane == 0) {
                     sh.item[slot] = it;
                     if (lost) sh.item[slot].tiles0 = 0;
@@ -312,7 +320,7 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                 }
                 for (int j = 0; j < 2 * kv_tiles; ++j, ++tile) {
                     const int stage = tile % kPStages;
-                    if (tile >= kPStages) wait_once(lost, &sh.kv_empty[stage], (tile / kPStages - 1) & 1);
+                    if (tile >= kPStages) wait_together(lost, &sh.kv_empty[stage], (tile / kPStages - 1) & 1);
                     if (lost) break;
                     if (lane == 0) {
                         mbar_arrive_expect_tx(&sh.kv_full[stage], kPKTile);
@@ -323,7 +331,7 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                     __syncwarp();
                     if (j > 0) continue;
                     // the first keys are on their way before the query tiles of the item in front are given back
-                    if (n > 0) wait_once(lost, &sh.q_empty, (n - 1) & 1);
+                    if (n > 0) wait_together(lost, &sh.q_empty, (n - 1) & 1);
                     if (lost) {
                         ++tile;
                         break;
@@ -338,7 +346,8 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                     }
                     __syncwarp();
                 }
-                wait_once(lost, &sh.cancel, n & 1);
+                // the reply is a write to shared memory like the copies: it is awaited whether another wait has run out or not
+                lost |= !__all_sync(0xffffffffu, mbar_wait(&sh.cancel, n & 1));
                 uint32_t taken, first;
                 asm volatile(
                     "{\n\t.reg .b128 reply;\n\t.reg .pred p;\n\t"
@@ -363,7 +372,7 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
             const UmmaDesc q0 = umma_desc_halves(smem_u32(qs), 16, 1024), k0 = umma_desc_halves(smem_u32(ring), 16, 1024);
             const uint32_t columns = uniform(tmem);
             uint32_t made[2] = {0, 0};
-            for_key_tiles(
+            const int items = for_key_tiles(
                 sh, lost, lane, 0,
                 [&](int n) { wait_once(lost, &sh.q_full, n & 1); },
                 [&](int i, int, uint32_t stage, bool issues) {
@@ -382,6 +391,7 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                 [&](bool issues) {
                     if (issues) umma_commit(&sh.q_empty);
                 });
+            if (items > 0) lost |= !mbar_wait(&sh.q_empty, (items - 1) & 1);  // of the last item, which nobody else waits for
         } else if (warp == 10) {
             // ---- outputs, as soon as weights are there ----------------------------------------------------------------------------
             constexpr uint32_t idesc = umma_idesc(128, false, true, BF16);
@@ -426,7 +436,7 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
             const bool posted = item_posted(&sh.item_full[slot], (n >> 1) & 1);
             const PromptItem it = sh.item[slot];
             lost |= !posted;
-            if (it.tiles0 == 0 || !posted) break;
+            if (it.tiles0 == 0 || __any_sync(0xffffffffu, !posted)) break;
             const int tiles = i ? it.tiles1 : it.tiles0, other = i ? it.tiles0 : it.tiles1;
             const int first_token = it.token0 + i * p.tile_tokens, token = first_token + row_token;
             const int limit = p.causal ? token : it.len - 1;  // last key that the row sees
