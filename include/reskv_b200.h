@@ -452,12 +452,17 @@ int reskv_kmeans_incremental(const void* x, int batch, int kv_heads, int tokens,
  *                [cu[s], cu[s+1]); clamped to [0, total], lengths may be 0
  *   out          [total, q_heads, 128] of the same type, 32-byte aligned, lse f32 [total, q_heads] or NULL:
  *                log of the sum of exponentials.  Rows of no sequence are left as they are.
- * reskv_prompt_attention_status: RESKV_STATUS_* bits of all calls on the device so far (copies four bytes
- * to the host and synchronises `stream`). */
+ * reskv_prompt_attention_reporting: the same call with a u32 in device memory that gets its RESKV_STATUS_* bits (a
+ * bounded wait that ran out: some rows were not written).  NULL, and the shorter call: a word of the device, which
+ * reskv_prompt_attention_status copies to the host (bits of all such calls so far; synchronises `stream`). */
 int reskv_prompt_attention(const void* q, const void* k, const void* v, const int32_t* cu_seqlens, int sequences, int total,
                            int kv_heads, int q_heads, int bf16, int64_t q_token, int64_t q_head, int64_t k_token,
                            int64_t k_head, int64_t v_token, int64_t v_head, float scaling, int causal, void* out, float* lse,
                            void* stream);
+int reskv_prompt_attention_reporting(const void* q, const void* k, const void* v, const int32_t* cu_seqlens, int sequences,
+                                     int total, int kv_heads, int q_heads, int bf16, int64_t q_token, int64_t q_head,
+                                     int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, float scaling, int causal,
+                                     void* out, float* lse, uint32_t* status, void* stream);
 int reskv_prompt_attention_status(uint32_t* status, void* stream);
 
 /* ---- 4-bit paged cache ------------------------------------------------------------------------

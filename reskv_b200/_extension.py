@@ -87,6 +87,7 @@ SIGNATURES = {
     "reskv_encode_tiled_fp16": (_I, [_P, _P, _P, _I, _I, _I, _L, _I, _I, _I, _P, _P, _L, _P]),
     "reskv_encode_structured_int4": (_I, [_P, _P, _P, _I, _I, _I, _L, _I, _P, _P, _P, _L, _P]),
     "reskv_prompt_attention": (_I, [_P] * 4 + [_I] * 5 + [_L] * 6 + [_F, _I, _P, _P, _P]),
+    "reskv_prompt_attention_reporting": (_I, [_P] * 4 + [_I] * 5 + [_L] * 6 + [_F, _I, _P, _P, _P, _P]),
     "reskv_prompt_attention_status": (_I, [_P, _P]),
     "reskv_paged_write": (_I, [_P, _P, _I] + [_L] * 4 + [_P] * 3 + [_I] * 4 + [_P, _I, _P, _P]),
     "reskv_paged_read": (_I, [_P, _P, _I] + [_P] * 3 + [_I] * 4 + [_P, _I, _P, _P]),

@@ -825,6 +825,23 @@ void refuse_gradients(std::initializer_list<at::Tensor> all, const char* who) {
         if (t.defined() && t.requires_grad()) value_error(std::string(who) + " is inference only: call it under torch.no_grad()");
 }
 
+// Whether a call waits for its kernels and looks at their status word: asked for, and not while the stream is captured.
+bool look_at_status(cudaStream_t stream) {
+    if (!g_check_status) return false;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    check_cuda(cudaStreamIsCapturing(stream, &capture), "cudaStreamIsCapturing");
+    return capture == cudaStreamCaptureStatusNone;
+}
+void raise_on_status(const uint32_t* word, cudaStream_t stream, const char* who) {
+    uint32_t status = 0;
+    check_cuda(cudaMemcpyAsync(&status, word, sizeof(status), cudaMemcpyDeviceToHost, stream), "status copy");
+    check_cuda(cudaStreamSynchronize(stream), "status synchronize");
+    if (!status) return;
+    char text[80];
+    std::snprintf(text, sizeof(text), "%s: device status 0x%x", who, status);
+    throw Failure{PyExc_RuntimeError, text};
+}
+
 // ---- packed prompts ---------------------------------------------------------------------------------------------------
 // x[T,H,128] as the kernels read it: dense rows, strides of whole 16-byte pieces.  Anything else is copied.
 at::Tensor packed_rows(const at::Tensor& x) {
@@ -835,15 +852,15 @@ at::Tensor packed_rows(const at::Tensor& x) {
 int64_t token_step(const at::Tensor& x) { return x.size(0) == 1 ? x.size(1) * 128 : x.stride(0); }
 int64_t head_step(const at::Tensor& x) { return x.size(1) == 1 ? 128 : x.stride(1); }
 
-// prompt_attention(query, key, value, cu_seqlens, scaling, causal, out, return_lse) -> out or (out, lse)
+// prompt_attention(query, key, value, cu_seqlens, scaling, causal, out, return_lse, status) -> out or (out, lse)
 PyObject* py_prompt_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        expect(n, 8);
+        expect(n, 9);
         at::Tensor x[3] = {tensor(o[0], "query"), tensor(o[1], "key"), tensor(o[2], "value")};
         const at::Tensor cu = tensor(o[3], "cu_seqlens");
         const double scaling = o[4] == Py_None ? 0.08838834764831845 : number(o[4]);  // 128 ** -0.5
         const bool causal = o[5] == Py_True, stats = o[7] == Py_True;
-        at::Tensor out = optional_tensor(o[6], "out"), lse;
+        at::Tensor out = optional_tensor(o[6], "out"), status = optional_tensor(o[8], "status"), lse;
         const at::ScalarType type = x[0].scalar_type();
         for (const at::Tensor& t : x)
             if (t.dim() != 3 || t.size(2) != 128 || t.scalar_type() != type || (type != at::kHalf && type != at::kBFloat16) || !t.is_cuda())
@@ -853,12 +870,13 @@ PyObject* py_prompt_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
         if (kh < 1 || nh < 1 || nh % kh || nh / kh > 128) value_error("query heads must be a multiple of the KV heads, at most 128 per KV head");
         if (total > 0x7fffffff) value_error("too many tokens for one call");
         const c10::DeviceIndex dev = x[0].get_device();
-        for (const at::Tensor& t : {x[1], x[2], cu, out}) same_device(dev, t);
+        for (const at::Tensor& t : {x[1], x[2], cu, out, status}) same_device(dev, t);
         if (cu.dim() != 1 || cu.size(0) < 1 || cu.scalar_type() != at::kInt || cu.size(0) > 0x7fffffff)
             value_error("cu_seqlens must be int32 [sequences + 1]");
         if (!(scaling > 0.0) || !(scaling < 3.0e38)) value_error("scaling must be positive and finite");
         if (out.defined() && (out.sizes() != x[0].sizes() || out.scalar_type() != type || !out.is_contiguous() || (reinterpret_cast<uintptr_t>(out.const_data_ptr()) & 31u)))
             value_error("out must be contiguous, of the query's shape and type, on a 32-byte boundary");
+        if (status.defined() && (status.numel() < 1 || status.scalar_type() != at::kInt)) value_error("status must be an int32 tensor");
         refuse_gradients({x[0], x[1], x[2], out}, "prompt_attention");
         {
             const Unlocked free;
@@ -869,22 +887,21 @@ PyObject* py_prompt_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
             if (total > 0) {
                 for (at::Tensor& t : x) t = packed_rows(t);
                 const at::Tensor ends = cu.contiguous();
-                check(reskv_prompt_attention(x[0].const_data_ptr(), x[1].const_data_ptr(), x[2].const_data_ptr(),
-                                             static_cast<const int32_t*>(ends.const_data_ptr()), static_cast<int>(ends.size(0) - 1),
-                                             static_cast<int>(total), static_cast<int>(kh), static_cast<int>(nh), type == at::kBFloat16,
-                                             token_step(x[0]), head_step(x[0]), token_step(x[1]), head_step(x[1]), token_step(x[2]),
-                                             head_step(x[2]), static_cast<float>(scaling), causal, out.data_ptr(),
-                                             stats ? static_cast<float*>(lse.data_ptr()) : nullptr,
-                                             c10::cuda::getCurrentCUDAStream(dev).stream()));
-                if (ends.size(0) > 1) ++g_launches;
-                if (g_check_status) {
-                    uint32_t status = 0;
-                    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-                    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
-                    check_cuda(cudaStreamIsCapturing(stream, &capture), "cudaStreamIsCapturing");
-                    if (capture == cudaStreamCaptureStatusNone) check(reskv_prompt_attention_status(&status, stream));
-                    if (status) throw Failure{PyExc_RuntimeError, "prompt_attention: a bounded wait ran out on the device"};
+                const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+                const bool look = look_at_status(stream);
+                if (look && !status.defined()) {  // of this call: what another one met is not its fault
+                    status = at::detail::empty_cuda({1}, at::kInt, x[0].device(), std::nullopt);
+                    check_cuda(cudaMemsetAsync(status.data_ptr(), 0, sizeof(uint32_t), stream), "status");
                 }
+                uint32_t* const word = status.defined() ? static_cast<uint32_t*>(status.data_ptr()) : nullptr;
+                check(reskv_prompt_attention_reporting(
+                    x[0].const_data_ptr(), x[1].const_data_ptr(), x[2].const_data_ptr(),
+                    static_cast<const int32_t*>(ends.const_data_ptr()), static_cast<int>(ends.size(0) - 1), static_cast<int>(total),
+                    static_cast<int>(kh), static_cast<int>(nh), type == at::kBFloat16, token_step(x[0]), head_step(x[0]), token_step(x[1]),
+                    head_step(x[1]), token_step(x[2]), head_step(x[2]), static_cast<float>(scaling), causal, out.data_ptr(),
+                    stats ? static_cast<float*>(lse.data_ptr()) : nullptr, word, stream));
+                if (ends.size(0) > 1) ++g_launches;
+                if (look) raise_on_status(word, stream, "prompt_attention");
             }
         }
         if (!stats) return THPVariable_Wrap(out);
@@ -919,18 +936,7 @@ struct Pool {
         return t;
     }
     void after(cudaStream_t stream) const {
-        if (!g_check_status) return;
-        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-        check_cuda(cudaStreamIsCapturing(stream, &capture), "cudaStreamIsCapturing");
-        if (capture != cudaStreamCaptureStatusNone) return;
-        uint32_t status_word = 0;
-        check_cuda(cudaMemcpyAsync(&status_word, word(), sizeof(status_word), cudaMemcpyDeviceToHost, stream), "status copy");
-        check_cuda(cudaStreamSynchronize(stream), "status synchronize");
-        if (status_word) {
-            char text[80];
-            std::snprintf(text, sizeof(text), "paged cache: device status 0x%x", status_word);
-            throw Failure{PyExc_RuntimeError, text};
-        }
+        if (look_at_status(stream)) raise_on_status(word(), stream, "paged cache");
     }
 };
 

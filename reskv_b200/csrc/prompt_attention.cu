@@ -57,7 +57,7 @@ static_assert(kPKeys + kPKeys / 2 <= 128 && kPKeys % 16 == 0, "scores and weight
 constexpr float kPSlack = 8.f;                  // the running maximum lags by at most this (in powers of two)
 constexpr float kPLowest = -0x1.ffffp127f;      // the running maximum of a row whose scores have all been -infinity
 
-__device__ uint32_t g_prompt_status;  // RESKV_STATUS_* bits
+__device__ uint32_t g_prompt_status;  // RESKV_STATUS_* bits of calls without a word of their own
 
 struct PromptParams {
     const int* cu;      // [sequences + 1]
@@ -69,6 +69,7 @@ struct PromptParams {
     float* lse;         // [total, query heads] or null
     float scale_log2;
     int causal;
+    uint32_t* status;   // or null: g_prompt_status
 };
 
 // A work item: one or two row tiles of one sequence and KV head.
@@ -574,7 +575,7 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
             if (lane == 0) mbar_arrive(&sh.item_empty[slot]);
         }
     }
-    if (lost) atomicOr(&g_prompt_status, RESKV_STATUS_WAIT_TIMEOUT);
+    if (lost) atomicOr(p.status ? p.status : &g_prompt_status, RESKV_STATUS_WAIT_TIMEOUT);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -617,6 +618,14 @@ extern "C" int reskv_prompt_attention(const void* q, const void* k, const void* 
                                       int kv_heads, int q_heads, int bf16, int64_t q_token, int64_t q_head, int64_t k_token,
                                       int64_t k_head, int64_t v_token, int64_t v_head, float scaling, int causal, void* out, float* lse,
                                       void* stream) {
+    return reskv_prompt_attention_reporting(q, k, v, cu_seqlens, sequences, total, kv_heads, q_heads, bf16, q_token, q_head, k_token, k_head,
+                                            v_token, v_head, scaling, causal, out, lse, nullptr, stream);
+}
+
+extern "C" int reskv_prompt_attention_reporting(const void* q, const void* k, const void* v, const int32_t* cu_seqlens, int sequences,
+                                                int total, int kv_heads, int q_heads, int bf16, int64_t q_token, int64_t q_head,
+                                                int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, float scaling, int causal,
+                                                void* out, float* lse, uint32_t* status, void* stream) {
     if (sequences < 0 || total < 0 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads)
         return fail(RESKV_ERR_INVALID, "prompt_attention: %d sequences, %d tokens, %d query and %d KV heads", sequences, total, q_heads, kv_heads);
     if (q_heads / kv_heads > 128) return fail(RESKV_ERR_LIMIT, "prompt_attention: more than 128 query heads per KV head");
@@ -629,11 +638,13 @@ extern "C" int reskv_prompt_attention(const void* q, const void* k, const void* 
     if (reinterpret_cast<uintptr_t>(out) & 31u) return fail(RESKV_ERR_INVALID, "prompt_attention: out must start on a 32-byte boundary");
     if (int rc = check_device_pointer(out, "prompt_attention", "out")) return rc;
     if (int rc = check_device_pointer(cu_seqlens, "prompt_attention", "cu_seqlens")) return rc;
+    if (status)
+        if (int rc = check_device_pointer(status, "prompt_attention", "status")) return rc;
     PromptParams p{};
     p.cu = cu_seqlens, p.sequences = sequences, p.total = total, p.kv_heads = kv_heads, p.group = q_heads / kv_heads;
     p.tile_tokens = 128 / p.group;
     p.v = static_cast<const unsigned short*>(v), p.v_token = v_token, p.v_head = v_head;
-    p.out = out, p.lse = lse, p.scale_log2 = scaling * kLog2e, p.causal = causal != 0;
+    p.out = out, p.lse = lse, p.scale_log2 = scaling * kLog2e, p.causal = causal != 0, p.status = status;
     CUtensorMap qm, km, vm;
     if (int rc = rows_map(&qm, q, q_heads, total, q_token, q_head, p.group, p.tile_tokens)) return rc;
     if (int rc = rows_map(&km, k, kv_heads, total, k_token, k_head, 1, kPKeys)) return rc;

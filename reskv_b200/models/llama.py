@@ -340,12 +340,15 @@ class ResKVLlama:
                 _, qr = self._qkv(layer, x[:, rows], trig, k, kr, v)
                 keys, values = kr[0].transpose(0, 1), v[0].transpose(0, 1)
                 self.paged.write(index, step, keys, values)
-                att = prompt_attention(qr[0].transpose(0, 1), keys, values, step.cu_seqlens, scaling=self.scaling)
+                att = prompt_attention(qr[0].transpose(0, 1), keys, values, step.cu_seqlens, scaling=self.scaling, status=self.paged.status)
                 self._add_projection(x[:, rows], att.view(1, step.total, -1), layer["wo"])
                 del k, kr, v, qr, keys, values, att
             self._add_mlp(layer, x)
         ends = torch.tensor(lengths, device=self.device).cumsum(0) - 1
-        return self._logits(x[0, ends].unsqueeze(1))
+        logits = self._logits(x[0, ends].unsqueeze(1))
+        if self._check_status:
+            self._raise_on_status()
+        return logits
 
     def select(self, rows) -> None:
         """``cache="int4"``: the batch becomes these rows of the present one, a row several times where it forks (samples of one

@@ -212,6 +212,11 @@ class PagedInt4Cache:
         if pairs:
             host().copy_pages(self.pages, *zip(*pairs))
 
+    @property
+    def status(self) -> torch.Tensor:
+        """What ``check`` reads, int32 on the device; ``prompt_attention(..., status=cache.status)`` reports there too."""
+        return self._status
+
     def check(self) -> None:
         """Waits for the device and raises if a kernel met a token or page outside its tables, or a wait that ran out."""
         word = self._status.item()

@@ -22,6 +22,7 @@ def prompt_attention(
     causal: bool = True,
     out: torch.Tensor | None = None,
     return_lse: bool = False,
+    status: torch.Tensor | None = None,
 ):
     """Attention of every token to the tokens of its own sequence (``causal``: up to itself).
 
@@ -35,7 +36,10 @@ def prompt_attention(
     with ``return_lse`` also FP32 ``[T,H]``, the natural logarithm of each row's sum of exponentials.  Rows that belong to no
     sequence are not written.  Scores, sums and products are FP32, the weights are rounded once to the type of ``value`` for
     the product with it.  Infinities and NaN count only where they are attended to.  Inference only: the result has no gradient.
+
+    ``status``, an int32 tensor on the device (``PagedInt4Cache.status``, whose ``check()`` then speaks for this call too), gets a
+    bit if a bounded wait on the device ran out and rows were left unwritten.
     """
     if isinstance(query, torch.Tensor) and query.is_cuda:
         require_device(query.get_device())
-    return host().prompt_attention(query, key, value, cu_seqlens, scaling, bool(causal), out, bool(return_lse))
+    return host().prompt_attention(query, key, value, cu_seqlens, scaling, bool(causal), out, bool(return_lse), status)

@@ -347,3 +347,31 @@ def test_leading_keys_whose_scores_are_minus_infinity(at, scaling, dtype, causal
         assert_within(got[rows, 4:], want, bound)
         # a score is off by less than 128 * 2^-23 * sum|q k| * scaling (sum|q k| < 600), the sum of exponentials by 2^-13
         assert (lse[rows, 4:].double() - want_lse).abs().max().item() < 2e-3 + 0.01 * scaling
+
+
+@pytest.mark.gpu
+def test_what_a_call_met_is_its_own():
+    """The words are set by the host, no wait runs out here: a call reports to the word that it is given, and calls without one do not
+    speak of others."""
+    q, k, v, ends, cu = inputs([50, 70], 2, 4, torch.float16, seed=16)
+    want = prompt_attention(q, k, v, cu)
+    clean, marked = torch.zeros(1, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    with pytest.raises(RuntimeError, match="prompt_attention: device status 0x1"):  # RESKV_CHECK_STATUS=1
+        prompt_attention(q, k, v, cu, status=marked)
+    assert torch.equal(prompt_attention(q, k, v, cu, status=clean), want) and clean.item() == 0
+    assert torch.equal(prompt_attention(q, k, v, cu), want)
+    for bad in (clean.float(), clean[:0], clean.cpu()):
+        with pytest.raises(ValueError):
+            prompt_attention(q, k, v, cu, status=bad)
+
+
+def test_the_library_refuses_a_status_word_of_the_host():
+    import numpy as np
+
+    from reskv_b200._extension import ERR_INVALID, library
+
+    x, cu = np.zeros((4, 2, 128), np.float16), np.array([0, 4], np.int32)
+    assert x.ctypes.data % 16 == 0
+    call = library().reskv_prompt_attention_reporting
+    assert call(*[x.ctypes.data] * 3, cu.ctypes.data, 1, 4, 2, 3, 0, *[256, 128] * 3, 0.1, 1, x.ctypes.data, None, cu.ctypes.data, None) == ERR_INVALID
+    assert call(*[x.ctypes.data] * 3, cu.ctypes.data, 0, 4, 2, 2, 0, *[256, 128] * 3, 0.1, 1, x.ctypes.data, None, cu.ctypes.data, None) == 0

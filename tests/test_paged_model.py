@@ -215,3 +215,23 @@ def test_reused_tables_belong_to_the_last_step_of_this_cache():
         other.extend(other.add(2), 1, reuse=third)
     cache.attend(0, third, x)  # and nothing changed
     cache.check()
+
+
+@pytest.mark.gpu
+def test_a_prompt_whose_wait_ran_out_raises(monkeypatch):
+    """The word is set by the host, no wait runs out here: what the attention of a prompt reports is the cache's to tell, and the model
+    asks for it."""
+    import reskv_b200.models.llama as llama
+
+    model, real = make(), llama.prompt_attention
+    assert model.prefill(prompts(5, 6)).isfinite().all()
+
+    def lost(*args, status=None, **kw):
+        out = real(*args, status=status, **kw)
+        if status is not None:
+            status.fill_(1)
+        return out
+
+    monkeypatch.setattr(llama, "prompt_attention", lost)
+    with pytest.raises(RuntimeError, match="device status"):
+        model.prefill(prompts(5, 6))
