@@ -819,10 +819,16 @@ PyObject* py_ids_in_range(PyObject*, PyObject* ticket) {
     });
 }
 
-void refuse_gradients(std::initializer_list<at::Tensor> all, const char* who) {
-    if (!c10::GradMode::is_enabled()) return;
-    for (const at::Tensor& t : all)
-        if (t.defined() && t.requires_grad()) value_error(std::string(who) + " is inference only: call it under torch.no_grad()");
+// A tensor of a caller for an operator without a derivative that is not an operation of the dispatcher: refused if something
+// that an operation would do with it would be lost without a word (see `plain`; negated views are copied, modes see nothing).
+at::Tensor inference_tensor(PyObject* o, const char* what, const char* who) {
+    const at::Tensor x = tensor(o, what);
+    if ((c10::GradMode::is_enabled() && x.requires_grad()) || x._fw_grad(0).defined())
+        value_error(std::string(who) + " is inference only, " + what + " has a gradient or a tangent: call it under torch.no_grad(), on detached tensors");
+    if (!THPVariable_CheckExact(o) || !(x.key_set() & at::kTensorSubclassLike).empty() || !x.unsafeGetTensorImpl()->has_storage() || x._is_zerotensor() ||
+        c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer))
+        value_error(std::string(who) + " takes plain tensors outside of a trace, " + what + " is none");
+    return x;
 }
 
 // Whether a call waits for its kernels and looks at their status word: asked for, and not while the stream is captured.
@@ -856,11 +862,14 @@ int64_t head_step(const at::Tensor& x) { return x.size(1) == 1 ? 128 : x.stride(
 PyObject* py_prompt_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         expect(n, 9);
-        at::Tensor x[3] = {tensor(o[0], "query"), tensor(o[1], "key"), tensor(o[2], "value")};
-        const at::Tensor cu = tensor(o[3], "cu_seqlens");
+        const char* const who = "prompt_attention";
+        at::Tensor x[3] = {inference_tensor(o[0], "query", who), inference_tensor(o[1], "key", who), inference_tensor(o[2], "value", who)};
+        const at::Tensor cu = inference_tensor(o[3], "cu_seqlens", who);
         const double scaling = o[4] == Py_None ? 0.08838834764831845 : number(o[4]);  // 128 ** -0.5
         const bool causal = o[5] == Py_True, stats = o[7] == Py_True;
-        at::Tensor out = optional_tensor(o[6], "out"), status = optional_tensor(o[8], "status"), lse;
+        at::Tensor out, status, lse;
+        if (o[6] != Py_None) out = inference_tensor(o[6], "out", who);
+        if (o[8] != Py_None) status = inference_tensor(o[8], "status", who);
         const at::ScalarType type = x[0].scalar_type();
         for (const at::Tensor& t : x)
             if (t.dim() != 3 || t.size(2) != 128 || t.scalar_type() != type || (type != at::kHalf && type != at::kBFloat16) || !t.is_cuda())
@@ -877,7 +886,6 @@ PyObject* py_prompt_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
         if (out.defined() && (out.sizes() != x[0].sizes() || out.scalar_type() != type || !out.is_contiguous() || (reinterpret_cast<uintptr_t>(out.const_data_ptr()) & 31u)))
             value_error("out must be contiguous, of the query's shape and type, on a 32-byte boundary");
         if (status.defined() && (status.numel() < 1 || status.scalar_type() != at::kInt)) value_error("status must be an int32 tensor");
-        refuse_gradients({x[0], x[1], x[2], out}, "prompt_attention");
         {
             const Unlocked free;
             const at::AutoDispatchBelowADInplaceOrView plain;
@@ -951,14 +959,13 @@ PyObject* py_paged_write(PyObject*, PyObject* const* o, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         expect(n, 8);
         const Pool pool(o[0], o[1], o[2]);
-        at::Tensor k = tensor(o[3], "key"), v = tensor(o[4], "value");
+        at::Tensor k = inference_tensor(o[3], "key", "paged_write"), v = inference_tensor(o[4], "value", "paged_write");
         const at::Tensor cu = pool.table(o[5], "cu_seqlens", 1), starts = pool.table(o[6], "starts", 1), table = pool.table(o[7], "table", 2);
         const at::ScalarType type = model_type(k, "key");
         same_device(pool.dev, k), same_device(pool.dev, v);
         if (k.dim() != 3 || k.size(1) != pool.heads || k.size(2) != 128 || k.sizes() != v.sizes() || v.scalar_type() != type || k.size(0) > 0x7fffffff)
             value_error("key and value must be [tokens, KV heads, 128] of one type");
         if (cu.size(0) != starts.size(0) + 1 || table.size(0) != starts.size(0)) value_error("cu_seqlens, starts and table belong to different numbers of sequences");
-        refuse_gradients({k, v}, "paged_write");
         {
             const Unlocked free;
             const at::AutoDispatchBelowADInplaceOrView plain;
@@ -1019,7 +1026,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         expect(n, 8);
         const Pool pool(o[0], o[1], o[2]);
-        at::Tensor q = tensor(o[3], "query");
+        at::Tensor q = inference_tensor(o[3], "query", "paged_attention");
         const at::Tensor lengths = pool.table(o[4], "lengths", 1), table = pool.table(o[5], "table", 2);
         const double scaling = o[6] == Py_None ? 0.08838834764831845 : number(o[6]);  // 128 ** -0.5
         const bool stats = o[7] == Py_True;
@@ -1031,7 +1038,6 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
             value_error("query heads must be a multiple of the KV heads, at most 8 per KV head");
         if (!(scaling > 0.0) || !(scaling < 3.0e38)) value_error("scaling must be positive and finite");
         if (q.size(0) * pool.heads > 0x7fffffff || table.size(1) > (1 << 24)) value_error("too many sequences or pages for one call");
-        refuse_gradients({q}, "paged_attention");
         at::Tensor out, lse;
         {
             const Unlocked free;

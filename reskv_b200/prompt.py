@@ -35,7 +35,8 @@ def prompt_attention(
     Returns ``[T,H,128]`` of the query's type, written to ``out`` if that is given (contiguous, not overlapping the inputs);
     with ``return_lse`` also FP32 ``[T,H]``, the natural logarithm of each row's sum of exponentials.  Rows that belong to no
     sequence are not written.  Scores, sums and products are FP32, the weights are rounded once to the type of ``value`` for
-    the product with it.  Infinities and NaN count only where they are attended to.  Inference only: the result has no gradient.
+    the product with it.  Infinities and NaN count only where they are attended to.  Inference only: tensors that ask for
+    a gradient, carry a tangent, are no plain tensors (subclasses, vmap) or are being traced are refused.
 
     ``status``, an int32 tensor on the device (``PagedInt4Cache.status``, whose ``check()`` then speaks for this call too), gets a
     bit if a bounded wait on the device ran out and rows were left unwritten.

@@ -645,3 +645,31 @@ def test_queries_of_zeros_with_a_tiny_scaling(dtype, scaling):
         want, want_lse, bound = formula(q[i], k[i], v[i], scaling)
         assert ((got[i].double() - want).abs() <= bound).all()
         assert (lse[i].double() - want_lse).abs().max() < 1e-3
+
+
+class Tagged(torch.Tensor):
+    pass
+
+
+@pytest.mark.gpu
+def test_what_would_be_lost_without_a_word_is_refused():
+    from torch.autograd import forward_ad
+
+    cache = PagedInt4Cache(1, 2, 4)
+    step = cache.extend(cache.add(2), [1, 1])
+    x, q = vectors(2, 2, torch.float16, 1), vectors(2, 8, torch.float16, 2)
+    cache.write(0, step, x, x)
+    want, pages = cache.attend(0, step, q), cache.pages[0, :2, :, 0].clone()
+    with forward_ad.dual_level():
+        dual = lambda y: forward_ad.make_dual(y, torch.ones_like(y))  # noqa: E731
+        for call in (lambda: cache.write(0, step, dual(x), x), lambda: cache.write(0, step, x, dual(x)), lambda: cache.attend(0, step, dual(q))):
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                call()
+    tag = lambda y: y.as_subclass(Tagged)  # noqa: E731
+    for call in (lambda: cache.write(0, step, tag(x), x), lambda: cache.write(0, step, x, tag(x)), lambda: cache.attend(0, step, tag(q)),
+                 lambda: torch.vmap(lambda y: cache.attend(0, step, y))(q[None]),
+                 lambda: torch.jit.trace(lambda y: cache.attend(0, step, y), (q,), check_trace=False)):
+        with pytest.raises(ValueError, match="plain tensors"):
+            call()
+    cache.write(0, step, torch._neg_view(-x), torch._neg_view(-x))
+    assert torch.equal(cache.pages[0, :2, :, 0, :64], pages[..., :64]) and torch.equal(cache.attend(0, step, torch._neg_view(-q)), want)

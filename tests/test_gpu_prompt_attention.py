@@ -375,3 +375,34 @@ def test_the_library_refuses_a_status_word_of_the_host():
     call = library().reskv_prompt_attention_reporting
     assert call(*[x.ctypes.data] * 3, cu.ctypes.data, 1, 4, 2, 3, 0, *[256, 128] * 3, 0.1, 1, x.ctypes.data, None, cu.ctypes.data, None) == ERR_INVALID
     assert call(*[x.ctypes.data] * 3, cu.ctypes.data, 0, 4, 2, 2, 0, *[256, 128] * 3, 0.1, 1, x.ctypes.data, None, cu.ctypes.data, None) == 0
+
+
+class Tagged(torch.Tensor):
+    pass
+
+
+@pytest.mark.gpu
+def test_what_would_be_lost_without_a_word_is_refused():
+    """Tangents, subclasses, vmap and traces; a negated view is read as what it stands for."""
+    from torch.autograd import forward_ad
+
+    q, k, v, ends, cu = inputs([30, 20], 1, 2, torch.float16, seed=17)
+    want = prompt_attention(q, k, v, cu)
+    with forward_ad.dual_level():
+        for i in range(3):
+            args = [forward_ad.make_dual(x, torch.ones_like(x)) if i == j else x for j, x in enumerate((q, k, v))]
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                prompt_attention(*args, cu)
+    for i in range(4):
+        args = [x.as_subclass(Tagged) if i == j else x for j, x in enumerate((q, k, v, cu))]
+        with pytest.raises(ValueError, match="plain tensors"):
+            prompt_attention(*args)
+    with pytest.raises(ValueError, match="plain tensors"):
+        torch.vmap(lambda x: prompt_attention(x, k, v, cu))(q[None])
+    with pytest.raises(ValueError, match="plain tensors"):
+        torch.jit.trace(lambda x: prompt_attention(x, k, v, cu), (q,), check_trace=False)
+    with torch.no_grad():
+        assert torch.equal(prompt_attention(torch.nn.Parameter(q), k, v, cu), want)
+    with torch.inference_mode():
+        assert torch.equal(prompt_attention(q.clone(), k, v, cu), want)
+    assert torch.equal(prompt_attention(torch._neg_view(-q), torch._neg_view(-k.contiguous()), v, cu), want)
