@@ -279,7 +279,8 @@ class ResKVLlama:
         ``prefill_chunk`` tokens at a time) so that their FP32 temporaries stay small at long contexts;
         the cache of a layer receives the whole batch at once.
 
-        With ``cache="int4"`` ``ids`` may also be a sequence of prompts ``[T_i]`` of different lengths."""
+        With ``cache="int4"`` ``ids`` may also be a sequence of prompts ``[T_i]`` of different lengths; a call that fails on its way
+        leaves no batch."""
         if self.cache_kind == "int4":
             return self._prefill_paged(list(ids), reserve)
         b, t = ids.shape
@@ -313,16 +314,30 @@ class ResKVLlama:
         return self._logits(x[:, -1:])
 
     def _prefill_paged(self, prompts, reserve):
-        lengths = [p.numel() for p in prompts]
-        if not prompts or any(p.ndim != 1 or p.numel() == 0 for p in prompts):
-            raise ValueError("prompts must be one-dimensional and hold a token at least")
+        if not prompts or any(not isinstance(p, torch.Tensor) or p.ndim != 1 or p.numel() == 0 for p in prompts):
+            raise ValueError("prompts must be one-dimensional tensors and hold a token at least")
         if type(reserve) is not int or reserve < 0:
             raise ValueError("reserve must be a non-negative integer")
+        self._end_paged_batch()  # the pool in front goes before the next one comes
+        try:
+            logits = self._run_prompts(prompts, reserve)
+            if self._check_status:
+                self._raise_on_status()
+            return logits
+        except BaseException:  # tokens that are counted but not written may not be attended to
+            self._end_paged_batch()
+            raise
+
+    def _end_paged_batch(self):
+        self.paged = self.caches = self._step = self._graph = None
+        self.sequences = []
+
+    def _run_prompts(self, prompts, reserve):
+        lengths = [p.numel() for p in prompts]
         need = sum(-(-(t + reserve) // PAGE_TOKENS) for t in lengths)
-        self.paged = self.caches = self._step = None  # the pool in front goes before the next one comes
         self.paged = PagedInt4Cache(self.shape.layers, self.h_kv, self.pages or need, dtype=torch.float16, device=self.device)
         self.sequences = self.paged.add(len(prompts))
-        self.caches, self._graph, self._reserve = [self.paged], None, reserve
+        self.caches, self._reserve = [self.paged], reserve
         x = self.embed[torch.cat([p.to(self.device) for p in prompts])].unsqueeze(0)
         # whole prompts, at most prefill_chunk tokens together: (step, rows of x, sin and cos)
         parts, at = [], 0
@@ -345,10 +360,7 @@ class ResKVLlama:
                 del k, kr, v, qr, keys, values, att
             self._add_mlp(layer, x)
         ends = torch.tensor(lengths, device=self.device).cumsum(0) - 1
-        logits = self._logits(x[0, ends].unsqueeze(1))
-        if self._check_status:
-            self._raise_on_status()
-        return logits
+        return self._logits(x[0, ends].unsqueeze(1))
 
     def select(self, rows) -> None:
         """``cache="int4"``: the batch becomes these rows of the present one, a row several times where it forks (samples of one

@@ -235,3 +235,36 @@ def test_a_prompt_whose_wait_ran_out_raises(monkeypatch):
     monkeypatch.setattr(llama, "prompt_attention", lost)
     with pytest.raises(RuntimeError, match="device status"):
         model.prefill(prompts(5, 6))
+
+
+@pytest.mark.gpu
+def test_a_prompt_that_fails_leaves_no_batch():
+    """Two slices of prompts, of which the second finds no pages: nothing may attend to the tokens that were never written."""
+    model = make(pages=3, prefill_chunk=100)
+    model.prefill(prompts(5, 6))
+    with pytest.raises(RuntimeError, match="out of pages"):
+        model.prefill(prompts(65, 65))
+    for call in (lambda: model.decode(torch.zeros(2, dtype=torch.long, device="cuda")), lambda: model.select([0]),
+                 lambda: model.begin_graph_decode(2)):
+        with pytest.raises((RuntimeError, ValueError)):
+            call()
+    assert model.sequences == [] and model.cache_bytes() == 0
+    ids = prompts(64, 65)
+    assert torch.equal(model.prefill(ids), make().prefill(ids))
+    model.layers[1] = None  # a layer that fails in the middle of a prompt
+    with pytest.raises(TypeError):
+        model.prefill(ids)
+    with pytest.raises((RuntimeError, ValueError)):
+        model.decode(torch.zeros(2, dtype=torch.long, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_bad_prompts_leave_the_batch_as_it_is():
+    model, ids = make(), prompts(5, 6)
+    logits = model.prefill(ids, reserve=4)
+    for bad in ([], [torch.zeros(0, dtype=torch.long, device="cuda")], [3]):
+        with pytest.raises((ValueError, TypeError)):
+            model.prefill(bad)
+    with pytest.raises(ValueError):
+        model.prefill(ids, reserve=1.5)
+    assert model.decode(logits.argmax(-1)).isfinite().all()
