@@ -130,6 +130,16 @@ class PagedInt4Cache:
                     raise ValueError(f"{most} pages of a sequence do not fit a table of {reuse.table.shape[1]}")
             width = reuse.table.shape[1]
         entries = book.extend(sequences, counts)
+        try:
+            step = self._tables_of(entries, sequences, counts, width, reuse)
+        except BaseException:  # no memory for the tables: the device has not heard of these tokens
+            book.retract(entries, counts)
+            raise
+        for e in entries:
+            e.supersede(step)
+        return step
+
+    def _tables_of(self, entries, sequences, counts, width, reuse) -> PagedStep:
         step = PagedStep()
         n, width = len(entries), max([width, *(len(e.pages) for e in entries)])
         step.sequences, step.counts, step.lengths = tuple(sequences), tuple(counts), tuple(e.length for e in entries)
@@ -142,7 +152,7 @@ class PagedInt4Cache:
         for row, e in zip(table, entries):
             row[:len(e.pages)] = e.pages
         if reuse is None:
-            step._tables = _Tables(_upload(numbers, self.device), book)
+            step._tables = _Tables(_upload(numbers, self.device), self._book)
         else:
             step._tables = reuse._tables
             step._tables.numbers.copy_(_pinned(numbers), non_blocking=True)
@@ -150,17 +160,13 @@ class PagedInt4Cache:
         step._use, there = step._tables.uses, step._tables.numbers
         step.cu_seqlens, step.starts, step.device_lengths = there[:n + 1], there[n + 1:2 * n + 1], there[2 * n + 1:3 * n + 1]
         step.table = there[3 * n + 1:].view(n, width)
-        step._whole, step._epoch, step._current = None, book.epoch, True
-        for e in entries:
-            e.supersede(step)
+        step._whole, step._epoch, step._current = None, self._book.epoch, True
         return step
 
     def fork(self, sequences) -> list[int]:
         """A new sequence with the tokens of each of ``sequences`` (one may be named several times).  Full pages are shared, a
         partly filled last page is copied; steps of the forked sequences may not be used any more."""
-        new, pairs = self._book.fork(list(sequences))
-        self._copy(pairs)
-        return new
+        return self._book.fork(list(sequences), self._copy)[0]
 
     def free(self, sequences) -> None:
         """Ends ``sequences``; pages that no other sequence shares go back to the pool."""
@@ -168,9 +174,7 @@ class PagedInt4Cache:
 
     def compact(self) -> int:
         """Moves the pages in use to the front of the pool and returns their number.  No earlier step may be used any more."""
-        used, pairs = self._book.compact()
-        self._copy(pairs)
-        return used
+        return self._book.compact(self._copy)[0]
 
     # -- device ----------------------------------------------------------------------------------------------------------------
     def _check(self, step: PagedStep) -> None:
@@ -290,18 +294,30 @@ class PageBook:
             e.length += c
         return entries
 
-    def fork(self, sequences):
-        """(new sequences, pages to copy)"""
+    def retract(self, entries, counts) -> None:
+        """Takes the last ``extend`` back."""
+        for e, c in zip(reversed(entries), reversed(counts)):
+            e.length -= c
+            while len(e.pages) > -(-e.length // PAGE_TOKENS):
+                self.holders[e.pages[-1]] = 0
+                self.free.append(e.pages.pop())
+
+    def fork(self, sequences, copy=None):
+        """(new sequences, pages to copy).  ``copy`` is called with the pages before anything changes; what it raises leaves the book
+        as it is."""
         entries = [self.of(s) for s in sequences]
-        self._need(sum(e.length % PAGE_TOKENS != 0 for e in entries))
-        new, pairs = [], []
+        parted = [e for e in entries if e.length % PAGE_TOKENS]
+        self._need(len(parted))
+        pairs = [(e.pages[-1], page) for e, page in zip(parted, reversed(self.free))]
+        if copy is not None:
+            copy(pairs)
+        new = []
         for e in entries:
             pages = list(e.pages)
             shared = pages
             if e.length % PAGE_TOKENS:
                 shared = pages[:-1]
                 pages[-1] = self._take()
-                pairs.append((e.pages[-1], pages[-1]))
             for page in shared:
                 self.holders[page] += 1
             e.supersede()
@@ -320,13 +336,15 @@ class PageBook:
                     self.free.append(page)
             del self.sequences[s]
 
-    def compact(self):
-        """(pages in use, pages to copy)"""
+    def compact(self, copy=None):
+        """(pages in use, pages to copy); ``copy`` as for ``fork``."""
         pages = len(self.holders)
         used = pages - len(self.free)
         behind = [p for p in range(used, pages) if self.holders[p]]
         room = [p for p in range(used) if not self.holders[p]]
         pairs = list(zip(behind, room))
+        if copy is not None:
+            copy(pairs)
         moved = dict(pairs)
         for a, b in pairs:
             self.holders[b], self.holders[a] = self.holders[a], 0

@@ -673,3 +673,38 @@ def test_what_would_be_lost_without_a_word_is_refused():
             call()
     cache.write(0, step, torch._neg_view(-x), torch._neg_view(-x))
     assert torch.equal(cache.pages[0, :2, :, 0, :64], pages[..., :64]) and torch.equal(cache.attend(0, step, torch._neg_view(-q)), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reuse", [False, True])
+def test_what_fails_in_front_of_the_device_leaves_the_cache_as_it_is(monkeypatch, reuse):
+    """No memory for a step's tables, a page copy that is not launched: no tokens counted, no sequences, no pages moved, and the step in
+    front is still the one."""
+    import reskv_b200.paged as paged
+
+    cache = PagedInt4Cache(1, 2, 12)
+    seqs, k, v = fill(cache, [100, 64, 130], seed=61)
+    cache.free([seqs.pop(1)])
+    k.pop(1), v.pop(1)
+    step = cache.extend(seqs, 0, width=8)
+    q = vectors(2, 8, torch.float16, 62)
+    want, free = cache.attend(0, step, q), cache.free_pages
+
+    def fails(*args):
+        raise MemoryError
+
+    with monkeypatch.context() as m:
+        m.setattr(paged, "_pinned", fails)
+        with pytest.raises(MemoryError):
+            cache.extend(seqs, [200, 1], reuse=step if reuse else None)
+        m.setattr(PagedInt4Cache, "_copy", fails)
+        for call in (lambda: cache.fork([seqs[0], seqs[1]]), cache.compact):
+            with pytest.raises(MemoryError):
+                call()
+    assert [cache.length(s) for s in seqs] == [100, 130] and cache.free_pages == free and len(cache._book.sequences) == 2
+    assert torch.equal(cache.attend(0, step, q), want)
+    assert_attends(cache, seqs, k, v, 4)
+    step = cache.extend(seqs, 0, reuse=step if reuse else None)
+    twins = cache.fork(seqs)
+    assert cache.compact() == 7
+    assert torch.equal(cache.attend(0, cache.extend(twins, 0, width=8), q), want)

@@ -155,3 +155,48 @@ def test_the_library_refuses_bad_arguments_before_any_launch():
     assert copy([0], [1]) == ERR_INVALID and b"copy_pages: pages" in lib.reskv_last_error()
     assert copy([0], [1], layers=65536) == ERR_LIMIT
     assert copy([], []) == 0 and copy([0], [1], layers=0) == 0
+
+
+def state(book):
+    return (list(book.free), list(book.holders), {s: (list(e.pages), e.length, e.step) for s, e in book.sequences.items()}, book.epoch, book._next)
+
+
+def test_a_copy_that_fails_changes_nothing():
+    book, seen = PageBook(12), []
+    a, b, c = book.add(3)
+    book.extend([a, b, c], [130, 64, 70])
+    book.release([b])
+
+    def fails(pairs):
+        seen.append(pairs)
+        raise MemoryError
+
+    before = state(book)
+    for call in (lambda: book.fork([a, c, a], fails), lambda: book.compact(fails)):
+        with pytest.raises(MemoryError):
+            call()
+        assert state(book) == before
+    # the pages that a copy was offered are those that it gets
+    assert book.fork([a, c, a])[1] == seen[0]
+    check(book, 12)
+    book.release([a])
+    assert book.compact(lambda pairs: seen.append(pairs))[1] == seen[-1]
+    check(book, 12)
+
+
+def test_an_extension_is_taken_back():
+    rng, book = random.Random(1), PageBook(40)
+    sequences = book.add(5)
+    for _ in range(200):
+        counts = [rng.choice((0, 1, 63, 64, 65, 200)) for _ in sequences]
+        before = state(book)
+        try:
+            entries = book.extend(sequences, counts)
+        except RuntimeError:
+            book.release(sequences)
+            sequences = book.add(5)
+            continue
+        if rng.random() < 0.5:
+            book.retract(entries, counts)
+            assert state(book) == before
+        check(book, 40)
