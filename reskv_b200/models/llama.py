@@ -413,6 +413,19 @@ class ResKVLlama:
     def _decode_paged(self, tokens):
         self._rows(tokens)
         step = self.paged.extend(self.sequences, 1)
+        with self._taken_back(step):
+            return self._run_paged_step(tokens, step)
+
+    @contextlib.contextmanager
+    def _taken_back(self, step):
+        """A step that fails inside does not count: nobody may attend to a token that some layers have not written."""
+        try:
+            yield
+        except BaseException:
+            self.paged._retract(step)
+            raise
+
+    def _run_paged_step(self, tokens, step):
         trig = self._trig_of(step.starts)
         x = self.embed[tokens].unsqueeze(0)
         for index, layer in enumerate(self.layers):
@@ -658,6 +671,8 @@ class ResKVLlama:
         """Same result as ``decode`` but replaying a captured CUDA graph of the step."""
         if self.cache_kind == "int4":
             self._next_paged_step(tokens)
+            with self._taken_back(self._step):
+                return self._replay(tokens)
         if self.cache_kind == "reskv" and self.caches[0].live + 1 == self.caches[0].keys.shape[2]:
             # this token fills the window.  The eager step appends it and then compresses the oldest
             # group before attending (as the reference does); the group does not contain the new
@@ -666,6 +681,9 @@ class ResKVLlama:
             for cache in self.caches:
                 cache._compress_oldest_group()
             self._sync_graph_inputs()
+        return self._replay(tokens)
+
+    def _replay(self, tokens):
         self._tok_in.copy_(tokens)
         if self._graph is None:
             self._capture_step()

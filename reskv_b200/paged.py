@@ -163,6 +163,14 @@ class PagedInt4Cache:
         step._whole, step._epoch, step._current = None, self._book.epoch, True
         return step
 
+    def _retract(self, step: PagedStep) -> None:
+        """Takes back the last step of its sequences, which failed on its way: its tokens do not count."""
+        self._check(step)
+        entries = [self._book.of(s) for s in step.sequences]
+        self._book.retract(entries, step.counts)
+        for e in entries:
+            e.supersede()
+
     def fork(self, sequences) -> list[int]:
         """A new sequence with the tokens of each of ``sequences`` (one may be named several times).  Full pages are shared, a
         partly filled last page is copied; steps of the forked sequences may not be used any more."""

@@ -268,3 +268,25 @@ def test_bad_prompts_leave_the_batch_as_it_is():
     with pytest.raises(ValueError):
         model.prefill(ids, reserve=1.5)
     assert model.decode(logits.argmax(-1)).isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_step_that_fails_does_not_count(graph):
+    """Some layers have written the token, others not: nobody attends to it, and the step can be made again."""
+    model, other, ids = make(pages=8), make(pages=8), prompts(64, 6)
+    tok = model.prefill(ids).argmax(-1)
+    other.prefill(ids)
+    if graph:
+        model.begin_graph_decode(2), other.begin_graph_decode(2)
+    step, want = (model.decode_graph, other.decode_graph) if graph else (model.decode, other.decode)
+    layer, model.layers[1] = model.layers[1], None
+    with pytest.raises(TypeError):
+        step(tok)
+    model.layers[1] = layer
+    assert [model.paged.length(s) for s in model.sequences] == [64, 6] and model.paged.free_pages == 6
+    for _ in range(3):
+        assert torch.equal(step(tok), want(tok))
+    with pytest.raises(ValueError):
+        step(tok[:1])
+    assert [model.paged.length(s) for s in model.sequences] == [67, 9]
