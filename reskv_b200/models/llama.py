@@ -364,15 +364,16 @@ class ResKVLlama:
 
     def select(self, rows) -> None:
         """``cache="int4"``: the batch becomes these rows of the present one, a row several times where it forks (samples of one
-        prompt, beams), rows that are not named end."""
+        prompt, beams), rows that are not named end and leave their pages to those that fork.  RuntimeError, and nothing changed, when
+        the pool has too few."""
         if self.paged is None:
             raise RuntimeError("select() needs cache='int4' and a prefilled batch")
         rows = list(rows)
         if any(type(r) is not int or not 0 <= r < len(self.sequences) for r in rows):
             raise ValueError(f"rows must be whole numbers below {len(self.sequences)}")
         again = [i for i, r in enumerate(rows) if r in rows[:i]]
-        forked = dict(zip(again, self.paged.fork([self.sequences[rows[i]] for i in again])))
-        self.paged.free([s for r, s in enumerate(self.sequences) if r not in rows])
+        ending = [s for r, s in enumerate(self.sequences) if r not in rows]
+        forked = dict(zip(again, self.paged._exchange(ending, [self.sequences[rows[i]] for i in again])))
         self.sequences = [forked.get(i, self.sequences[r]) for i, r in enumerate(rows)]
         self._graph = None
 

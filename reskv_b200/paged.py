@@ -15,6 +15,7 @@ A step of a model::
 
 from __future__ import annotations
 
+from collections import Counter
 
 import numpy as np
 import torch
@@ -176,6 +177,10 @@ class PagedInt4Cache:
         partly filled last page is copied; steps of the forked sequences may not be used any more."""
         return self._book.fork(list(sequences), self._copy)[0]
 
+    def _exchange(self, ending, sequences) -> list[int]:
+        """``free(ending)`` and ``fork(sequences)`` in one, all or nothing: the copies may take the pages that become free."""
+        return self._book.fork(list(sequences), self._copy, list(ending))[0]
+
     def free(self, sequences) -> None:
         """Ends ``sequences``; pages that no other sequence shares go back to the pool."""
         self._book.release(list(sequences))
@@ -310,22 +315,34 @@ class PageBook:
                 self.holders[e.pages[-1]] = 0
                 self.free.append(e.pages.pop())
 
-    def fork(self, sequences, copy=None):
+    def fork(self, sequences, copy=None, ending=()):
         """(new sequences, pages to copy).  ``copy`` is called with the pages before anything changes; what it raises leaves the book
-        as it is."""
-        entries = [self.of(s) for s in sequences]
+        as it is.  The sequences ``ending`` end with it, and their pages serve the new ones."""
+        entries, ends = [self.of(s) for s in sequences], [self.of(s) for s in ending]
+        if len(set(ending)) != len(ends) or not set(ending).isdisjoint(sequences):
+            raise ValueError("a sequence that ends is named twice")
         parted = [e for e in entries if e.length % PAGE_TOKENS]
-        self._need(len(parted))
-        pairs = [(e.pages[-1], page) for e, page in zip(parted, reversed(self.free))]
+        left = Counter(page for e in ends for page in e.pages)  # how many of a page's holders end
+        freed = [page for page, n in left.items() if n == self.holders[page]]
+        if len(parted) > len(self.free) + len(freed):
+            raise RuntimeError(f"out of pages: {len(parted)} needed, {len(self.free) + len(freed)} free")
+        stay = max(0, len(self.free) - len(parted))
+        taken = (self.free[:stay - 1:-1] if stay else self.free[::-1]) + freed
+        pairs = [(e.pages[-1], page) for e, page in zip(parted, taken)]
         if copy is not None:
             copy(pairs)
-        new = []
+        del self.free[stay:]
+        self.release(list(ending))
+        given = {page for _, page in pairs}
+        self.free[stay:] = [page for page in self.free[stay:] if page not in given]
+        new, at = [], iter(taken)
         for e in entries:
             pages = list(e.pages)
             shared = pages
             if e.length % PAGE_TOKENS:
                 shared = pages[:-1]
-                pages[-1] = self._take()
+                pages[-1] = next(at)
+                self.holders[pages[-1]] = 1
             for page in shared:
                 self.holders[page] += 1
             e.supersede()

@@ -200,3 +200,48 @@ def test_an_extension_is_taken_back():
             book.retract(entries, counts)
             assert state(book) == before
         check(book, 40)
+
+
+def test_sequences_that_end_leave_their_pages_to_the_forked_ones():
+    book = PageBook(5)
+    a, b = book.add(2)
+    book.extend([a, b], [130, 65])  # pages 0 1 2, 3 4: none free
+    before = state(book)
+    with pytest.raises(RuntimeError, match="out of pages: 1 needed, 0 free"):
+        book.fork([a])
+    with pytest.raises(RuntimeError, match="out of pages: 3 needed, 2 free"):
+        book.fork([a, a, a], ending=[b])
+    for sequences, ending in (([a], [a]), ([a], [b, b]), ([b], [a, b])):
+        with pytest.raises(ValueError):
+            book.fork(sequences, ending=ending)
+    assert state(book) == before
+    new, pairs = book.fork([a, a], ending=[b])
+    assert [s for s, _ in pairs] == [2, 2] and {d for _, d in pairs} == {3, 4} and set(book.sequences) == {a, *new}
+    check(book, 5)
+    new, pairs = book.fork([new[0]], ending=[new[1], a])  # shared pages stay with the one that is left
+    assert len(book.free) == 1 and book.of(new[0]).pages[:2] == [0, 1]
+    check(book, 5)
+
+
+def test_random_traffic_with_endings():
+    rng, pages = random.Random(2), 30
+    book = PageBook(pages)
+    for _ in range(2000):
+        live, before = list(book.sequences), None
+        if not live or rng.random() < 0.3:
+            book.add(rng.randint(1, 2))
+        try:
+            if live and rng.random() < 0.5:
+                book.extend([rng.choice(live)], [rng.choice((1, 5, 64, 100))])
+            elif live:
+                ending = rng.sample(live, rng.randint(0, len(live) - 1))
+                kept = [s for s in book.sequences if s not in ending]
+                before, seen = state(book), []
+                new, pairs = book.fork([rng.choice(kept) for _ in range(rng.randint(0, 3))], seen.extend, ending)
+                before = None
+                assert seen == pairs and not {s for s, _ in pairs} & {d for _, d in pairs} and len({d for _, d in pairs}) == len(pairs)
+                assert set(book.sequences) == {*kept, *new}
+        except RuntimeError:
+            if before is not None:
+                assert state(book) == before
+        check(book, pages)

@@ -290,3 +290,25 @@ def test_a_step_that_fails_does_not_count(graph):
     with pytest.raises(ValueError):
         step(tok[:1])
     assert [model.paged.length(s) for s in model.sequences] == [67, 9]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_beam_replaces_another_in_a_full_pool(graph):
+    """The pool that a prompt brings has room for its rows and no more: the dropped row's pages serve the forked one."""
+    model, ids = make(), prompts(70, 80)
+    tok = model.prefill(ids, reserve=2).argmax(-1)
+    assert model.paged.free_pages == 0
+    if graph:
+        model.begin_graph_decode(2)
+    decode = model.decode_graph if graph else model.decode
+    decode(tok)
+    before = model.paged.read(1, model.paged.extend([model.sequences[1]], 0), everything=True)
+    with pytest.raises(RuntimeError, match="out of pages"):
+        model.select([0, 1, 1])
+    model.select([1, 1])
+    for s in model.sequences:
+        got = model.paged.read(1, model.paged.extend([s], 0), everything=True)
+        assert torch.equal(got[0], before[0]) and torch.equal(got[1], before[1])
+    tok = torch.tensor([5, 6], device="cuda")
+    torch.testing.assert_close(decode(tok).clone(), plain_rows(model, tok), **CLOSE)
