@@ -200,7 +200,7 @@ class ResKVLlama:
         self.length = 0
         self._lib = None
         # graph decode: the last captured graph (owner of the captures' memory pool), batch sizes whose step has run once
-        self._last_graph = None
+        self._tok_in = self._last_graph = None
         self._warm = set()
 
     # -- helpers -----------------------------------------------------------------------------
@@ -408,6 +408,8 @@ class ResKVLlama:
         return self._logits(x)
 
     def _rows(self, tokens):
+        if not self.sequences:
+            raise ValueError("the batch has no rows: prefill() brings some")
         if tokens.shape != (len(self.sequences),):
             raise ValueError(f"a step takes one token for each of the {len(self.sequences)} rows")
 
@@ -591,11 +593,11 @@ class ResKVLlama:
         """Prepare static buffers after ``prefill``; call once before ``decode_graph``."""
         from .._extension import library
 
+        if self.cache_kind == "int4" and (not self.sequences or batch != len(self.sequences)):
+            raise ValueError(f"the batch has {len(self.sequences) or 'no'} rows: prefill() brings some")
         self._tok_in = torch.zeros(batch, dtype=torch.long, device=self.device)
         self._graph = self._logits_out = None
         if self.cache_kind == "int4":
-            if batch != len(self.sequences):
-                raise ValueError(f"the batch has {len(self.sequences)} rows")
             self._step = None
         elif self.cache_kind == "reskv":
             self._state = torch.zeros(4, dtype=torch.int32, device=self.device)
@@ -702,14 +704,16 @@ class ResKVLlama:
         """Room for one more token of every row, in the tables that the captured step reads; a table that has become too narrow, or
         another batch, invalidates the graph."""
         self._rows(tokens)
+        if self._tok_in is None:
+            raise RuntimeError("begin_graph_decode() comes first")
+        if self._tok_in.shape != tokens.shape:
+            self._tok_in, self._graph = torch.zeros_like(tokens, device=self.device, dtype=torch.long), None
         wide = max(-(-(self.paged.length(s) + 1) // PAGE_TOKENS) for s in self.sequences)
         if self._step is not None and len(self._step.sequences) == len(tokens) and wide <= self._step.table.shape[1]:
             self._step = self.paged.extend(self.sequences, 1, reuse=self._step)
         else:
             more = -(-max(self._reserve, PAGE_TOKENS) // PAGE_TOKENS)
             self._step, self._graph = self.paged.extend(self.sequences, 1, width=wide + more), None
-            if self._tok_in.shape != tokens.shape:
-                self._tok_in = torch.zeros_like(tokens, device=self.device, dtype=torch.long)
 
     def cache_bytes(self) -> int:
         total = 0

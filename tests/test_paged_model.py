@@ -312,3 +312,25 @@ def test_a_beam_replaces_another_in_a_full_pool(graph):
         assert torch.equal(got[0], before[0]) and torch.equal(got[1], before[1])
     tok = torch.tensor([5, 6], device="cuda")
     torch.testing.assert_close(decode(tok).clone(), plain_rows(model, tok), **CLOSE)
+
+
+@pytest.mark.gpu
+def test_a_batch_without_rows():
+    """select([]) ends all rows; there is nothing to decode then, said in words, until the next prompt."""
+    model, ids = make(pages=8), prompts(5, 6)
+    none = torch.zeros(0, dtype=torch.long, device="cuda")
+    for call in (lambda: model.decode(none), lambda: model.begin_graph_decode(0)):
+        with pytest.raises((RuntimeError, ValueError), match="prefill"):
+            call()
+    model.prefill(ids)
+    with pytest.raises(RuntimeError, match="begin_graph_decode"):
+        model.decode_graph(torch.tensor([1, 2], device="cuda"))
+    assert [model.paged.length(s) for s in model.sequences] == [5, 6]
+    model.begin_graph_decode(2)
+    model.decode_graph(torch.tensor([1, 2], device="cuda"))
+    model.select([])
+    assert model.paged.free_pages == 8
+    for call in (lambda: model.decode(none), lambda: model.decode_graph(none), lambda: model.begin_graph_decode(0)):
+        with pytest.raises(ValueError, match="no rows"):
+            call()
+    assert model.generate(ids, 3).shape == (2, 3)
