@@ -40,7 +40,7 @@ class PagedStep:
     def _everything(self):
         """``(cu_seqlens, starts, tokens)`` of all tokens of the sequences, the earlier ones included."""
         if self._whole is None:
-            _refuse_capture()
+            _refuse_capture(self.table.device)
             ends = np.concatenate(([0], np.cumsum(self.lengths)))
             if ends[-1] > 2**31 - 1:
                 raise ValueError("too many tokens for one call")
@@ -57,9 +57,11 @@ class _Tables:
         self.numbers, self.book, self.uses = numbers, book, 0
 
 
-def _refuse_capture() -> None:
-    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("a step's tables come from the host: make them outside of the capture (extend(reuse=) fills those of a captured step)")
+def _refuse_capture(device, what="a step's tables come from the host: make them", instead=" (extend(reuse=) fills those of a captured step)") -> None:
+    with torch.cuda.device(device):
+        capturing = torch.cuda.is_current_stream_capturing()
+    if capturing:
+        raise RuntimeError(f"{what} outside of the capture{instead}")
 
 
 def _pinned(numbers: np.ndarray) -> torch.Tensor:
@@ -117,7 +119,7 @@ class PagedInt4Cache:
         sequences, the tables are written to that step's tensors, whose addresses a graph holds; the step that had them last may
         not be used any more either.  ValueError, and nothing
         changed, when a sequence has more pages than that table is wide."""
-        _refuse_capture()
+        _refuse_capture(self.device)
         book = self._book
         sequences, counts = list(sequences), [counts] * len(sequences) if type(counts) is int else list(counts)
         if type(width) is not int or width < 0:
@@ -175,10 +177,12 @@ class PagedInt4Cache:
     def fork(self, sequences) -> list[int]:
         """A new sequence with the tokens of each of ``sequences`` (one may be named several times).  Full pages are shared, a
         partly filled last page is copied; steps of the forked sequences may not be used any more."""
+        self._refuse_capture()
         return self._book.fork(list(sequences), self._copy)[0]
 
     def _exchange(self, ending, sequences) -> list[int]:
         """``free(ending)`` and ``fork(sequences)`` in one, all or nothing: the copies may take the pages that become free."""
+        self._refuse_capture()
         return self._book.fork(list(sequences), self._copy, list(ending))[0]
 
     def free(self, sequences) -> None:
@@ -187,6 +191,7 @@ class PagedInt4Cache:
 
     def compact(self) -> int:
         """Moves the pages in use to the front of the pool and returns their number.  No earlier step may be used any more."""
+        self._refuse_capture()
         return self._book.compact(self._copy)[0]
 
     # -- device ----------------------------------------------------------------------------------------------------------------
@@ -224,6 +229,9 @@ class PagedInt4Cache:
         """Copies pages ``src[i]`` to ``dst[i]`` in all layers, all at once: no page may be a destination twice, or source and
         destination.  What ``fork`` and ``compact`` use; the caller of this one answers for whose pages they are."""
         host().copy_pages(self.pages, src, dst)
+
+    def _refuse_capture(self) -> None:
+        _refuse_capture(self.device, "pages are given out by the host: fork and compact", " (copy_pages may be captured)")
 
     def _copy(self, pairs) -> None:
         if pairs:

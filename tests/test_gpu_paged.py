@@ -708,3 +708,55 @@ def test_what_fails_in_front_of_the_device_leaves_the_cache_as_it_is(monkeypatch
     twins = cache.fork(seqs)
     assert cache.compact() == 7
     assert torch.equal(cache.attend(0, cache.extend(twins, 0, width=8), q), want)
+
+
+@pytest.mark.gpu
+def test_pages_are_not_forked_or_moved_in_a_capture():
+    """The book would change once and the captured copies run at every replay, the first time behind whoever reads the pages."""
+    cache = PagedInt4Cache(1, 1, 8)
+    seqs, k, v = fill(cache, [70, 5, 70])
+    cache.free([seqs.pop(1)])
+    step, q = cache.extend(seqs, 0), vectors(2, 2, torch.float16, 3)
+    want = cache.attend(0, step, q)
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        graph.capture_begin()
+        try:
+            for call in (lambda: cache.fork(seqs), cache.compact):
+                with pytest.raises(RuntimeError, match="outside of the capture"):
+                    call()
+            out = cache.attend(0, step, q)
+        finally:
+            graph.capture_end()
+    assert len(cache._book.sequences) == 2 and cache.free_pages == 4
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    twins = cache.fork(seqs)
+    assert cache.compact() == 6
+    assert torch.equal(cache.attend(0, cache.extend(twins, 0), q), want)
+
+
+def test_a_capture_is_looked_for_on_the_cache_s_device(monkeypatch):
+    """The stream that counts is the current one of the cache's device, whichever device is current."""
+    import reskv_b200.paged as paged
+
+    seen = []
+
+    class On:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            seen.append(self.device)
+
+        def __exit__(self, *args):
+            seen.append(None)
+
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: bool(seen) and seen[-1] == torch.device("cuda", 1))
+    with pytest.raises(RuntimeError, match="outside of the capture"):
+        paged._refuse_capture(torch.device("cuda", 1))
+    paged._refuse_capture(torch.device("cuda", 0))
+    assert seen == [torch.device("cuda", 1), None, torch.device("cuda", 0), None]
