@@ -35,7 +35,7 @@ import torch.nn.functional as F
 from .._attention import attention
 from ..cache import ResKVLayerCache
 from ..config import ResKVKernelConfig
-from ..paged import PAGE_TOKENS, PagedInt4Cache
+from ..paged import MOST_GROUP, PAGE_TOKENS, PagedInt4Cache
 from ..prompt import prompt_attention
 
 try:  # dense baseline only: library flash-decoding kernel, if the image has it
@@ -150,6 +150,8 @@ class ResKVLlama:
             raise ValueError("cache must be 'reskv', 'dense' or 'int4'")
         if pages is not None and (cache != "int4" or type(pages) is not int or pages < 1):
             raise ValueError("pages is the size of the 4-bit cache's pool, a positive integer")
+        if cache == "int4" and shape.heads > MOST_GROUP * shape.kv_heads:
+            raise ValueError(f"the 4-bit cache takes up to {MOST_GROUP} query heads per KV head")
         self.pages = pages  # None: as many as the prompt and its reserve need
         self.shape, self.cache_kind, self.device = shape, cache, torch.device(device)
         self.kernel_config = kernel_config or ResKVKernelConfig()

@@ -23,6 +23,7 @@ import torch
 from ._extension import device_index_of, host, require_device
 
 PAGE_TOKENS = 64
+MOST_GROUP = 8  # query heads per KV head
 _PAGE_HEAD = (4, 2304)  # blocks of 16 tokens, bytes of a block
 _TYPES = (torch.float16, torch.bfloat16)
 

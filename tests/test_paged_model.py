@@ -334,3 +334,14 @@ def test_a_batch_without_rows():
         with pytest.raises(ValueError, match="no rows"):
             call()
     assert model.generate(ids, 3).shape == (2, 3)
+
+
+def test_more_query_heads_than_the_cache_takes_are_refused_at_the_start():
+    """The prompt's attention takes more, so that the first token behind a prompt would have been the first refusal."""
+    from reskv_b200.models import LlamaShape, ResKVLlama
+
+    with pytest.raises(ValueError, match="8 query heads per KV head"):
+        ResKVLlama(LlamaShape(**TINY | dict(heads=9, kv_heads=1)), cache="int4", device="cpu")
+    for heads in (8, 16):
+        ResKVLlama(LlamaShape(**TINY | dict(heads=heads)), cache="int4", device="cpu")
+    ResKVLlama(LlamaShape(**TINY | dict(heads=9, kv_heads=1)), cache="dense", device="cpu")
