@@ -752,6 +752,9 @@ extern "C" int reskv_paged_attention(const void* q, int bf16, int64_t q_sequence
     if (int rc = check_device_pointer(lengths, "paged_attention", "lengths")) return rc;
     if (int rc = check_device_pointer(workspace, "paged_attention", "workspace")) return rc;
     if (int rc = check_device_pointer(out, "paged_attention", "out")) return rc;
+    if (int rc = check_device_pointer(status, "paged_attention", "status")) return rc;
+    if (lse)
+        if (int rc = check_device_pointer(lse, "paged_attention", "lse")) return rc;
     if (width > 0) {
         if (int rc = check_device_pointer(table, "paged_attention", "table")) return rc;
         if (int rc = check_device_pointer(pages, "paged_attention", "pages")) return rc;

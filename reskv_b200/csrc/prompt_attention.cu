@@ -638,6 +638,8 @@ extern "C" int reskv_prompt_attention_reporting(const void* q, const void* k, co
     if (reinterpret_cast<uintptr_t>(out) & 31u) return fail(RESKV_ERR_INVALID, "prompt_attention: out must start on a 32-byte boundary");
     if (int rc = check_device_pointer(out, "prompt_attention", "out")) return rc;
     if (int rc = check_device_pointer(cu_seqlens, "prompt_attention", "cu_seqlens")) return rc;
+    if (lse)
+        if (int rc = check_device_pointer(lse, "prompt_attention", "lse")) return rc;
     if (status)
         if (int rc = check_device_pointer(status, "prompt_attention", "status")) return rc;
     PromptParams p{};
