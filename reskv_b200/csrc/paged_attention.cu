@@ -43,6 +43,7 @@ constexpr int kPaSmem = kPaWarps * kPaStages * kChunkBytes + kPaSumBytes;
 constexpr float kCodeMiddle = 8.f;
 constexpr uint32_t kMiddleLow = 0x80088008u, kMiddleByte = 0x80888088u;  // pairs of -8 * 2^-24 and -(8 + 16 * 8) * 2^-24
 constexpr int kPaSlack = 5;
+constexpr float kPaNear = 8192.f;                 // a maximum up to here has a rounding of 2^-12 at most
 constexpr int kPartialFloats = kPagedGroup * (kHeadDim + 2);  // of a part: outputs [8][128], maxima [8], sums [8]
 
 struct PagedParams {
@@ -369,9 +370,26 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
         // m may lag behind the maximum by kPaSlack powers of two: fewer rescalings.
         // It starts at the lowest finite number: scores of -infinity (BF16 offsets so large that their products leave FP32) have weights
         // of 0 then, where a maximum of -infinity would make them NaN.
-        constexpr float kNone = 3.402823466e38f;
-        float shift[2] = {kNone, kNone};  // unit_up - m * q_scale
+        constexpr float kNone = -3.402823466e38f;
+        float m[2] = {kNone, kNone};  // times q_scale
+        bool far = false;  // one of the warp's is far from 0
         float unit_up = 0.f, unit_limit = -1.f;
+        // Powers of the weights: s * q_scale - m + unit_up in one step where m is near 0, otherwise rounded in front of the subtraction, as
+        // m was: in one step the largest score's power would be m's rounding, 2^6 for scores of 2^30, and unit_up lost beside m.
+        const auto powers_of = [&](float(&power)[kChunkBlocks][4], const float(&s)[kChunkBlocks][4]) {
+            const float shift[2] = {unit_up - m[0], unit_up - m[1]};
+#pragma unroll
+            for (int b = 0; b < kChunkBlocks; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) power[b][i] = fmaf(s[b][i], q_scale[i & 1], shift[i & 1]);
+            if (far) {
+#pragma unroll
+                for (int b = 0; b < kChunkBlocks; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (fabsf(m[i & 1]) > kPaNear) power[b][i] = __fadd_rn(__fadd_rn(__fmul_rn(s[b][i], q_scale[i & 1]), -m[i & 1]), unit_up);
+            }
+        };
         float2 l = make_float2(0.f, 0.f), flat[2] = {l, l};
         float acc[8][4];  // rows = coordinates, columns = heads 2t, 2t + 1
 #pragma unroll
@@ -449,10 +467,11 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
                 }
             }
             float power[kChunkBlocks][4], highest = -INFINITY;
+            powers_of(power, s);
 #pragma unroll
             for (int b = 0; b < kChunkBlocks; ++b)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) power[b][i] = fmaf(s[b][i], q_scale[i & 1], shift[i & 1]), highest = fmaxf(highest, power[b][i]);
+                for (int i = 0; i < 4; ++i) highest = fmaxf(highest, power[b][i]);
             if (__any_sync(0xffffffffu, highest > unit_up + kPaSlack || most > unit_limit)) {
                 float top[2] = {fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])), fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]))};
 #pragma unroll
@@ -471,15 +490,13 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
                 float factor[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float before = unit_up - shift[h], next = fmaxf(before, top[h] * q_scale[h]);
-                    factor[h] = (before == next ? 1.f : fast_exp2(before - next)) * change;
-                    shift[h] = up - next;
+                    const float next = fmaxf(m[h], __fmul_rn(top[h], q_scale[h]));
+                    factor[h] = (m[h] == next ? 1.f : fast_exp2(m[h] - next)) * change;
+                    m[h] = next;
                 }
                 unit_up = up;
-#pragma unroll
-                for (int b = 0; b < kChunkBlocks; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) power[b][i] = fmaf(s[b][i], q_scale[i & 1], shift[i & 1]);
+                far = __any_sync(0xffffffffu, fmaxf(fabsf(m[0]), fabsf(m[1])) > kPaNear);
+                powers_of(power, s);
                 l.x *= factor[0], l.y *= factor[1];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) flat[i].x *= factor[0], flat[i].y *= factor[1];
@@ -562,7 +579,6 @@ __global__ void __launch_bounds__(kPaThreads, kPaPerSm) paged_attention_kernel(c
             return x;
         };
         l = over_tokens(l);
-        const float m[2] = {unit_up - shift[0], unit_up - shift[1]};
         if (g == 0) s_max[warp][2 * t] = m[0], s_max[warp][2 * t + 1] = m[1];
         ctas_sync();
         const int active = min(kPaWarps, end - at.first_chunk());

@@ -760,3 +760,38 @@ def test_a_capture_is_looked_for_on_the_cache_s_device(monkeypatch):
         paged._refuse_capture(torch.device("cuda", 1))
     paged._refuse_capture(torch.device("cuda", 0))
     assert seen == [torch.device("cuda", 1), None, torch.device("cuda", 0), None]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scaling", [2.0**-10, 128**-0.5, 1.0])
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 32000.0), (torch.bfloat16, 32000.0), (torch.bfloat16, 2.0**60)])
+@pytest.mark.parametrize("ratio", [3, 6])
+def test_scores_so_large_that_one_key_takes_all(ratio, dtype, size, scaling):
+    """Scores up to 2^30, 2^120: the largest one's weight is 1 (of several that are alike an equal share), the others' are 0, however
+    large the step of FP32 is there.  Value groups with scales far apart bring other units to the weights."""
+    cache = PagedInt4Cache(1, 1, 200, dtype=dtype)
+    seqs, lengths = cache.add(3), [40, 700, 3000]
+    places = torch.randperm(250, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV) - 125
+    k = torch.zeros(3740, 1, 128, dtype=dtype, device=DEV)
+    k[:, 0, 3] = places.repeat(15)[:3740].double().mul(size / 128).to(dtype)
+    v = vectors(3740, 1, dtype, 5) * torch.where(torch.arange(3740, device=DEV) % 7 == 0, 100.0, 0.01).to(dtype)[:, None, None]
+    step = cache.extend(seqs, lengths)
+    cache.write(0, step, k, v)
+    key = stored(k)[0].double().flatten(-2).to(DEV)
+    q = torch.zeros(3, ratio, 128, dtype=dtype, device=DEV)
+    q[..., 3] = size * torch.tensor([1.0, -1.0] * 4, device=DEV)[:ratio].to(dtype)
+    got, lse = cache.attend(0, step, q, scaling=scaling, return_lse=True)
+    u = torch.finfo(dtype).eps / 2
+    for i, (a, b) in enumerate(((0, 40), (40, 740), (740, 3740))):
+        low, scale, code = (x[a:b] for x in (stored(v)[2], stored(v)[1], stored(v)[3]))
+        value = (low.double() + scale.double() * code.double()).flatten(-2)[:, 0].to(DEV)
+        size_of = (low.double().abs() + scale.double() * code.double()).flatten(-2)[:, 0].to(DEV)
+        for h in range(ratio):
+            s = key[a:b, 0].double() @ q[i, h].double() * scaling
+            share = (s == s.max()).double() / (s == s.max()).sum()
+            want, terms = share @ value, share @ size_of
+            # as in `formula`, without an error of the scores
+            bound = u * want.abs() + (2.0**-11 + 2.0**-19) * terms + 2.0**-38 * (b - a) * terms.amax() + 2.0**-25
+            off = (got[i, h].double() - want).abs()
+            assert (off <= bound).all(), f"sequence {i}, head {h}: off by {off.max():.3e}, {(off - bound).max():.3e} too much"
+            assert (lse[i, h].double() - s.max()).abs() <= 2.0**-20 * s.max().abs() + 8
