@@ -55,6 +55,9 @@ __host__ __device__ constexpr uint32_t weight_column(int i) { return i * 128 + k
 __host__ __device__ constexpr uint32_t output_column(int i) { return 256 + i * 128; }
 static_assert(kPKeys + kPKeys / 2 <= 128 && kPKeys % 16 == 0, "scores and weights of a row tile share 128 columns");
 constexpr float kPSlack = 8.f;                  // the running maximum lags by at most this (in powers of two)
+// Where the maximum times the scale is beyond this, it is taken off the scores in front of the multiplication: the rounding of the
+// product (2^-12 here) would be the largest score's power, 2^6 for scores of 2^30.
+constexpr float kPNear = 8192.f;
 constexpr float kPLowest = -0x1.ffffp127f;      // the running maximum of a row whose scores have all been -infinity
 
 __device__ uint32_t g_prompt_status;  // RESKV_STATUS_* bits of calls without a word of their own
@@ -442,6 +445,7 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
             const int first_token = it.token0 + i * p.tile_tokens, token = first_token + row_token;
             const int limit = p.causal ? token : it.len - 1;  // last key that the row sees
             float m = 0.f, l = 0.f;
+            bool far = false;  // the maximum of one of the warp's rows is
             for (int j = 0; j < tiles; ++j) {
                 wait_once(lost, &sh.s_full[i], seen & 1);
                 tc_fence_after();
@@ -474,11 +478,13 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                 ++seen;
                 if (j == 0) {
                     m = max_nan(most, lowest);
+                    far = __any_sync(0xffffffffu, fabsf(m * scale) > kPNear);
                 } else {
                     const bool grows = !(most <= m + slack);
                     if (__any_sync(0xffffffffu, grows)) {
                         const float next = grows ? max_nan(m, most) : m, factor = grows ? fast_exp2((m - next) * scale) : 1.f;
                         m = next, l *= factor;
+                        far = __any_sync(0xffffffffu, fabsf(m * scale) > kPNear);
 #pragma unroll 1
                         for (int c = 0; c < 4; ++c) {
                             float o[32];
@@ -491,7 +497,16 @@ prompt_attention_kernel(const PromptParams p, const __grid_constant__ CUtensorMa
                     }
                 }
                 // an infinite maximum: inf - inf, NaN for the whole row as in the formula
-                const float shift = m == INFINITY ? __int_as_float(0x7fffffff) : -m * scale;
+                float shift = m == INFINITY ? __int_as_float(0x7fffffff) : -m * scale;
+                if (far) {
+                    const bool mine = fabsf(shift) > kPNear;
+                    const float off = mine ? m : 0.f;
+#pragma unroll
+                    for (int c = 0; c < kPChunks; ++c)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s[c][e] -= off;
+                    if (mine) shift = 0.f;
+                }
                 const float2 scales = make_float2(scale, scale), shifts = make_float2(shift, shift);
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll

@@ -406,3 +406,29 @@ def test_what_would_be_lost_without_a_word_is_refused():
     with torch.inference_mode():
         assert torch.equal(prompt_attention(q.clone(), k, v, cu), want)
     assert torch.equal(prompt_attention(torch._neg_view(-q), torch._neg_view(-k.contiguous()), v, cu), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scaling", [2.0**-10, 128**-0.5, 1.0])
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 32000.0), (torch.bfloat16, 32000.0), (torch.bfloat16, 2.0**60)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_so_large_that_one_key_takes_all(sign, dtype, size, scaling):
+    """Scores up to 2^30, 2^120: the largest one's distance to the next is thousands at least, so its weight is 1 (of two that are alike
+    a half each) and the others' are 0, however large the step of FP32 is there.  Weights and results are rounded once, an exponential
+    is off by 2^-13 at most (see ``formula``)."""
+    q, k, v, ends, cu = inputs([50, 300], 1, 4, dtype, seed=18)
+    q[..., :], k[..., :] = 0, 0
+    q[..., 3] = sign * size
+    places = torch.randperm(250, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV) - 125  # exact in either type
+    k[:, 0, 3] = torch.cat((places, places))[:350].double().mul(size / 128).to(dtype)
+    got, lse = prompt_attention(q, k, v, cu, scaling=scaling, return_lse=True)
+    for a, b in zip(ends, ends[1:]):
+        s = q[a:b, 0].double() @ k[a:b, 0].double().T * scaling
+        s = s.masked_fill(torch.ones_like(s, dtype=torch.bool).triu(1), -torch.inf)
+        best = s.amax(-1, keepdim=True)
+        share = (s == best).double() / (s == best).sum(-1, keepdim=True)
+        want, spread = share @ v[a:b, 0].double(), share @ v[a:b, 0].double().abs()
+        u = torch.finfo(dtype).eps / 2
+        for h in range(4):
+            assert_within(got[a:b, h], want, u * (spread + want.abs()) + 2 * spread * 2.0**-13)
+            assert ((lse[a:b, h].double() - best[:, 0]).abs() <= 2.0**-21 * best[:, 0].abs() + 1).all()
