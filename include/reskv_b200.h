@@ -439,7 +439,7 @@ int reskv_kmeans_incremental(const void* x, int batch, int kv_heads, int tokens,
                              int32_t* ids, void* stream);
 
 /* ---- attention over packed prompts ----------------------------------------------------------
- * What the model integrations do with a prompt before it is compressed (the reference attends with
+ * What a model does with a prompt before it is cached (the reference attends with
  * the framework's own attention, reskv/models/llama.py:25-170), for prompts of different lengths that
  * lie one behind the other: out[i,h] = sum_j softmax_j(q[i,h].k[j,g] * scaling) v[j,g] over the tokens j of
  * i's sequence, up to i itself if causal != 0; g = h / (q_heads / kv_heads), at most 128 query heads per
@@ -486,8 +486,9 @@ int reskv_prompt_attention_status(uint32_t* status, void* stream);
  * reskv_paged_read: the reverse, into dense [total, kv_heads, 128]; tokens of no sequence are left as they are.
  * reskv_paged_attention: one query per sequence, q [sequences, q_heads, 128] (strides q_sequence, q_head), up to
  * eight query heads per KV head, against tokens [0, lengths[s]) (clamped to the table); out [sequences, q_heads, 128]
- * dense, lse f32 [sequences, q_heads] or NULL; length 0 gives zeros and -infinity.  The workspace is the call's own
- * until it has run.
+ * dense, lse f32 [sequences, q_heads] or NULL; length 0 gives zeros and -infinity.  What FP32 holds on the way limits
+ * bf16 caches to keys up to 2^111 in magnitude and values up to 2^101 (NaN beyond); values' scales below 2^-60 lose bits.
+ * The workspace is the call's own until it has run.
  * reskv_copy_pages: pages src[i] -> dst[i] (HOST arrays) in each of `layers` pools that lie one behind the other,
  * page_bytes a multiple of 16; all at once, so no page may be a destination twice or both source and destination. */
 int reskv_paged_write(const void* k, const void* v, int bf16, int64_t k_token, int64_t k_head, int64_t v_token,

@@ -7,11 +7,11 @@
 //     sum p v   = sum_j (p_j scale_j,g) (code_j,g - 8) + sum_j p_j (offset_j,g + 8 scale_j,g)
 // with p * scale in FP16 as the product's operand, for FP16 models in two parts.
 //
-// 32 x 8128 tokens, 32 / 8 heads: 71 us for 300 MB, 4.2 TB/s (0.65 of the copy rate).  Bound by
-// instructions, 20 of a warp per token and KV head (issue slots 57 %, integer pipe 48 %: masks and shifts that bring the codes into
-// operands).  Small calls are bound by latency: one sequence of 300 tokens 7.0 us, of 8128 10.6 us, nine ragged BF16 ones with eight
-// query heads 16 us (28 MB), of which two dependent launches, look-ups of lengths and pages, a copy, a chunk, two meetings of the
-// warps and the merge follow one another.
+// 32 x 8128 tokens, 32 / 8 heads: 71 us for 300 MB, 4.2 TB/s (0.65 of the copy rate).  Neither bytes nor issue slots (57 %) nor a pipe
+// (integer 48 %: masks and shifts that bring the codes into operands) are full: 20 instructions of a warp per token and KV head, most of
+// them in chains, and the registers leave 16 warps an SM to cover them.  Small calls are bound by latency: one sequence of 300 tokens
+// 6.9 us, of 8128 10.4 us, nine ragged BF16 ones with eight query heads 16 us (28 MB), of which two dependent launches, look-ups of
+// lengths and pages, a copy, a chunk, two meetings of the warps and the merge follow one another.
 //
 // Work: the pages of all (sequence, KV head) units lie end to end and every CTA takes an equal share; a unit that lies in one
 // CTA is finished there, the parts of the others are added by a second kernel.  Eight warps take a segment's chunks of 32 tokens

@@ -2,13 +2,13 @@
 //
 // Storing: of a token's vector of one head, every group of 64 coordinates becomes offset = min, scale = (max - min) / 15
 // rounded to the model's type, code = round((x - offset) / scale) to the nearest, ties to even, at most 15 (0 where the scale
-// is 0).  512 bytes of K and V become 144.  Bound by bytes, and close to that by instructions.  Four lanes hold a row of one side,
+// is 0).  512 bytes of K and V become 144.  Four lanes hold a row of one side,
 // sixteen coordinates of either group each, eight rows (K and V of four heads) to a warp; a lane's words of a key row are then 16
 // bytes in a row of their own.  Extremes of both groups travel together as 16-bit pairs.  A warp looks up by itself where its tokens
 // go, while their rows are on the way.
 //
-// 8 x 4000 tokens, 8 heads: written in 36 us (168 MB, 4.7 TB/s, 0.72 of the copy rate), read back in 30 us (5.6 TB/s, 0.87); 65 % of the
-// issue slots are taken.  Loads that ask to leave L2 first: 34.6 us, but attention over the prompt reads the same rows.
+// 8 x 4000 tokens, 8 heads: written in 36 us (168 MB, 4.7 TB/s, 0.72 of the copy rate), read back in 30 us (5.6 TB/s, 0.87); 65 and 59 % of
+// the issue slots are taken: writing is bound by neither alone, reading nearly by bytes.  Loads that ask to leave L2 first: 34.6 us, but attention over the prompt reads the same rows.
 // Eight lanes to a row: 46 and 32 us, sixteen: 91 and 51 us.  Ties and what is near them left to the division: 2 us more, with six BF16
 // prompts of 4546 tokens 11 us for 7.9.  Places looked up by a few threads for the block: 0.2 to 0.9 us more on small calls.
 #include <algorithm>

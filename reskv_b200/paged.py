@@ -220,7 +220,8 @@ class PagedInt4Cache:
         """One query per sequence of the step, ``[sequences, H, 128]`` after RoPE, against all of its tokens; ``H`` is up to
         eight times the KV heads, ``scaling`` (positive) defaults to ``128**-0.5``.  Returns ``[sequences, H, 128]``, with
         ``return_lse`` also FP32 ``[sequences, H]``, the logarithm of the sum of exponentials.  A sequence without tokens gets
-        zeros (and minus infinity)."""
+        zeros (and minus infinity).  In a BF16 cache keys up to ``2**111`` and values up to ``2**101`` in magnitude can be
+        attended to (NaN beyond); scales of values below ``2**-60`` lose bits."""
         self._check(step)
         if isinstance(query, torch.Tensor) and query.dtype != self.dtype:
             raise ValueError(f"query must be {self.dtype}")

@@ -1,8 +1,9 @@
 """Attention over whole prompts of different lengths, packed one behind the other.
 
-The model integrations attend to a prompt before its keys and values are compressed.  ``prompt_attention`` is that step for
-packed batches: tensors ``[tokens, heads, 128]`` without padding, ``cu_seqlens`` saying where each sequence starts and ends.
-The kernel is ``csrc/prompt_attention.cu``.
+A model attends to a prompt before its keys and values go into a cache.  ``prompt_attention`` is that step for batches whose prompts
+differ in length: tensors ``[tokens, heads, 128]`` without padding, ``cu_seqlens`` saying where each sequence starts and ends.
+``ResKVLlama(cache="int4")`` calls it; the models with a compressed or dense cache have one length per batch and use the library's
+attention for the prompt.  The kernel is ``csrc/prompt_attention.cu``.
 """
 
 from __future__ import annotations
@@ -35,7 +36,7 @@ def prompt_attention(
     Returns ``[T,H,128]`` of the query's type, written to ``out`` if that is given (contiguous, not overlapping the inputs);
     with ``return_lse`` also FP32 ``[T,H]``, the natural logarithm of each row's sum of exponentials.  Rows that belong to no
     sequence are not written.  Scores, sums and products are FP32, the weights are rounded once to the type of ``value`` for
-    the product with it.  Infinities and NaN count only where they are attended to.  Inference only: tensors that ask for
+    the product with it.  A row whose scores are all minus infinity has no weights: NaN, with a logarithm of minus infinity.  Infinities and NaN count only where they are attended to.  Inference only: tensors that ask for
     a gradient, carry a tangent, are no plain tensors (subclasses, vmap) or are being traced are refused.
 
     ``status``, an int32 tensor on the device (``PagedInt4Cache.status``, whose ``check()`` then speaks for this call too), gets a

@@ -795,3 +795,21 @@ def test_scores_so_large_that_one_key_takes_all(ratio, dtype, size, scaling):
             off = (got[i, h].double() - want).abs()
             assert (off <= bound).all(), f"sequence {i}, head {h}: off by {off.max():.3e}, {(off - bound).max():.3e} too much"
             assert (lse[i, h].double() - s.max()).abs() <= 2.0**-20 * s.max().abs() + 8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("key_power,value_power", [(0, -57), (0, 98), (108, 0), (108, 98), (-100, 0)])
+def test_bf16_at_the_ends_of_its_range(key_power, value_power):
+    """The largest keys (2^111) and values (2^101) and the finest scales (2^-60) that are promised."""
+    dtype = torch.bfloat16
+    cache = PagedInt4Cache(1, 1, 20, dtype=dtype)
+    seqs, lengths = cache.add(2), [500, 90]
+    k = [vectors(t, 1, torch.float32, i).clamp(-8, 8).double().mul(2.0**key_power).to(dtype) for i, t in enumerate(lengths)]
+    v = [vectors(t, 1, torch.float32, 5 + i).clamp(-8, 8).double().mul(2.0**value_power).to(dtype) for i, t in enumerate(lengths)]
+    cache.write(0, cache.extend(seqs, lengths), torch.cat(k), torch.cat(v))
+    q = vectors(2, 4, dtype, 6)
+    scaling = 0.1 * 2.0**-key_power
+    got = cache.attend(0, cache.extend(seqs, 0), q, scaling=scaling)
+    for i in range(2):
+        want, _, bound = formula(q[i], k[i], v[i], scaling)
+        assert ((got[i].double() - want).abs() <= bound - 2.0**-25).all()  # without the part that is not relative to the values
