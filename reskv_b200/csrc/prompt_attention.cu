@@ -17,12 +17,12 @@
 // infinities or NaN in rows of V that only part of a row tile sees are cleared there too and added where they are seen.
 //
 // Bound (1 x 8192 tokens, 32 / 8 heads, 550 GFLOP): 460 us = 1.20 PFLOP/s in short runs, 521 to 531 us = 1.05 PFLOP/s in long ones under
-// the power cap; seven ragged prompts of 84 GFLOP 101 us in short runs, 108 with cold inputs, five short ones of 0.9 GFLOP 13 us.  A row
-// tile's softmax is what takes longest: 2070 cycles per tile of 80 keys, of them 1230 forming weights (16 exponentials per clock and SM, two row tiles: 1280 for
-// both), 180 and 280 waiting for scores and for the product in front, 150 the maximum; per item another 1300 waiting for the last
-// product, 2300 storing, 1000 until the first scores.  (Without the way for scores far from 0 454 and 517 us, 99 and 107.)  An item has
-// all keys of its rows, so a call of few items takes as long as its longest one: one sequence of 2000 tokens with one head keeps 16 SMs
-// busy.  What was measured besides, on 1 x 8192 in short runs of the form that took 449 us:
+// the power cap; seven ragged prompts of 84 GFLOP 101 us in short runs, 108 with cold inputs, five short ones of 0.9 GFLOP 13 us.  (Without
+// the way for scores far from 0 454 and 517 us, 99 and 107.)  A row tile's softmax is what takes longest: 2070 cycles per tile of 80
+// keys, of them 1230 forming weights (16 exponentials per clock and SM, two row tiles: 1280 for both), 180 and 280 waiting for scores
+// and for the product in front, 150 the maximum; per item another 1300 waiting for the last product, 2300 storing, 1000 until the first
+// scores.  An item has all keys of its rows, so a call of few items takes as long as its longest one: one sequence of 2000 tokens with
+// one head keeps 16 SMs busy, 31 us.  What was measured besides, on 1 x 8192 in short runs of the form that took 449 us:
 //   128 keys a tile, weights in the scores' place, one warp for both products, ring of five: 463 us (seven ragged: 100 us)
 //   a quarter of the exponentials by a polynomial: 447 us, not worth its code; a half: no faster
 //   two threads per row (16 softmax warps): 502 us
