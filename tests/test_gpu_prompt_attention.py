@@ -432,3 +432,16 @@ def test_scores_so_large_that_one_key_takes_all(sign, dtype, size, scaling):
         for h in range(4):
             assert_within(got[a:b, h], want, u * (spread + want.abs()) + 2 * spread * 2.0**-13)
             assert ((lse[a:b, h].double() - best[:, 0]).abs() <= 2.0**-21 * best[:, 0].abs() + 1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ratio", [3, 5, 7, 12, 40])
+def test_what_an_earlier_call_left_on_the_chip_does_not_matter(ratio):
+    """128 rows are no multiple of these groups; the rows beyond them hold what was there."""
+    q, k, v, ends, cu = inputs([300, 90], 2, ratio, torch.float16, seed=19)
+    want = prompt_attention(q, k, v, cu)
+    assert_within(want, *formula(q, k, v, ends)[::2])
+    for left in (float("nan"), float("inf"), 60000.0):
+        y = torch.full((3000, 8, 128), left, dtype=torch.float16, device=DEV)
+        prompt_attention(y, y, y, torch.arange(0, 3001, 20, dtype=torch.int32, device=DEV))  # a block or more on every SM
+        assert torch.equal(prompt_attention(q, k, v, cu), want)
